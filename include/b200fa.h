@@ -152,6 +152,32 @@ void b200fa_dropout_bytes_host(uint64_t philox_seed, uint64_t philox_offset, int
                                int64_t col_block, uint8_t* out16);
 
 /*
+ * Attention over a window of keys and the first ones ("sinks"), forward and backward.  `causal` is
+ * B200FA_CAUSAL_TOP_LEFT or B200FA_CAUSAL_BOTTOM_RIGHT; with p the last key that the diagonal lets a query row see
+ * (i, or i + Sk - Sq), the row sees key j iff j <= p and (j > p - window or j < sinks).  window >= 1, sinks >= 0; a window of
+ * Sk + Sq keys is the causal mask.  Otherwise the contracts of b200fa_fwd and b200fa_bwd: out, lse, gradients, types,
+ * lengths, strides, rows that see no key.  Work goes with the keys that are seen: blocks of 128 keys that no row of a
+ * tile sees are not visited.  Blocks that are visited have to hold finite values of v also where the mask hides them (0 * inf
+ * is NaN in every kernel that multiplies whole tiles).  bf16 and fp16 run the tcgen05 kernels; fp32 runs FMA kernels, both
+ * directions, so that a forward's out and lse fit the backward.
+ * `workspace` of the backward: b200fa_window_bwd_workspace_bytes(...) bytes of caller-owned device scratch, 256-byte aligned,
+ * contents irrelevant (the row statistics of b200fa_bwd and, where the query rows of a K/V tile with sinks in it are shared
+ * by several blocks, their fp32 sums); calls that overlap on the GPU need workspaces of their own.  No counterpart in the
+ * reference, whose kernels carry an unreachable window argument
+ * (torch_mojo_backend/eager_flash_attention/fa4_fwd_common.mojo:26-29).
+ */
+int b200fa_window_fwd(const b200fa_tensor4* q, const b200fa_tensor4* k, const b200fa_tensor4* v,
+                      const b200fa_tensor4* out, float* lse, int dtype, int causal, int64_t window, int64_t sinks,
+                      float scale, void* stream, int device, uint32_t* status_word);
+size_t b200fa_window_bwd_workspace_bytes(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t seqlen_q,
+                                         int64_t seqlen_k, int64_t head_dim, int dtype, int64_t window, int64_t sinks);
+int b200fa_window_bwd(const b200fa_tensor4* q, const b200fa_tensor4* k, const b200fa_tensor4* v,
+                      const b200fa_tensor4* out, const b200fa_tensor4* dout, const float* lse,
+                      const b200fa_tensor4* dq, const b200fa_tensor4* dk, const b200fa_tensor4* dv, void* workspace,
+                      size_t workspace_bytes, int dtype, int causal, int64_t window, int64_t sinks, float scale,
+                      void* stream, int device, uint32_t* status_word);
+
+/*
  * Forward for short query blocks against a long key/value sequence (decode): the key sequence
  * is split over many thread blocks, each streams its share of K and V once for every query
  * head of the GQA group and every query row.  Few splits form a cluster that merges the partial

@@ -52,6 +52,9 @@ EXPORTED_SYMBOLS = (
     "b200fa_fwd_splitkv",
     "b200fa_fwd_splitkv_piece_workspace_bytes",
     "b200fa_fwd_splitkv_piece",
+    "b200fa_window_fwd",
+    "b200fa_window_bwd_workspace_bytes",
+    "b200fa_window_bwd",
     "b200fa_set_wait_budget",
     "b200fa_wait_budget",
     "b200fa_set_fwd_tiles",
@@ -135,6 +138,12 @@ def load() -> ctypes.CDLL:
     lib.b200fa_fwd_dropout.restype = ctypes.c_int
     lib.b200fa_bwd_dropout.argtypes = bwd_args[:14] + drop_args + bwd_args[14:]
     lib.b200fa_bwd_dropout.restype = ctypes.c_int
+    lib.b200fa_window_fwd.argtypes = fwd_args[:7] + [ctypes.c_int64] * 2 + fwd_args[7:]
+    lib.b200fa_window_fwd.restype = ctypes.c_int
+    lib.b200fa_window_bwd.argtypes = bwd_args[:13] + [ctypes.c_int64] * 2 + bwd_args[13:]
+    lib.b200fa_window_bwd.restype = ctypes.c_int
+    lib.b200fa_window_bwd_workspace_bytes.argtypes = [ctypes.c_int64] * 6 + [ctypes.c_int] + [ctypes.c_int64] * 2
+    lib.b200fa_window_bwd_workspace_bytes.restype = ctypes.c_size_t
     lib.b200fa_dropout_threshold.argtypes = [ctypes.c_float]
     lib.b200fa_dropout_threshold.restype = ctypes.c_uint32
     lib.b200fa_dropout_bytes_host.argtypes = [ctypes.c_uint64, ctypes.c_uint64, ctypes.c_int64, ctypes.c_int64,
@@ -238,6 +247,27 @@ def bwd(q: Tensor4, k: Tensor4, v: Tensor4, out: Tensor4, dout: Tensor4, lse_ptr
         return load().b200fa_bwd_parts(*head, *tail, parts)
     fn = load().b200fa_bwd_simt if simt else load().b200fa_bwd
     return fn(*head, *tail)
+
+
+def window_fwd(q: Tensor4, k: Tensor4, v: Tensor4, out: Tensor4, lse_ptr: int, dtype: int, causal, window: int, sinks: int,
+               scale: float, stream: int, device: int, status_ptr: int = 0) -> int:
+    """Raw forward over a window of keys and the first ones (see b200fa_window_fwd); returns the library's status code."""
+    return load().b200fa_window_fwd(ctypes.byref(q), ctypes.byref(k), ctypes.byref(v), ctypes.byref(out), lse_ptr, dtype,
+                                    causal_code(causal), window, sinks, scale, stream, device, status_ptr)
+
+
+def window_bwd_workspace_bytes(B: int, Hq: int, Hkv: int, Sq: int, Sk: int, D: int, dtype: int, window: int, sinks: int) -> int:
+    return int(load().b200fa_window_bwd_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, dtype, window, sinks))
+
+
+def window_bwd(q: Tensor4, k: Tensor4, v: Tensor4, out: Tensor4, dout: Tensor4, lse_ptr: int, dq: Tensor4, dk: Tensor4,
+               dv: Tensor4, workspace_ptr: int, workspace_bytes: int, dtype: int, causal, window: int, sinks: int, scale: float,
+               stream: int, device: int, status_ptr: int = 0) -> int:
+    """Raw backward of `window_fwd`; returns the library's status code."""
+    return load().b200fa_window_bwd(
+        ctypes.byref(q), ctypes.byref(k), ctypes.byref(v), ctypes.byref(out), ctypes.byref(dout), lse_ptr, ctypes.byref(dq),
+        ctypes.byref(dk), ctypes.byref(dv), workspace_ptr, workspace_bytes, dtype, causal_code(causal), window, sinks, scale,
+        stream, device, status_ptr)
 
 
 def fwd_splitkv_workspace_bytes(B: int, Hq: int, Hkv: int, Sq: int, Sk: int, D: int, whole_heads: int = 0) -> int:

@@ -142,6 +142,8 @@ int check_device_is_sm100(int device) {
   return cached[device] == 1 ? B200FA_OK : B200FA_ERR_UNSUPPORTED;
 }
 
+constexpr int64_t kMaxWindow = 1 << 25;   // longer than any sequence and, at bottom-right alignment, its distance to position 0
+
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 }  // namespace
@@ -204,7 +206,18 @@ struct Options {
   float dropout_p = 0.f;
   uint64_t seed = 0, offset = 0;
   int64_t whole_heads = 0;   // 0: the call is a whole problem
+  bool windowed = false;     // `window` and `sinks` are given
+  int64_t window = 0, sinks = 0;
 };
+
+// Checks a window and its sinks; more keys than a sequence can have are as good as all of it.
+int window_params(const Options& opt, int causal, int* window, int* sinks) {
+  if (!opt.windowed) return B200FA_OK;
+  if (causal == B200FA_CAUSAL_NONE || opt.window <= 0 || opt.sinks < 0) return B200FA_ERR_UNSUPPORTED;
+  *window = static_cast<int>(std::min<int64_t>(opt.window, kMaxWindow));
+  *sinks = static_cast<int>(std::min<int64_t>(opt.sinks, kMaxWindow));
+  return B200FA_OK;
+}
 
 // causal argument -> (flag, diagonal offset); false if it is not one of the three modes
 bool causal_mode(int causal, int64_t Sq, int64_t Sk, int* flag, int* off) {
@@ -244,6 +257,7 @@ int fwd_impl(const b200fa_tensor4* q, const b200fa_tensor4* k, const b200fa_tens
   if (!dropout_params(opt.dropout_p, opt.seed, opt.offset, &p.drop)) return B200FA_ERR_UNSUPPORTED;
   if (reinterpret_cast<uintptr_t>(lse) % 4 != 0) return B200FA_ERR_MISALIGNED;
   int rc;
+  if ((rc = window_params(opt, causal, &p.window, &p.sinks)) != B200FA_OK) return rc;
   if ((rc = check_view(q, B, Hq, Sq, D, dtype, &p.q)) != B200FA_OK) return rc;
   if ((rc = check_view(k, B, Hkv, Sk, D, dtype, &p.k)) != B200FA_OK) return rc;
   if ((rc = check_view(v, B, Hkv, Sk, D, dtype, &p.v)) != B200FA_OK) return rc;
@@ -255,7 +269,7 @@ int fwd_impl(const b200fa_tensor4* q, const b200fa_tensor4* k, const b200fa_tens
   p.scale_log2 = scale * 1.4426950408889634f;
   p.status = status_word;
   p.whole_heads = opt.whole_heads > 0 ? opt.whole_heads : B * Hq;
-  p.tiles_per_cta = fwd_tiles();
+  p.tiles_per_cta = p.window ? 0 : fwd_tiles();
   p.wait_budget = wait_budget();
 
   DeviceGuard guard(device);
@@ -268,7 +282,7 @@ int fwd_impl(const b200fa_tensor4* q, const b200fa_tensor4* k, const b200fa_tens
   // A stale error left on this thread by an earlier, unrelated runtime call must not be
   // mistaken for a launch failure.
   (void)cudaGetLastError();
-  cudaError_t e = opt.force_simt ? launch_fwd_simt(p, dtype, static_cast<cudaStream_t>(stream), &launches)
+  cudaError_t e = opt.force_simt || (dtype == kF32 && p.window) ? launch_fwd_simt(p, dtype, static_cast<cudaStream_t>(stream), &launches)
                   : dtype == kF32 ? launch_fwd_fp32(p, static_cast<cudaStream_t>(stream), &launches)
                                   : launch_fwd_sm100(p, dtype, static_cast<cudaStream_t>(stream), &launches);
   g_launches += launches;
@@ -296,6 +310,7 @@ int bwd_impl(const b200fa_tensor4* q, const b200fa_tensor4* k, const b200fa_tens
   if (!(scale > 0.f) || !std::isfinite(scale)) return B200FA_ERR_UNSUPPORTED;
   if (!dropout_params(opt.dropout_p, opt.seed, opt.offset, &p.drop)) return B200FA_ERR_UNSUPPORTED;
   int rc;
+  if ((rc = window_params(opt, causal, &p.window, &p.sinks)) != B200FA_OK) return rc;
   if ((rc = check_view(q, B, Hq, S, D, dtype, &p.q)) != B200FA_OK) return rc;
   if ((rc = check_view(k, B, Hkv, Sk, D, dtype, &p.k)) != B200FA_OK) return rc;
   if ((rc = check_view(v, B, Hkv, Sk, D, dtype, &p.v)) != B200FA_OK) return rc;
@@ -304,7 +319,8 @@ int bwd_impl(const b200fa_tensor4* q, const b200fa_tensor4* k, const b200fa_tens
   if ((rc = check_view(dq, B, Hq, S, D, dtype, &p.dq, true)) != B200FA_OK) return rc;
   if ((rc = check_view(dk, B, Hkv, Sk, D, dtype, &p.dk, true)) != B200FA_OK) return rc;
   if ((rc = check_view(dv, B, Hkv, Sk, D, dtype, &p.dv, true)) != B200FA_OK) return rc;
-  const size_t need = b200fa_bwd_workspace_bytes(B, Hq, Hkv, S, D, dtype);
+  const size_t statistics = b200fa_bwd_workspace_bytes(B, Hq, Hkv, S, D, dtype);
+  const size_t need = p.window ? b200fa_window_bwd_workspace_bytes(B, Hq, Hkv, S, Sk, D, dtype, p.window, p.sinks) : statistics;
   if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
     return B200FA_ERR_WORKSPACE;
   const size_t spad = static_cast<size_t>((S + 127) / 128 * 128);
@@ -320,6 +336,8 @@ int bwd_impl(const b200fa_tensor4* q, const b200fa_tensor4* k, const b200fa_tens
   p.status = status_word;
   p.wait_budget = wait_budget();
   p.parts = opt.parts;
+  p.sink_chunks = p.window && dtype != kF32 ? bwd_sink_chunks(p) : 1;
+  p.sink_part = reinterpret_cast<float*>(ws + statistics);
 
   DeviceGuard guard(device);
   if (!guard.ok) {
@@ -329,7 +347,7 @@ int bwd_impl(const b200fa_tensor4* q, const b200fa_tensor4* k, const b200fa_tens
   if ((rc = check_device_is_sm100(device)) != B200FA_OK) return rc;
   int launches = 0;
   (void)cudaGetLastError();
-  cudaError_t e = opt.force_simt || (dtype == kF32 && D != 64)
+  cudaError_t e = opt.force_simt || (dtype == kF32 && (D != 64 || p.window))
                       ? launch_bwd_simt(p, dtype, static_cast<cudaStream_t>(stream), &launches)
                   : dtype == kF32 ? launch_bwd_fp32(p, static_cast<cudaStream_t>(stream), &launches)
                                   : launch_bwd_sm100(p, dtype, static_cast<cudaStream_t>(stream), &launches);
@@ -533,6 +551,46 @@ int b200fa_bwd_simt(const b200fa_tensor4* q, const b200fa_tensor4* k, const b200
                     uint32_t* status_word) {
   Options opt;
   opt.force_simt = true;
+  return bwd_impl(q, k, v, out, dout, lse, dq, dk, dv, workspace, workspace_bytes, dtype, causal, scale, stream,
+                  device, status_word, opt);
+}
+
+int b200fa_window_fwd(const b200fa_tensor4* q, const b200fa_tensor4* k, const b200fa_tensor4* v,
+                      const b200fa_tensor4* out, float* lse, int dtype, int causal, int64_t window, int64_t sinks,
+                      float scale, void* stream, int device, uint32_t* status_word) {
+  Options opt;
+  opt.windowed = true;
+  opt.window = window;
+  opt.sinks = sinks;
+  return fwd_impl(q, k, v, out, lse, dtype, causal, scale, stream, device, status_word, opt);
+}
+
+size_t b200fa_window_bwd_workspace_bytes(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t seqlen_q,
+                                         int64_t seqlen_k, int64_t head_dim, int dtype, int64_t window, int64_t sinks) {
+  if (heads_kv <= 0 || heads_q < heads_kv || seqlen_k <= 0 || window <= 0 || sinks < 0) return 0;
+  const size_t statistics = b200fa_bwd_workspace_bytes(batch, heads_q, heads_kv, seqlen_q, head_dim, dtype);
+  if (statistics == 0 || dtype == kF32 || batch > 65535 || heads_q > 65535 || seqlen_q > (1 << 24) || seqlen_k > (1 << 24)) return statistics;
+  BwdParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.B = static_cast<int>(batch); p.Hq = static_cast<int>(heads_q); p.Hkv = static_cast<int>(heads_kv);
+  p.S = static_cast<int>(seqlen_q); p.Sk = static_cast<int>(seqlen_k);
+  p.window = static_cast<int>(std::min(window, kMaxWindow));
+  p.sinks = static_cast<int>(std::min(sinks, kMaxWindow));
+  const int64_t chunks = bwd_sink_chunks(p);
+  if (chunks <= 1) return statistics;
+  const int64_t tiles = std::min<int64_t>((seqlen_k + 127) / 128, (p.sinks + 127) / 128);
+  return statistics + static_cast<size_t>(batch * heads_kv * tiles * chunks * 2 * 128 * head_dim) * 4;
+}
+
+int b200fa_window_bwd(const b200fa_tensor4* q, const b200fa_tensor4* k, const b200fa_tensor4* v,
+                      const b200fa_tensor4* out, const b200fa_tensor4* dout, const float* lse,
+                      const b200fa_tensor4* dq, const b200fa_tensor4* dk, const b200fa_tensor4* dv, void* workspace,
+                      size_t workspace_bytes, int dtype, int causal, int64_t window, int64_t sinks, float scale,
+                      void* stream, int device, uint32_t* status_word) {
+  Options opt;
+  opt.windowed = true;
+  opt.window = window;
+  opt.sinks = sinks;
   return bwd_impl(q, k, v, out, dout, lse, dq, dk, dv, workspace, workspace_bytes, dtype, causal, scale, stream,
                   device, status_word, opt);
 }

@@ -22,6 +22,7 @@
 // dK/dV kernel: warps 0-15 are four compute warpgroups that split the 128 score columns of a tile in
 // quarters (thread <-> TMEM lane), warp 16 issues every MMA, warp 17 drives TMA.  dQ kernel: warps 0-3 and
 // 4-7 split the columns in halves, warps 8 and 9 each issue one of two independent MMA chains, warp 10 drives TMA.
+#include <algorithm>
 #include <mutex>
 
 #include "common.cuh"
@@ -68,13 +69,16 @@ __device__ __forceinline__ float2 exp2_mufu2(float2 x) { return make_float2(ex2_
 // TMEM columns: two work buffers of 128, in turn: S^T of a step, over which 16-bit P^T and dS^T go (the A operands of the
 // dV and dK MMAs); then the dV and dK accumulators; dP^T at D = 64 in a third buffer, at D = 128 in the other step's.
 // ------------------------------------------------------------------------------------------
-template <int kD, bool kBf16, bool kCausal, bool kDropout>
+// Under a window a K/V tile with sinks in it is seen by every later query row, all others by those of a window.  Its steps are
+// dealt to sink_chunks blocks, which leave fp32 sums for sink_sum_kernel to add up (bwd_sink_chunks says when).
+template <int kD, bool kBf16, int kMask, bool kDropout>
 __global__ void __launch_bounds__(kDkdvThreads, 1)
 bwd_dkdv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
                 const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapDO,
                 const __grid_constant__ CUtensorMap mapDK, const __grid_constant__ CUtensorMap mapDV,
                 const BwdParams p, const int sched_group) {
   using Cfg = BwdCfg<kD>;
+  constexpr bool kCausal = kMask != kAll, kWindow = kMask == kWindowMask;
   // TMEM: two 128-column work buffers (step i has S^T in buffer i & 1, then P^T and dS^T, 16-bit, in its place),
   // the dV and dK accumulators, and at D = 64 a third buffer for dP^T; at D = 128 dP^T is in the other step's buffer.
   constexpr bool kOwnDp = kD == 64;
@@ -113,9 +117,11 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant_
   const int m_tiles = (p.S + kTile - 1) / kTile;      // query tiles
   const int n_tiles = (p.Sk + kTile - 1) / kTile;     // K/V tiles (== m_tiles when causal)
   int n_tile, hk, b;
+  int chunk = 0, chunks = 1;                          // of this tile's steps
+  const int sink_tiles = kWindow ? min(n_tiles, (p.sinks + kTile - 1) / kTile) : 0;
   {
     const int pairs = p.B * p.Hkv;
-    const int per_group = sched_group * n_tiles;
+    const int per_group = sched_group * (kWindow ? n_tiles + sink_tiles * (p.sink_chunks - 1) : n_tiles);
     const int g = static_cast<int>(blockIdx.x) / per_group;
     const int gsize = min(sched_group, pairs - g * sched_group);
     const int within = static_cast<int>(blockIdx.x) - g * per_group;
@@ -123,14 +129,30 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant_
     const int pair = g * sched_group + within % gsize;
     b = pair / p.Hkv;
     hk = pair - b * p.Hkv;
+    if constexpr (kWindow) {
+      if (n_tile < sink_tiles * p.sink_chunks) {
+        chunks = p.sink_chunks;
+        chunk = n_tile % chunks;
+        n_tile /= chunks;
+      } else {
+        n_tile -= sink_tiles * (p.sink_chunks - 1);
+      }
+    }
   }
   const int group = p.Hq / p.Hkv;
   const int n0 = n_tile * kTile;
   // query row i sees key column j iff j <= i + causal_off: the first query tile with a row that
   // sees a key of this tile (none: the tile's dK and dV are zero)
   const int m_start = kCausal ? min(m_tiles, max(0, n0 - p.causal_off) / kTile) : 0;
-  const int per_head = m_tiles - m_start;
-  const int steps = group * per_head;
+  int m_end = m_tiles;
+  if constexpr (kWindow) {   // the last row whose window reaches the tile's last key
+    const int last = min(n0 + kTile, p.Sk) - 1 + p.window - 1 - p.causal_off;
+    if (n0 >= p.sinks) m_end = max(m_start, last < 0 ? 0 : min(m_tiles, last / kTile + 1));
+  }
+  const int per_head = m_end - m_start;
+  const int all_steps = group * per_head;
+  const int step0 = kWindow ? static_cast<int>(static_cast<int64_t>(all_steps) * chunk / chunks) : 0;   // this block's first
+  const int steps = kWindow ? static_cast<int>(static_cast<int64_t>(all_steps) * (chunk + 1) / chunks) - step0 : all_steps;
 
   // A launch whose status word already reports a failed wait is not worth running; the swizzled
   // tiles assume a 1024-byte aligned shared-memory window.
@@ -153,15 +175,15 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant_
   auto load_q = [&](int i) {
     const int stage = i % Cfg::kQStages;
     mbar_arrive_expect_tx(&q_full[stage], Cfg::kTileBytes);
-    load_tile(&mapQ, sQ + stage * Cfg::kTileBytes, &q_full[stage], (m_start + i % per_head) * kTile, hk * group + i / per_head);
+    load_tile(&mapQ, sQ + stage * Cfg::kTileBytes, &q_full[stage], (m_start + (step0 + i) % per_head) * kTile, hk * group + (step0 + i) / per_head);
   };
   auto load_do = [&](int i) {
     const int stage = i % Cfg::kDoStages;
     mbar_arrive_expect_tx(&do_full[stage], Cfg::kTileBytes);
-    load_tile(&mapDO, sDO + stage * Cfg::kTileBytes, &do_full[stage], (m_start + i % per_head) * kTile, hk * group + i / per_head);
+    load_tile(&mapDO, sDO + stage * Cfg::kTileBytes, &do_full[stage], (m_start + (step0 + i) % per_head) * kTile, hk * group + (step0 + i) / per_head);
   };
   auto load_stat = [&](int i) {
-    const int64_t off = (static_cast<int64_t>(b) * p.Hq + hk * group + i / per_head) * p.Spad + (m_start + i % per_head) * kTile;
+    const int64_t off = (static_cast<int64_t>(b) * p.Hq + hk * group + (step0 + i) / per_head) * p.Spad + (m_start + (step0 + i) % per_head) * kTile;
     float* st = sStat + (i & 1) * 256;
     mbar_arrive_expect_tx(&stat_full[i & 1], 1024);
     bulk_load_1d(st, p.lse_log2 + off, 512, &stat_full[i & 1]);
@@ -226,7 +248,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant_
     const uint32_t tWork = tmem_base + lane_off + kTmemWork + wg * 32;
     const float c = p.scale_log2;
     for (int i = 0; i < steps; ++i) {
-      const int m_tile = m_start + i % per_head;
+      const int m_tile = m_start + (step0 + i) % per_head;
       const float4* lse2 = reinterpret_cast<const float4*>(sStat + (i & 1) * 256 + wg * 32);
       const float4* dps = lse2 + 32;
       // ---- P^T = exp2(S^T * c - lse2).  P^T and then dS^T (16-bit) take the columns of S^T that this warp has read
@@ -253,6 +275,14 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant_
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           if (e < first_q) pf[e] = 0.f;
+        }
+      }
+      if (kWindow && m_tile * kTile + kTile - 1 + p.causal_off - n0 >= p.window && n0 + j >= p.sinks) {
+        // rows whose window lies behind the key
+        const int last_q = n0 + j + p.window - 1 - p.causal_off - (m_tile * kTile + wg * 32);   // last column that sees key j
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          if (e > last_q) pf[e] = 0.f;
         }
       }
       // dropout: bit e of `keep` <-> query column e of these 32.  Lane L draws the bits of query
@@ -342,6 +372,13 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant_
           for (int e = 0; e < kQuarter; ++e) a[e] = 0u;
         }
         const float* af = reinterpret_cast<const float*>(a);
+        if (kWindow && chunks > 1) {
+          const int64_t slot = ((static_cast<int64_t>(b) * p.Hkv + hk) * sink_tiles + n_tile) * chunks + chunk;
+          float4* part = reinterpret_cast<float4*>(p.sink_part + ((slot * 2 + which) * kTile + j) * kD + wg * kQuarter);
+#pragma unroll
+          for (int v = 0; v < kQuarter / 4; ++v) part[v] = make_float4(af[v * 4] * mul, af[v * 4 + 1] * mul, af[v * 4 + 2] * mul, af[v * 4 + 3] * mul);
+          continue;
+        }
 #pragma unroll
         for (int v = 0; v < kQuarter / 8; ++v) {
           uint4 w;
@@ -355,7 +392,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant_
       }
       fence_proxy_async_smem();
       mbar_arrive_warp(staged);
-      if (threadIdx.x == 0) {
+      if (threadIdx.x == 0 && !(kWindow && chunks > 1)) {
         B200FA_WAIT(staged, 0, 0x521);
 #pragma unroll
         for (int cs = 0; cs < Cfg::kSub; ++cs) {
@@ -484,12 +521,13 @@ teardown:
 // scalars.  TMEM columns: S double-buffered at [0,128) and [128,256) (16-bit dS overwrites
 // the buffer it was computed from), dP at [256,384), the dQ accumulator after that.
 // ------------------------------------------------------------------------------------------
-template <int kD, bool kBf16, bool kCausal, bool kDropout>
+template <int kD, bool kBf16, int kMask, bool kDropout>
 __global__ void __launch_bounds__(kThreads, 1)
 bwd_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
               const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapDO,
               const __grid_constant__ CUtensorMap mapDQ, const BwdParams p) {
   using Cfg = BwdCfg<kD>;
+  constexpr bool kCausal = kMask != kAll, kWindow = kMask == kWindowMask;
   constexpr int kTmemS = 0, kTmemDP = 256, kTmemDQ = 384;
   extern __shared__ __align__(1024) uint8_t smem[];
   // K_j is needed twice, a whole step apart (S_j, then dQ += dS_j K_j); V_j only once (dP_j).
@@ -526,10 +564,15 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ 
   // last real row still sees (none: dQ of the tile is zero)
   const int nkv_total = (p.Sk + kTile - 1) / kTile;
   int n_tiles = nkv_total;
-  if (kCausal) {
+  KeyBlocks list = {0, 0, 0};
+  if constexpr (kWindow) {
+    list = window_blocks<kTile>(m0 + p.causal_off, min(m0 + kTile, p.S) - 1 + p.causal_off, p.Sk, p.window, p.sinks);
+    n_tiles = list.n;
+  } else if (kCausal) {
     const int last = min(m0 + kTile - 1, p.S - 1) + p.causal_off;
     n_tiles = last < 0 ? 0 : min(nkv_total, last / kTile + 1);
   }
+  auto key_row = [&](int j) { return (kWindow ? list.at(j) : j) * kTile; };   // first key row of the j-th K/V tile
 
   // This kernel may have started beside the dK/dV kernel.  It still ends after it: its last block waits for that, so
   // that what is ordered behind this kernel is ordered behind both.
@@ -577,9 +620,9 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ 
     fence_proxy_async_smem();
     if (n_tiles > 0) {
       load_tile(&mapQ, sQ, q_full, m0, h);
-      load_tile(&mapK, sK, &k_full[0], 0, hk);
+      load_tile(&mapK, sK, &k_full[0], key_row(0), hk);
       load_tile(&mapDO, sDO, do_full, m0, h);
-      load_tile(&mapV, sV, &v_full[0], 0, hk);
+      load_tile(&mapV, sV, &v_full[0], key_row(0), hk);
     }
   }
   if (warp == 8) {
@@ -604,6 +647,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ 
     const float2 c2 = make_float2(c, c), nl2 = make_float2(nlse2, nlse2), nd2 = make_float2(ndps, ndps);
     for (int j = 0; j < n_tiles; ++j) {
       const int buf = j & 1;
+      const int n0 = key_row(j);
       const uint32_t tS = tmem_base + lane_off + kTmemS + buf * 128 + wg * 64;
       B200FA_WAIT(&s_full[buf], (j >> 1) & 1, 0x900);
       tc_fence_after();
@@ -624,10 +668,10 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ 
         // Columns to blank: beyond the causal diagonal, and beyond the last key.  K rows past Sk are
         // zero-filled, so their dS would be multiplied by zero, but with a very negative lse their
         // probability exp2(0 - lse2) overflows the 16-bit dS to inf, and inf * 0 is NaN.
-        const bool diagonal = kCausal && j * kTile + kTile - 1 > m0 + p.causal_off;
-        const bool past_end = (j + 1) * kTile > p.Sk;
+        const bool diagonal = kCausal && n0 + kTile - 1 > m0 + p.causal_off;
+        const bool past_end = n0 + kTile > p.Sk;
+        const int col0 = n0 + wg * 64 + ch * 32;
         if (diagonal || past_end) {
-          const int col0 = j * kTile + wg * 64 + ch * 32;
           int last_e = 31;   // last visible of these 32
           if (diagonal) last_e = m0 + r + p.causal_off - col0;   // query row r sees a key column only if column <= r + causal_off
           if (past_end) last_e = min(last_e, p.Sk - 1 - col0);
@@ -636,10 +680,17 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ 
             if (e > last_e) pf[ch * 32 + e] = 0.f;
           }
         }
+        if (kWindow && col0 <= m0 + kTile - 1 + p.causal_off - p.window && col0 + 31 >= p.sinks) {
+          const int before = m0 + r + p.causal_off - p.window - col0;   // the last column ahead of the row's window
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            if (e <= before && e >= p.sinks - col0) pf[ch * 32 + e] = 0.f;
+          }
+        }
       }
       uint32_t keep[2] = {0xffffffffu, 0xffffffffu};   // dropout: bit e of keep[ch] <-> key column ch*32 + e of this half
       if constexpr (kDropout) {
-        const int blk = (j * kTile + wg * 64) >> 4;
+        const int blk = (n0 + wg * 64) >> 4;
         const int bh = b * p.Hq + h;
 #pragma unroll
         for (int ch = 0; ch < 2; ++ch) {
@@ -803,10 +854,10 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ 
       int kslot = 1;
       for (int j = 1; j < n_tiles; ++j) {
         if (j >= 3) { B200FA_WAIT(&k_empty[kslot], static_cast<uint32_t>((j / 3 - 1) & 1), 0xb00); }
-        load_tile(&mapK, sK + kslot * Cfg::kTileBytes, &k_full[kslot], j * kTile, hk);
+        load_tile(&mapK, sK + kslot * Cfg::kTileBytes, &k_full[kslot], key_row(j), hk);
         const int vslot = j & 1;
         if (j >= 2) { B200FA_WAIT(&v_empty[vslot], ((j >> 1) - 1) & 1, 0xb01); }
-        load_tile(&mapV, sV + vslot * Cfg::kTileBytes, &v_full[vslot], j * kTile, hk);
+        load_tile(&mapV, sV + vslot * Cfg::kTileBytes, &v_full[vslot], key_row(j), hk);
         if (++kslot == 3) kslot = 0;
       }
     }
@@ -917,14 +968,38 @@ cudaError_t allow_dynamic_smem(Kernel kern, int bytes, std::once_flag (&once)[64
   return result[dev];
 }
 
-template <int kD, bool kBf16, bool kCausal, bool kDropout>
+// dV and dK of the K/V tiles whose steps several blocks shared: the sum of their parts, in their order
+template <int kD, bool kBf16>
+__global__ void __launch_bounds__(256) sink_sum_kernel(const BwdParams p) {
+  const int tiles = static_cast<int>(gridDim.y) / 2, tile = static_cast<int>(blockIdx.y) >> 1, which = blockIdx.y & 1;
+  const int pair = blockIdx.z;   // (batch, kv head)
+  const int idx = static_cast<int>(blockIdx.x) * 256 + threadIdx.x;   // four elements of a row
+  const int row = idx / (kD / 4), c = idx % (kD / 4) * 4;
+  const int s = tile * kTile + row;
+  if (s >= p.Sk || status_is_set(p.status)) return;
+  const int64_t slot = (static_cast<int64_t>(pair) * tiles + tile) * p.sink_chunks;
+  const float* part = p.sink_part + ((slot * 2 + which) * kTile + row) * kD + c;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int i = 0; i < p.sink_chunks; ++i) {
+    const float4 x = *reinterpret_cast<const float4*>(part + static_cast<int64_t>(i) * 2 * kTile * kD);
+    sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+  }
+  const View4& t = which == 0 ? p.dv : p.dk;
+  const int b = pair / p.Hkv, hk = pair - b * p.Hkv;
+  uint16_t* dst = reinterpret_cast<uint16_t*>(t.ptr) + static_cast<int64_t>(b) * t.sb + static_cast<int64_t>(hk) * t.sh +
+                  static_cast<int64_t>(s) * t.ss + c;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<kBf16>(sum.x, sum.y), pack2<kBf16>(sum.z, sum.w));
+}
+
+template <int kD, bool kBf16, int kMask, bool kDropout>
 cudaError_t launch_one(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mdo,
                        const CUtensorMap& mdq, const CUtensorMap& mdk, const CUtensorMap& mdv, const BwdParams& p,
                        cudaStream_t stream) {
   using Cfg = BwdCfg<kD>;
   cudaError_t e = cudaSuccess;
-  auto k1 = bwd_dkdv_kernel<kD, kBf16, kCausal, kDropout>;
-  auto k2 = bwd_dq_kernel<kD, kBf16, kCausal, kDropout>;
+  auto k1 = bwd_dkdv_kernel<kD, kBf16, kMask, kDropout>;
+  auto k2 = bwd_dq_kernel<kD, kBf16, kMask, kDropout>;
   static std::once_flag once1[64], once2[64];
   static cudaError_t result1[64], result2[64];
   if ((e = allow_dynamic_smem(k1, Cfg::kSmemBytes, once1, result1)) != cudaSuccess) return e;
@@ -945,7 +1020,9 @@ cudaError_t launch_one(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
     const int64_t pairs = static_cast<int64_t>(p.B) * p.Hkv;
     if (sched_group < 1) sched_group = 1;
     if (sched_group > pairs) sched_group = pairs;
-    e = launch_early(k1, dim3(static_cast<unsigned>(kv_tiles * pairs)), kDkdvThreads, Cfg::kSmemBytes, stream, (p.parts & 1) != 0,
+    const int sink_tiles = kMask == kWindowMask ? std::min(kv_tiles, (p.sinks + kTile - 1) / kTile) : 0;
+    const int64_t blocks = (kv_tiles + sink_tiles * (p.sink_chunks - 1)) * pairs;
+    e = launch_early(k1, dim3(static_cast<unsigned>(blocks)), kDkdvThreads, Cfg::kSmemBytes, stream, (p.parts & 1) != 0,
                      mq, mk, mv, mdo, mdk, mdv, p, static_cast<int>(sched_group));
   }
   if (e == cudaSuccess && (p.parts & 4)) {
@@ -955,6 +1032,13 @@ cudaError_t launch_one(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
     // D128 51.6 / 47.7, B4 Hq32 Hkv8 S4096 D128 1494 / 1485, B8 H16 S2048 D128 unmasked (one after the other) 815 / 806.
     e = launch_early(k2, dim3(tiles, p.Hq, p.B), kThreads, Cfg::kSmemBytes, stream, (p.parts & 2) != 0, mq, mk, mv, mdo, mdq, p);
   }
+  if constexpr (kMask == kWindowMask) {
+    if (e == cudaSuccess && p.sink_chunks > 1) {
+      const int sink_tiles = std::min(kv_tiles, (p.sinks + kTile - 1) / kTile);
+      sink_sum_kernel<kD, kBf16><<<dim3(kTile * kD / 4 / 256, sink_tiles * 2, p.B * p.Hkv), 256, 0, stream>>>(p);
+      e = cudaGetLastError();
+    }
+  }
   return e;
 }
 
@@ -963,15 +1047,32 @@ cudaError_t launch_mask(const CUtensorMap& mq, const CUtensorMap& mk, const CUte
                         const CUtensorMap& mdq, const CUtensorMap& mdk, const CUtensorMap& mdv, const BwdParams& p,
                         cudaStream_t stream) {
   const bool drop = p.drop.threshold != 0;
+  if (p.window) return launch_one<kD, kBf16, kWindowMask, false>(mq, mk, mv, mdo, mdq, mdk, mdv, p, stream);
   if (p.causal) {
-    return drop ? launch_one<kD, kBf16, true, true>(mq, mk, mv, mdo, mdq, mdk, mdv, p, stream)
-                : launch_one<kD, kBf16, true, false>(mq, mk, mv, mdo, mdq, mdk, mdv, p, stream);
+    return drop ? launch_one<kD, kBf16, kCausalMask, true>(mq, mk, mv, mdo, mdq, mdk, mdv, p, stream)
+                : launch_one<kD, kBf16, kCausalMask, false>(mq, mk, mv, mdo, mdq, mdk, mdv, p, stream);
   }
-  return drop ? launch_one<kD, kBf16, false, true>(mq, mk, mv, mdo, mdq, mdk, mdv, p, stream)
-              : launch_one<kD, kBf16, false, false>(mq, mk, mv, mdo, mdq, mdk, mdv, p, stream);
+  return drop ? launch_one<kD, kBf16, kAll, true>(mq, mk, mv, mdo, mdq, mdk, mdv, p, stream)
+              : launch_one<kD, kBf16, kAll, false>(mq, mk, mv, mdo, mdq, mdk, mdv, p, stream);
 }
 
 }  // namespace
+
+// How many blocks share the steps of a K/V tile with sinks in it.  Every query row behind such a tile sees it, so its block runs
+// (rows / 128) steps per head where the others run a window's; with few heads it would outlast all of them.  A share is at most a
+// quarter of what each SM has to do in all, and at least eight steps (the sums of a share are 128 KB at head dimension 128).
+int bwd_sink_chunks(const BwdParams& p) {
+  const int64_t m_tiles = (p.S + kTile - 1) / kTile, n_tiles = (p.Sk + kTile - 1) / kTile, pairs = static_cast<int64_t>(p.B) * p.Hkv;
+  const int64_t sink_tiles = std::min<int64_t>(n_tiles, (p.sinks + kTile - 1) / kTile);
+  if (!p.window || sink_tiles == 0) return 1;
+  const int64_t group = p.Hq / p.Hkv;
+  const int64_t sink_steps = group * m_tiles;
+  const int64_t others = group * std::min<int64_t>(m_tiles, (p.window + kTile - 1) / kTile + 1);
+  const int64_t all = pairs * (sink_tiles * sink_steps + (n_tiles - sink_tiles) * others);
+  int64_t chunks = (4 * 148 * sink_steps + all - 1) / all;
+  chunks = std::min(chunks, sink_steps / 8);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(chunks, 64)));
+}
 
 cudaError_t launch_bwd_sm100(const BwdParams& p, int dtype, cudaStream_t stream, int* launches) {
   const bool bf16 = (dtype == kBF16);
@@ -991,7 +1092,7 @@ cudaError_t launch_bwd_sm100(const BwdParams& p, int dtype, cudaStream_t stream,
     e = bf16 ? launch_mask<64, true>(mq, mk, mv, mdo, mdq, mdk, mdv, p, stream)
              : launch_mask<64, false>(mq, mk, mv, mdo, mdq, mdk, mdv, p, stream);
   }
-  if (e == cudaSuccess && launches) *launches += (p.parts & 1) + ((p.parts >> 1) & 1) + ((p.parts >> 2) & 1);
+  if (e == cudaSuccess && launches) *launches += (p.parts & 1) + ((p.parts >> 1) & 1) + ((p.parts >> 2) & 1) + (p.window && p.sink_chunks > 1);
   return e;
 }
 

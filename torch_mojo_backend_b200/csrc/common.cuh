@@ -29,6 +29,7 @@ struct FwdParams {
   int B, Hq, Hkv, Sq, Sk, D;
   int causal;        // 0: no mask; otherwise query row i sees key column j iff j <= i + causal_off
   int causal_off;    // 0 (top-left aligned diagonal) or Sk - Sq (bottom-right aligned)
+  int window, sinks; // window > 0 (causal only): row i sees the last `window` of those keys and the first `sinks`; 0: all of them
   float scale;       // softmax scale
   float scale_log2;  // scale * log2(e)
   uint32_t* status;  // optional device status word
@@ -46,6 +47,9 @@ struct BwdParams {
   int B, Hq, Hkv, S, Sk, Spad, D;   // S: query rows (Spad: padded to 128); Sk: key rows
   int causal;
   int causal_off;
+  int window, sinks;   // as in FwdParams
+  int sink_chunks;     // blocks that share the query rows of a K/V tile with sinks in it (1: none do)
+  float* sink_part;    // workspace, if sink_chunks > 1: their dV and dK, (B, Hkv, tiles with sinks, sink_chunks, 2, 128, D)
   float scale;
   float scale_log2;
   uint32_t* status;
@@ -67,7 +71,36 @@ struct SplitKvParams {
   float scale, scale_log2;
 };
 
+// The blocks of `kRows` keys that query rows at positions p_first .. p_last visit under a window: those with one of the first
+// `sinks` keys, then the ones from the window of p_first on.  Rows at p_first with a smaller p_last visit a prefix of the list.
+struct KeyBlocks {
+  int n_sink;   // leading blocks 0 .. n_sink - 1
+  int first;    // block that follows them
+  int n;        // blocks in all; 0: no row sees a key
+  __host__ __device__ __forceinline__ int at(int i) const { return i < n_sink ? i : first + (i - n_sink); }
+};
+template <int kRows>
+__host__ __device__ __forceinline__ KeyBlocks window_blocks(int p_first, int p_last, int Sk, int window, int sinks) {
+  const int last = p_last < Sk - 1 ? p_last : Sk - 1;   // last key that any of the rows sees
+  KeyBlocks r = {0, 0, 0};
+  if (last < 0) return r;
+  const int begin = p_first - window + 1;
+  const int first = begin > 0 ? begin / kRows : 0;
+  const int n_sink = ((sinks < last + 1 ? sinks : last + 1) + kRows - 1) / kRows;
+  if (first <= n_sink) {   // no gap
+    r.n = last / kRows + 1;
+    return r;
+  }
+  r.n_sink = n_sink;
+  r.first = first;
+  r.n = n_sink + (last / kRows >= first ? last / kRows - first + 1 : 0);
+  return r;
+}
+
 constexpr int kSplitkvCluster = 16;   // splits of a KV head that may merge as a cluster
+
+// mask of a tensor-core kernel: every key, the causal diagonal, or the diagonal with a window and sinks
+constexpr int kAll = 0, kCausalMask = 1, kWindowMask = 2;
 
 // dtype tags shared with the C header
 constexpr int kF32 = 0, kBF16 = 1, kF16 = 2;
@@ -82,6 +115,7 @@ cudaError_t launch_bwd_fp32(const BwdParams& p, cudaStream_t stream, int* launch
 cudaError_t launch_fwd_splitkv(const SplitKvParams& p, int dtype, cudaStream_t stream, int* launches);
 cudaError_t launch_bwd_sm100(const BwdParams& p, int dtype, cudaStream_t stream, int* launches);
 cudaError_t launch_bwd_simt(const BwdParams& p, int dtype, cudaStream_t stream, int* launches);
+int bwd_sink_chunks(const BwdParams& p);   // the tensor-core backward's sink_chunks (host only; sizes, mask, window and sinks are read)
 // A one-warp kernel whose only job is to wait, with `budget` SM cycles, on a barrier nobody
 // arrives at: exercises the bounded-wait give-up path without touching the attention kernels.
 cudaError_t launch_wait_timeout_selftest(uint32_t* status, long long budget, cudaStream_t stream, int* launches);

@@ -163,12 +163,14 @@ __device__ __forceinline__ void merge_split(const FwdParams& p, const uint8_t* s
 
 // kSplit: the K/V blocks of a query unit are dealt to the CTAs of a cluster, which merge their
 // (max, sum, O) through distributed shared memory at the end (choose_splits says when).
-template <int kD, bool kBf16, bool kCausal, bool kDropout, int kTiles, bool kSplit>
+// kMask: kAll, kCausalMask, or kWindowMask (causal, a window of keys and the first ones; no dropout)
+template <int kD, bool kBf16, int kMask, bool kDropout, int kTiles, bool kSplit>
 __global__ void __launch_bounds__(FwdCfg<kD, kTiles>::kThreads, kTiles == 2 ? 1 : 2)
 fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
            const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapO, const FwdParams p,
            const FwdSched sched) {
   using Cfg = FwdCfg<kD, kTiles>;
+  constexpr bool kCausal = kMask != kAll, kWindow = kMask == kWindowMask;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                                   // 2 tiles
@@ -219,11 +221,16 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
 
   // KV tiles each query tile visits
   int n_t[2] = {0, 0};
+  KeyBlocks list = {0, 0, 0};   // under a window: the blocks of this unit, in order; a tile visits the first n_t of them
+  if constexpr (kWindow) list = window_blocks<kBN>(row0 + p.causal_off, min(row0 + kTiles * kBM, p.Sq) - 1 + p.causal_off, p.Sk, p.window, p.sinks);
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) {
     const int r0 = row0 + t * kBM;
     if (r0 >= p.Sq) {
       n_t[t] = 0;
+    } else if constexpr (kWindow) {
+      // (the whole unit's list starts at its first row's window: up to a block earlier than the second tile needs)
+      n_t[t] = max(1, window_blocks<kBN>(row0 + p.causal_off, min(r0 + kBM, p.Sq) - 1 + p.causal_off, p.Sk, p.window, p.sinks).n);
     } else if (kCausal) {
       // query row i sees key columns 0 .. i + causal_off: tiles up to the one the tile's last real
       // row still sees; a tile none of whose rows sees a key still runs one fully masked step so
@@ -243,6 +250,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
     for (int t = 0; t < kTiles; ++t) n_t[t] = max(0, min(n_t[t], j_end) - j_first);
   }
   const int n_max = max(n_t[0], n_t[1]);
+  // first key row of this CTA's K/V block j
+  auto key_row = [&](int j) { return (kWindow ? list.at(j_first + j) : j_first + j) * kBN; };
 
   // Lane 0 of the producer warp sets up the barriers and at once issues the loads that need
   // no free slot and are needed first (Q, K_0, V_0), so that their latency overlaps the TMEM
@@ -257,14 +266,14 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
   // K/V ring entry `seq`: K_j for even seq, V_j for odd, j = seq / 2; Q rides along with K_0
   auto produce = [&](int seq) {
     const int slot = seq % Cfg::kStages;
-    const int j = j_first + (seq >> 1);
+    const int krow = key_row(seq >> 1);
     if (seq == 0) {
       // Q tile 0 rides ahead of K_0, Q tile 1 right behind it
       if (n_t[0] > 0) load_tile(&mapQ, sQ, &q_full[0], row0, h);
-      load_tile(&mapK, sKV + slot * Cfg::kTileBytes, &kv_full[slot], j * kBN, hk);
+      load_tile(&mapK, sKV + slot * Cfg::kTileBytes, &kv_full[slot], krow, hk);
       if (kTiles == 2 && n_t[1] > 0) load_tile(&mapQ, sQ + Cfg::kTileBytes, &q_full[1], row0 + kBM, h);
     } else {
-      load_tile((seq & 1) ? &mapV : &mapK, sKV + slot * Cfg::kTileBytes, &kv_full[slot], j * kBN, hk);
+      load_tile((seq & 1) ? &mapV : &mapK, sKV + slot * Cfg::kTileBytes, &kv_full[slot], krow, hk);
     }
   };
   const int n_loads = 2 * n_max;
@@ -330,7 +339,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
     for (int j = 0; j < nblk; ++j) {
       uint32_t keep_bits[4] = {0, 0, 0, 0};   // dropout: one bit per column of this row of the KV block
       if constexpr (kDropout) {
-        dropout_row_bits(p.drop, b * p.Hq + h, q_row, (j_first + j) * kBN, keep_bits);
+        dropout_row_bits(p.drop, b * p.Hq + h, q_row, key_row(j), keep_bits);
       }
       // The 128 key columns of a block are scored, exponentiated and fed to P V in two halves of
       // 64, each with its own S columns: while this warp works on one half, the tensor pipe runs
@@ -342,9 +351,14 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
         tc_fence_after();
         uint32_t s[64];
         float* sf = reinterpret_cast<float*>(s);
-        const int col0 = (j_first + j) * kBN + half * 64;
-        // mask: causal diagonal and/or columns beyond Sk
-        const bool need_mask = (kCausal && (col0 + 63 > row0 + t * kBM + p.causal_off)) || (col0 + 64 > p.Sk);
+        const int col0 = key_row(j) + half * 64;
+        // mask: causal diagonal and/or columns beyond Sk, columns between the sinks and the window
+        bool need_mask = (kCausal && (col0 + 63 > row0 + t * kBM + p.causal_off)) || (col0 + 64 > p.Sk);
+        bool need_low = false;
+        if constexpr (kWindow) {
+          need_low = col0 <= row0 + t * kBM + kBM - 1 + p.causal_off - p.window && col0 + 63 >= p.sinks;
+          need_mask |= need_low;
+        }
         auto load_scores = [&]() {
           tmem_ld32(tSh + 0, s + 0);
           tmem_ld32(tSh + 32, s + 32);
@@ -354,6 +368,13 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
 #pragma unroll
             for (int i = 0; i < 64; ++i) {
               if (col0 + i > limit) sf[i] = -INFINITY;
+            }
+            if (kWindow && need_low) {
+              const int before = q_row + p.causal_off - p.window;   // the last column ahead of the row's window
+#pragma unroll
+              for (int i = 0; i < 64; ++i) {
+                if (col0 + i <= before && col0 + i >= p.sinks) sf[i] = -INFINITY;
+              }
             }
           }
         };
@@ -370,7 +391,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
         float m_new = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
         m_new = fmaxf(m_new, m);
         // rows past the end of the sequence (or fully masked) must not produce NaN
-        if (m_new == -INFINITY) m_new = 0.f;
+        // (under a window a row may see no key yet and see some later: its maximum stays -inf until it does)
+        if (!kWindow && m_new == -INFINITY) m_new = 0.f;
         // Lazy rescaling: nothing moves until some row's true maximum has grown by more than
         // 2^kRescaleLog2 over the maximum its exponentials are taken against.  When one does (the
         // first blocks of a row; rarely later), the warp rewrites its 32 rows of O anyway, so every
@@ -413,7 +435,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
             if (hb < 2 * n_t[0]) { B200FA_WAIT(&xturn[4 + (warp & 3)], hb & 1, 0x111); }
           }
         }
-        const float mc = m * c;
+        const float mc = kWindow && m == -INFINITY ? 0.f : m * c;
         const float2 nmc2 = make_float2(-mc, -mc);
         float2 rsa = make_float2(0.f, 0.f), rsb = make_float2(0.f, 0.f);
         uint32_t pk[32];
@@ -690,11 +712,11 @@ teardown:
   if constexpr (kSplit) cluster_sync();   // no CTA leaves while a peer may still read its shared memory
 }
 
-template <int kD, bool kBf16, bool kCausal, bool kDropout, int kTiles, bool kSplit>
+template <int kD, bool kBf16, int kMask, bool kDropout, int kTiles, bool kSplit>
 cudaError_t launch_tiles(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mo,
                        const FwdParams& p, const FwdSched& sched, cudaStream_t stream) {
   using Cfg = FwdCfg<kD, kTiles>;
-  auto kern = fwd_kernel<kD, kBf16, kCausal, kDropout, kTiles, kSplit>;
+  auto kern = fwd_kernel<kD, kBf16, kMask, kDropout, kTiles, kSplit>;
   // cudaFuncSetAttribute once per device for THIS kernel (the flags are statics of this function
   // template: kernels of the same signature must not share them), safe against concurrent first calls
   static std::once_flag once[64];
@@ -763,7 +785,9 @@ int choose_splits(const FwdParams& p, const FwdSched& sched) {
     int64_t ctas = 0;
     for (int u = sched.npairs - 1; u >= 0; --u) {   // the longest first
       int n = sched.nkv_total;
-      if (p.causal) {
+      if (p.window) {
+        n = std::max(1, window_blocks<kBN>(u * rows + p.causal_off, std::min((u + 1) * rows, p.Sq) - 1 + p.causal_off, p.Sk, p.window, p.sinks).n);
+      } else if (p.causal) {
         const int last = std::min((u + 1) * rows, p.Sq) - 1 + p.causal_off;
         n = last < 0 ? 1 : std::min(n, last / kBN + 1);
       }
@@ -781,15 +805,19 @@ int choose_splits(const FwdParams& p, const FwdSched& sched) {
   return best;
 }
 
-template <int kD, bool kBf16, bool kCausal, bool kDropout>
+template <int kD, bool kBf16, int kMask, bool kDropout>
 cudaError_t launch_one(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mo,
                        const FwdParams& p, const FwdSched& sched, cudaStream_t stream) {
+  constexpr int kTilesChosen = kD == 64 ? 1 : 2;   // what choose_one_tile says unless it is overridden
   if constexpr (!kDropout) {
-    constexpr int kTilesChosen = kD == 64 ? 1 : 2;   // what choose_one_tile says unless it is overridden
-    if (sched.splits > 1) return launch_tiles<kD, kBf16, kCausal, false, kTilesChosen, true>(mq, mk, mv, mo, p, sched, stream);
+    if (sched.splits > 1) return launch_tiles<kD, kBf16, kMask, false, kTilesChosen, true>(mq, mk, mv, mo, p, sched, stream);
   }
-  return sched.one_tile ? launch_tiles<kD, kBf16, kCausal, kDropout, 1, false>(mq, mk, mv, mo, p, sched, stream)
-                        : launch_tiles<kD, kBf16, kCausal, kDropout, 2, false>(mq, mk, mv, mo, p, sched, stream);
+  if constexpr (kMask == kWindowMask) {   // (never overridden)
+    return launch_tiles<kD, kBf16, kMask, kDropout, kTilesChosen, false>(mq, mk, mv, mo, p, sched, stream);
+  } else {
+    return sched.one_tile ? launch_tiles<kD, kBf16, kMask, kDropout, 1, false>(mq, mk, mv, mo, p, sched, stream)
+                          : launch_tiles<kD, kBf16, kMask, kDropout, 2, false>(mq, mk, mv, mo, p, sched, stream);
+  }
 }
 
 // Which kernel shape.  Two CTAs per SM with one query tile each hide a CTA's set-up, first loads
@@ -808,12 +836,13 @@ template <int kD, bool kBf16>
 cudaError_t launch_mask(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mo,
                         const FwdParams& p, const FwdSched& sched, cudaStream_t stream) {
   const bool drop = p.drop.threshold != 0;
+  if (p.window) return launch_one<kD, kBf16, kWindowMask, false>(mq, mk, mv, mo, p, sched, stream);
   if (p.causal) {
-    return drop ? launch_one<kD, kBf16, true, true>(mq, mk, mv, mo, p, sched, stream)
-                : launch_one<kD, kBf16, true, false>(mq, mk, mv, mo, p, sched, stream);
+    return drop ? launch_one<kD, kBf16, kCausalMask, true>(mq, mk, mv, mo, p, sched, stream)
+                : launch_one<kD, kBf16, kCausalMask, false>(mq, mk, mv, mo, p, sched, stream);
   }
-  return drop ? launch_one<kD, kBf16, false, true>(mq, mk, mv, mo, p, sched, stream)
-              : launch_one<kD, kBf16, false, false>(mq, mk, mv, mo, p, sched, stream);
+  return drop ? launch_one<kD, kBf16, kAll, true>(mq, mk, mv, mo, p, sched, stream)
+              : launch_one<kD, kBf16, kAll, false>(mq, mk, mv, mo, p, sched, stream);
 }
 
 FwdSched schedule(const FwdParams& p) {

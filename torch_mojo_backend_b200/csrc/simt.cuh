@@ -27,6 +27,9 @@
 // Loads are asynchronous copies into the one buffer that each streamed tile has: a tile is fetched
 // while the product that does not need it runs.
 //
+// fp32 calls with a window of keys and sinks run here at either head dimension (kWin): the same loops over the tiles that
+// `window_blocks` lists.
+//
 // One translation unit per storage type (simt.cu, simt_bf16.cu, simt_f16.cu): together they are most of the
 // library's compile time.
 #pragma once
@@ -231,10 +234,22 @@ __device__ __forceinline__ void tile_and_head(int tiles, int heads, bool latest_
   *tile = latest_first ? tiles - 1 - t : t;
 }
 
+// the column tiles a block visits: those up to n_end, or the ones among them that its rows' windows and the sinks reach
+template <bool kWin>
+__device__ __forceinline__ KeyBlocks blocks_of(int p_first, int n_end, int Sk, int window, int sinks) {
+  if constexpr (kWin) return window_blocks<kBN>(p_first, n_end - 1, Sk, window, sinks);
+  return KeyBlocks{0, 0, (n_end + kBN - 1) / kBN};
+}
+// column `key` lies between the sinks and the window of query row `row`
+template <class Params>
+__device__ __forceinline__ bool behind_window(const Params& p, int row, int key) {
+  return row + p.causal_off - key >= p.window && key >= p.sinks;
+}
+
 // ------------------------------------------------------------------------------------------
 // forward
 // ------------------------------------------------------------------------------------------
-template <class S, typename T, int kD, bool kDrop>
+template <class S, typename T, int kD, bool kDrop, bool kWin>
 __global__ void __launch_bounds__(S::NT, 1) fwd_simt_kernel(const FwdParams p) {
   extern __shared__ __align__(16) float sm[];
   float* sQ = sm;
@@ -261,10 +276,12 @@ __global__ void __launch_bounds__(S::NT, 1) fwd_simt_kernel(const FwdParams p) {
   }
   // query row i sees key column j iff j <= i + causal_off
   const int n_end = p.causal ? max(0, min(p.Sk, min(m0 + S::BM, p.Sq) + p.causal_off)) : p.Sk;
+  const KeyBlocks list = blocks_of<kWin>(m0 + p.causal_off, n_end, p.Sk, p.window, p.sinks);
   stage_tile<T, kD, S::BM, S::NT, 2>(sQ, p.q, b, h, m0, p.Sq);
-  if (n_end > 0) stage_tile<T, kD, kBN, S::NT, 0>(sK, p.k, b, hk, 0, p.Sk);
+  if (list.n > 0) stage_tile<T, kD, kBN, S::NT, 0>(sK, p.k, b, hk, list.at(0) * kBN, p.Sk);
   cp_commit();
-  for (int n0 = 0; n0 < n_end; n0 += kBN) {
+  for (int it = 0; it < list.n; ++it) {
+    const int n0 = list.at(it) * kBN;
     cp_wait<0>();
     __syncthreads();   // K is here; the last step is done with V and the score tile
     stage_tile<T, kD, kBN, S::NT, 0>(sV, p.v, b, hk, n0, p.Sk);
@@ -277,9 +294,9 @@ __global__ void __launch_bounds__(S::NT, 1) fwd_simt_kernel(const FwdParams p) {
     float s[S::TM][kTN];
     rows_by_cols<S, kD>(sQ, sK, tx, ty, s);
     __syncthreads();   // everyone is done with K
-    if (n0 + kBN < n_end) stage_tile<T, kD, kBN, S::NT, 0>(sK, p.k, b, hk, n0 + kBN, p.Sk);
+    if (it + 1 < list.n) stage_tile<T, kD, kBN, S::NT, 0>(sK, p.k, b, hk, list.at(it + 1) * kBN, p.Sk);
     cp_commit();
-    const bool need_mask = n0 + kBN > p.Sk || (p.causal && n0 + kBN - 1 > m0 + p.causal_off);
+    const bool need_mask = kWin || n0 + kBN > p.Sk || (p.causal && n0 + kBN - 1 > m0 + p.causal_off);
 #pragma unroll
     for (int i = 0; i < S::TM; ++i) {
       const int r = S::row(ty, i);
@@ -287,19 +304,21 @@ __global__ void __launch_bounds__(S::NT, 1) fwd_simt_kernel(const FwdParams p) {
         const int last = p.causal ? min(m0 + r + p.causal_off, p.Sk - 1) : p.Sk - 1;
 #pragma unroll
         for (int j = 0; j < kTN; ++j)
-          if (n0 + tx + kTX * j > last) s[i][j] = -INFINITY;
+          if (n0 + tx + kTX * j > last || (kWin && behind_window(p, m0 + r, n0 + tx + kTX * j))) s[i][j] = -INFINITY;
       }
       float mx = s[i][0];
 #pragma unroll
       for (int j = 1; j < kTN; ++j) mx = fmaxf(mx, s[i][j]);
       mx = group_max<kTX>(mx);
       float m_new = fmaxf(mrow[i], mx);
-      if (m_new == -INFINITY) m_new = 0.f;
-      const float corr = exp2f((mrow[i] - m_new) * c);
+      // (under a window a row may see no key yet and see some later: its maximum stays -inf until it does)
+      if (!kWin && m_new == -INFINITY) m_new = 0.f;
+      const float m_use = kWin && m_new == -INFINITY ? 0.f : m_new;
+      const float corr = exp2f((mrow[i] - m_use) * c);
       float rs = 0.f;
 #pragma unroll
       for (int j = 0; j < kTN; ++j) {
-        s[i][j] = exp2f((s[i][j] - m_new) * c);
+        s[i][j] = exp2f((s[i][j] - m_use) * c);
         rs += s[i][j];   // the row sum keeps every probability; only what multiplies V is dropped
       }
       if constexpr (kDrop) {
@@ -338,7 +357,7 @@ __global__ void __launch_bounds__(S::NT, 1) fwd_simt_kernel(const FwdParams p) {
 // are queries.
 //   P = exp2(S*c - lse*log2e),  dV += P^T dO,  dS = P * (dP - dpsum),  dK += scale * dS^T Q
 // ------------------------------------------------------------------------------------------
-template <class S, typename T, int kD, bool kDrop>
+template <class S, typename T, int kD, bool kDrop, bool kWin>
 __global__ void __launch_bounds__(S::NT, 1) bwd_dkdv_simt_kernel(const BwdParams p) {
   extern __shared__ __align__(16) float sm[];
   float* sK = sm;
@@ -364,7 +383,9 @@ __global__ void __launch_bounds__(S::NT, 1) bwd_dkdv_simt_kernel(const BwdParams
     for (int e = 0; e < kD / 32; ++e) dk[i][e] = dv[i][e] = make_float2(0.f, 0.f);
 
   const int m_begin = p.causal ? max(0, n0 - p.causal_off) / kBN * kBN : 0;   // first tile with a query that sees a key
-  const int per_head = max(0, (p.S - m_begin + kBN - 1) / kBN);
+  int m_end = p.S;
+  if (kWin && n0 >= p.sinks) m_end = min(p.S, max(0, min(n0 + S::BM, p.Sk) - 1 + p.window - p.causal_off));   // behind the last row that sees the tile
+  const int per_head = max(0, (m_end - m_begin + kBN - 1) / kBN);
   const int steps = group * per_head;
   stage_tile<T, kD, S::BM, S::NT, 2>(sK, p.k, b, hk, n0, p.Sk);
   stage_tile<T, kD, S::BM, S::NT, 2>(sV, p.v, b, hk, n0, p.Sk);
@@ -397,7 +418,7 @@ __global__ void __launch_bounds__(S::NT, 1) bwd_dkdv_simt_kernel(const BwdParams
     cp_wait<0>();
     __syncthreads();   // Q and the statistics are here
     rows_by_cols<S, kD>(sK, sQ, tx, ty, s);
-    const bool need_mask = n0 + S::BM > p.Sk || m0 + kBN > p.S || (p.causal && n0 + S::BM - 1 > m0 + p.causal_off);
+    const bool need_mask = kWin || n0 + S::BM > p.Sk || m0 + kBN > p.S || (p.causal && n0 + S::BM - 1 > m0 + p.causal_off);
 #pragma unroll
     for (int j = 0; j < kTN; ++j) {
       const int ql = tx + kTX * j, qr = m0 + ql;
@@ -406,7 +427,7 @@ __global__ void __launch_bounds__(S::NT, 1) bwd_dkdv_simt_kernel(const BwdParams
       for (int i = 0; i < S::TM; ++i) {
         const int kc = n0 + S::row(ty, i);
         float pv = exp2f(s[i][j] * c - l2);
-        if (need_mask && (kc >= p.Sk || qr >= p.S || (p.causal && kc > qr + p.causal_off))) pv = 0.f;
+        if (need_mask && (kc >= p.Sk || qr >= p.S || (p.causal && kc > qr + p.causal_off) || (kWin && behind_window(p, qr, kc)))) pv = 0.f;
         float dm = 1.f;   // dropout multiplier of this entry: 0 or 1 / (1 - p)
         if constexpr (kDrop) {
           const int r = S::row(ty, i);
@@ -443,7 +464,7 @@ __global__ void __launch_bounds__(S::NT, 1) bwd_dkdv_simt_kernel(const BwdParams
 // backward, part 2: dQ.  One block per (query tile, q head, batch); loops over the key tiles up
 // to the diagonal.  dQ = scale * dS K.  Deterministic: no atomics.
 // ------------------------------------------------------------------------------------------
-template <class S, typename T, int kD, bool kDrop>
+template <class S, typename T, int kD, bool kDrop, bool kWin>
 __global__ void __launch_bounds__(S::NT, 1) bwd_dq_simt_kernel(const BwdParams p) {
   extern __shared__ __align__(16) float sm[];
   float* sQ = sm;
@@ -477,9 +498,11 @@ __global__ void __launch_bounds__(S::NT, 1) bwd_dq_simt_kernel(const BwdParams p
   const int n_end = p.causal ? max(0, min(p.Sk, min(m0 + S::BM, p.S) + p.causal_off)) : p.Sk;
   stage_tile<T, kD, S::BM, S::NT, 2>(sQ, p.q, b, h, m0, p.S);
   stage_tile<T, kD, S::BM, S::NT, 2>(sdO, p.dout, b, h, m0, p.S);
-  if (n_end > 0) stage_tile<T, kD, kBN, S::NT, 0>(sV, p.v, b, hk, 0, p.Sk);
+  const KeyBlocks list = blocks_of<kWin>(m0 + p.causal_off, n_end, p.Sk, p.window, p.sinks);
+  if (list.n > 0) stage_tile<T, kD, kBN, S::NT, 0>(sV, p.v, b, hk, list.at(0) * kBN, p.Sk);
   cp_commit();
-  for (int n0 = 0; n0 < n_end; n0 += kBN) {
+  for (int it = 0; it < list.n; ++it) {
+    const int n0 = list.at(it) * kBN;
     cp_wait<0>();
     __syncthreads();   // V is here; the last step is done with K and the score tile
     stage_tile<T, kD, kBN, S::NT, 0>(sK, p.k, b, hk, n0, p.Sk);
@@ -493,10 +516,10 @@ __global__ void __launch_bounds__(S::NT, 1) bwd_dq_simt_kernel(const BwdParams p
     rows_by_cols<S, kD>(sdO, sV, tx, ty, dp);
     cp_wait<0>();
     __syncthreads();   // K is here; everyone is done with V
-    if (n0 + kBN < n_end) stage_tile<T, kD, kBN, S::NT, 0>(sV, p.v, b, hk, n0 + kBN, p.Sk);
+    if (it + 1 < list.n) stage_tile<T, kD, kBN, S::NT, 0>(sV, p.v, b, hk, list.at(it + 1) * kBN, p.Sk);
     cp_commit();
     rows_by_cols<S, kD>(sQ, sK, tx, ty, s);
-    const bool need_mask = n0 + kBN > p.Sk || m0 + S::BM > p.S || (p.causal && n0 + kBN - 1 > m0 + p.causal_off);
+    const bool need_mask = kWin || n0 + kBN > p.Sk || m0 + S::BM > p.S || (p.causal && n0 + kBN - 1 > m0 + p.causal_off);
 #pragma unroll
     for (int i = 0; i < S::TM; ++i) {
       const int r = S::row(ty, i), qr = m0 + r;
@@ -506,7 +529,7 @@ __global__ void __launch_bounds__(S::NT, 1) bwd_dq_simt_kernel(const BwdParams p
       for (int j = 0; j < kTN; ++j) {
         const int kc = n0 + tx + kTX * j;
         float pv = exp2f(s[i][j] * c - lse2[i]);
-        if (need_mask && (kc >= p.Sk || qr >= p.S || (p.causal && kc > qr + p.causal_off))) pv = 0.f;
+        if (need_mask && (kc >= p.Sk || qr >= p.S || (p.causal && kc > qr + p.causal_off) || (kWin && behind_window(p, qr, kc)))) pv = 0.f;
         float dm = 1.f;
         if constexpr (kDrop) dm = ((keep >> (kTX * j)) & 1u) ? p.drop.inv_keep : 0.f;
         s[i][j] = pv * (dp[i][j] * dm - dps[i]);
@@ -567,8 +590,11 @@ template <class S, typename T, int kD>
 cudaError_t launch_fwd_s(const FwdParams& p, cudaStream_t stream) {
   const int64_t blocks = (int64_t)p.B * p.Hq * ((p.Sq + S::BM - 1) / S::BM);
   constexpr int smem = smem_bytes<S, kD>(1);
-  return p.drop.threshold != 0 ? launch(fwd_simt_kernel<S, T, kD, true>, blocks, S::NT, smem, stream, p)
-                               : launch(fwd_simt_kernel<S, T, kD, false>, blocks, S::NT, smem, stream, p);
+  if constexpr (sizeof(T) == 4) {
+    if (p.window) return launch(fwd_simt_kernel<S, T, kD, false, true>, blocks, S::NT, smem, stream, p);
+  }
+  return p.drop.threshold != 0 ? launch(fwd_simt_kernel<S, T, kD, true, false>, blocks, S::NT, smem, stream, p)
+                               : launch(fwd_simt_kernel<S, T, kD, false, false>, blocks, S::NT, smem, stream, p);
 }
 
 template <typename T, int kD>
@@ -581,16 +607,22 @@ template <class S, typename T, int kD>
 cudaError_t launch_dkdv_s(const BwdParams& p, cudaStream_t stream) {
   const int64_t blocks = (int64_t)p.B * p.Hkv * ((p.Sk + S::BM - 1) / S::BM);
   constexpr int smem = smem_bytes<S, kD>(2);
-  return p.drop.threshold != 0 ? launch(bwd_dkdv_simt_kernel<S, T, kD, true>, blocks, S::NT, smem, stream, p)
-                               : launch(bwd_dkdv_simt_kernel<S, T, kD, false>, blocks, S::NT, smem, stream, p);
+  if constexpr (sizeof(T) == 4) {
+    if (p.window) return launch(bwd_dkdv_simt_kernel<S, T, kD, false, true>, blocks, S::NT, smem, stream, p);
+  }
+  return p.drop.threshold != 0 ? launch(bwd_dkdv_simt_kernel<S, T, kD, true, false>, blocks, S::NT, smem, stream, p)
+                               : launch(bwd_dkdv_simt_kernel<S, T, kD, false, false>, blocks, S::NT, smem, stream, p);
 }
 
 template <class S, typename T, int kD>
 cudaError_t launch_dq_s(const BwdParams& p, cudaStream_t stream) {
   const int64_t blocks = (int64_t)p.B * p.Hq * ((p.S + S::BM - 1) / S::BM);
   constexpr int smem = smem_bytes<S, kD>(2);
-  return p.drop.threshold != 0 ? launch(bwd_dq_simt_kernel<S, T, kD, true>, blocks, S::NT, smem, stream, p)
-                               : launch(bwd_dq_simt_kernel<S, T, kD, false>, blocks, S::NT, smem, stream, p);
+  if constexpr (sizeof(T) == 4) {
+    if (p.window) return launch(bwd_dq_simt_kernel<S, T, kD, false, true>, blocks, S::NT, smem, stream, p);
+  }
+  return p.drop.threshold != 0 ? launch(bwd_dq_simt_kernel<S, T, kD, true, false>, blocks, S::NT, smem, stream, p)
+                               : launch(bwd_dq_simt_kernel<S, T, kD, false, false>, blocks, S::NT, smem, stream, p);
 }
 
 template <typename T, int kD>

@@ -122,3 +122,77 @@ def flash_bwd(dout, q, k, v, out, lse, *, causal, scale: float | None = None, dq
     if rc != _lib.OK:
         raise _lib.B200FAError(rc, "b200fa_bwd")
     return dq, dk, dv
+
+
+def _need_cuda(q) -> None:
+    if q.device.type != "cuda":
+        raise RuntimeError("b200fa kernels need CUDA memory; there is no CPU implementation")
+
+
+def _same_kind(q, others) -> None:
+    """Pointers are all that the library sees of a tensor: its type and device are checked here."""
+    for t in others:
+        if t is not None and (t.dtype != q.dtype or t.device != q.device):
+            raise ValueError(f"expected {q.dtype} tensors on {q.device}, got {t.dtype} on {t.device}")
+
+
+def _fp32_statistic(lse, shape, device) -> None:
+    if lse.dtype != torch.float32 or tuple(lse.shape) != tuple(shape) or not lse.is_contiguous() or lse.device != device:
+        raise ValueError(f"lse has to be a contiguous float32 tensor of shape {tuple(shape)} on {device}")
+
+
+def window_fwd(q, k, v, *, window: int, sinks: int = 0, causal=True, scale: float | None = None, out=None, lse=None,
+               status=None):
+    """out, lse = causal attention over the last ``window`` keys and the first ``sinks`` ones.
+
+    ``causal``: True (diagonal from the top-left corner) or ``_lib.CAUSAL_BOTTOM_RIGHT`` (new queries against a longer
+    key sequence).  With p the last key that the diagonal lets a row see, the row sees key j iff ``j <= p`` and
+    (``j > p - window`` or ``j < sinks``).  Shapes, types and results as for ``flash_fwd``; a row that sees no key is 0
+    with lse -inf.  Values behind the mask have to be finite where a visible key shares their block of 128.
+    """
+    _need_cuda(q)
+    B, Hq, Sq, D = q.shape
+    if scale is None:
+        scale = default_scale(D)
+    if out is None:
+        out = torch.empty((B, Hq, Sq, D), dtype=q.dtype, device=q.device)
+    if lse is None:
+        lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device)
+    else:
+        _fp32_statistic(lse, (B, Hq, Sq), q.device)
+    _same_kind(q, (k, v, out))
+    stream, dev = _stream_and_device(q)
+    rc = _lib.window_fwd(t4(q), t4(k), t4(v), t4(out), lse.data_ptr(), dtype_code(q.dtype), causal, window, sinks,
+                         float(scale), stream, dev, status.data_ptr() if status is not None else 0)
+    if rc != _lib.OK:
+        raise _lib.B200FAError(rc, "b200fa_window_fwd")
+    return out, lse
+
+
+def window_bwd(dout, q, k, v, out, lse, *, window: int, sinks: int = 0, causal=True, scale: float | None = None, dq=None,
+               dk=None, dv=None, workspace=None, status=None):
+    """dq, dk, dv of ``window_fwd``, whose ``out`` and ``lse`` are given."""
+    _need_cuda(q)
+    B, Hq, S, D = q.shape
+    Hkv, Sk = k.shape[1], k.shape[2]
+    if scale is None:
+        scale = default_scale(D)
+    if dq is None:
+        dq = torch.empty((B, Hq, S, D), dtype=q.dtype, device=q.device)
+    if dk is None:
+        dk = torch.empty(tuple(k.shape), dtype=q.dtype, device=q.device)
+    if dv is None:
+        dv = torch.empty(tuple(v.shape), dtype=q.dtype, device=q.device)
+    _fp32_statistic(lse, (B, Hq, S), q.device)
+    _same_kind(q, (dout, k, v, out, dq, dk, dv))
+    code = dtype_code(q.dtype)
+    need = _lib.window_bwd_workspace_bytes(B, Hq, Hkv, S, Sk, D, code, window, sinks)
+    if workspace is None:
+        workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
+    stream, dev = _stream_and_device(q)
+    rc = _lib.window_bwd(t4(q), t4(k), t4(v), t4(out), t4(dout), lse.data_ptr(), t4(dq), t4(dk), t4(dv),
+                         workspace.data_ptr(), workspace.numel() * workspace.element_size(), code, causal, window, sinks,
+                         float(scale), stream, dev, status.data_ptr() if status is not None else 0)
+    if rc != _lib.OK:
+        raise _lib.B200FAError(rc, "b200fa_window_bwd")
+    return dq, dk, dv
