@@ -52,6 +52,7 @@ extern "C" {
 #define B200FA_ERR_CUDA (-7)
 #define B200FA_ERR_NULL (-8)
 #define B200FA_ERR_TIMEOUT (-9)
+#define B200FA_ERR_BAD_INDEX (-10)
 
 /* causal argument of every entry point: query row i sees key column j iff
  *   B200FA_CAUSAL_NONE          always
@@ -195,6 +196,68 @@ int b200fa_fwd_splitkv(const b200fa_tensor4* q, const b200fa_tensor4* k, const b
                        const b200fa_tensor4* out, float* lse, void* workspace, size_t workspace_bytes,
                        int dtype, int causal, float scale, void* stream, int device,
                        uint32_t* status_word);
+
+/*
+ * A paged key/value cache: a pool of pages, each `page_size` tokens (a power of two, 16 to 4096) of every KV head, and for each
+ * sequence of the batch a row of page numbers, in order.  No counterpart in the reference, whose caches are dense.
+ *   k, v        (pages, heads, page_size, head_dim) contiguous, of `dtype` (B200FA_BF16 or B200FA_F16), for bits = 16;
+ *               (pages, heads, page_size, head_dim / 2) bytes, two codes to a byte, for bits = 4.
+ *   k_scales,   bits = 4: (pages, heads, page_size, head_dim / 32, 2) contiguous, of `dtype`: scale and minimum of every 32
+ *   v_scales    elements; an element is code * scale + minimum.  Code i of a row (the low half of a byte first) is, of a key,
+ *               element 32 G + 8 t + j with i = (t * (head_dim / 32) + G) * 8 + j, t < 4, j < 8; of a value, element
+ *               32 G + 4 g + j with i = (g * (head_dim / 32) + G) * 4 + j, g < 8, j < 4.
+ *   table       (batch, table_width) page numbers, rows `table_stride` apart; entries behind a sequence's last page are not read.
+ *   lengths     (batch) tokens in the cache, the new ones of the call included; 0: an idle place in the batch.
+ *   new_lengths (batch) or NULL: how many of the S tokens of a call's tensors are new tokens of the sequence (the first ones of
+ *               its rows; those behind are padding).  NULL: all S.  Token s is at position length - new + s; one whose position
+ *               would be negative is not there: it is not written, and sees no key.
+ * table, lengths and new_lengths are read by the kernels, on `stream`: a captured call follows their contents.  A page, a length or a
+ * position out of range is never used; the results that depend on it are NaN (nothing is written by an append), and
+ * `status_word` becomes a value that b200fa_status_to_error maps to B200FA_ERR_BAD_INDEX.  No two tokens of one append may name
+ * the same place.  A page may belong to several sequences as long as none appends to it.
+ */
+typedef struct b200fa_paged_kv {
+  void *k, *v, *k_scales, *v_scales;
+  const int32_t *table, *lengths, *new_lengths;
+  int64_t pages, heads, page_size, head_dim;
+  int64_t batch, table_width, table_stride;
+  int dtype, bits;
+} b200fa_paged_kv;
+
+/*
+ * Writes k and v (batch, heads, S, head_dim) of the new tokens to the pages, k rotated by position, and q (or NULL),
+ * (batch, Hq, S, head_dim), rotated the same way to q_out (which may be q).  rotary_dim: how many of the first elements turn, a
+ * multiple of 16 (0: none, q NULL), in pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if `interleaved`; cos, sin:
+ * (positions, rotary_dim / 2) fp32, 16-byte aligned.  (a, b) becomes (a c - b s, b c + a s), every operation rounded to fp32,
+ * then to `dtype`.  4 bits: scale = (max - min) / 15 rounded to `dtype`, code = round((x - min) / scale); a group with an
+ * element that is not finite reads NaN.  Rows of q_out behind a sequence's new tokens are left as they are.
+ */
+int b200fa_paged_append(const b200fa_paged_kv* cache, const b200fa_tensor4* k, const b200fa_tensor4* v,
+                        const b200fa_tensor4* q, const b200fa_tensor4* q_out, const float* cos, const float* sin,
+                        int64_t rotary_dim, int64_t positions, int interleaved, void* stream, int device,
+                        uint32_t* status_word);
+
+/*
+ * Attention of the new tokens' queries q (batch, Hq, S, head_dim) over the pages, causal by position, over the last `window`
+ * keys and the first `sinks` of them where window > 0 (0: all).  out like q; lse fp32 (batch, Hq, S) contiguous; Hq % heads == 0.
+ * Rows behind a sequence's new tokens are left as they are; a row that sees no key gets out = 0, lse = -inf.  Keys that no
+ * new token of the sequence sees are not read: pages that hold none of the others may be given away.  `longest` (0: not
+ * known, table_width * page_size then) is no bound but a hint, how many keys to spread over the GPU.  Sums of a row depend
+ * on how many blocks share its keys, which goes by the sizes and that hint, not by the contents of the device tensors.  No
+ * workspace: the blocks that share the keys of a KV head are a cluster.  16-bit pages and 4-bit pages; rows beyond 16 of a
+ * KV head's group (Hq / heads * S) read the pages again, 16 at a time (long prompts: b200fa_paged_gather, then b200fa_window_fwd
+ * or b200fa_fwd).
+ */
+int b200fa_paged_attention(const b200fa_paged_kv* cache, const b200fa_tensor4* q, const b200fa_tensor4* out, float* lse,
+                           int64_t window, int64_t sinks, float scale, int64_t longest, void* stream, int device,
+                           uint32_t* status_word);
+
+/*
+ * The first S tokens of every sequence as dense k and v (batch, heads, S, head_dim) of `dtype`, rows behind a sequence's
+ * length zero; 4-bit pages give code * scale + minimum, each operation rounded to fp32, then to `dtype`.  new_lengths is not read.
+ */
+int b200fa_paged_gather(const b200fa_paged_kv* cache, const b200fa_tensor4* k, const b200fa_tensor4* v, void* stream,
+                        int device, uint32_t* status_word);
 
 /*
  * b200fa_bwd for callers that cannot allocate device memory.  (No counterpart in the

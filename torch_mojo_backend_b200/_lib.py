@@ -31,6 +31,7 @@ ERR_UNSUPPORTED = -6
 ERR_CUDA = -7
 ERR_NULL = -8
 ERR_TIMEOUT = -9
+ERR_BAD_INDEX = -10
 
 #: every symbol include/b200fa.h declares; the CPU test-suite checks the library exports them
 EXPORTED_SYMBOLS = (
@@ -55,6 +56,9 @@ EXPORTED_SYMBOLS = (
     "b200fa_window_fwd",
     "b200fa_window_bwd_workspace_bytes",
     "b200fa_window_bwd",
+    "b200fa_paged_append",
+    "b200fa_paged_attention",
+    "b200fa_paged_gather",
     "b200fa_set_wait_budget",
     "b200fa_wait_budget",
     "b200fa_set_fwd_tiles",
@@ -86,6 +90,26 @@ class Tensor4(ctypes.Structure):
             raise ValueError("b200fa tensors are 4-D (batch, heads, seq, head_dim)")
         # (packed as bytes: field by field ctypes takes five times as long, and a training step makes twelve)
         return cls.from_buffer_copy(_pack_tensor4(ptr or 0, *shape, *stride))
+
+
+_pack_paged = struct.Struct("7P7q2i").pack
+
+
+class PagedCache(ctypes.Structure):
+    """``b200fa_paged_kv``: addresses of a paged cache, its block table and lengths, and their sizes."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p),
+        ("table", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("new_lengths", ctypes.c_void_p),
+        ("pages", ctypes.c_int64), ("heads", ctypes.c_int64), ("page_size", ctypes.c_int64), ("head_dim", ctypes.c_int64),
+        ("batch", ctypes.c_int64), ("table_width", ctypes.c_int64), ("table_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int), ("bits", ctypes.c_int),
+    ]
+
+    @classmethod
+    def make(cls, *fields) -> "PagedCache":
+        """The fields in their order, pointers as integers (0: NULL)."""
+        return cls.from_buffer_copy(_pack_paged(*fields))
 
 
 class B200FAError(RuntimeError):
@@ -144,6 +168,15 @@ def load() -> ctypes.CDLL:
     lib.b200fa_window_bwd.restype = ctypes.c_int
     lib.b200fa_window_bwd_workspace_bytes.argtypes = [ctypes.c_int64] * 6 + [ctypes.c_int] + [ctypes.c_int64] * 2
     lib.b200fa_window_bwd_workspace_bytes.restype = ctypes.c_size_t
+    cache = ctypes.POINTER(PagedCache)
+    lib.b200fa_paged_append.argtypes = [cache, t4p, t4p, t4p, t4p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+                                        ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
+    lib.b200fa_paged_append.restype = ctypes.c_int
+    lib.b200fa_paged_attention.argtypes = [cache, t4p, t4p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_float,
+                                           ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
+    lib.b200fa_paged_attention.restype = ctypes.c_int
+    lib.b200fa_paged_gather.argtypes = [cache, t4p, t4p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
+    lib.b200fa_paged_gather.restype = ctypes.c_int
     lib.b200fa_dropout_threshold.argtypes = [ctypes.c_float]
     lib.b200fa_dropout_threshold.restype = ctypes.c_uint32
     lib.b200fa_dropout_bytes_host.argtypes = [ctypes.c_uint64, ctypes.c_uint64, ctypes.c_int64, ctypes.c_int64,
@@ -268,6 +301,24 @@ def window_bwd(q: Tensor4, k: Tensor4, v: Tensor4, out: Tensor4, dout: Tensor4, 
         ctypes.byref(q), ctypes.byref(k), ctypes.byref(v), ctypes.byref(out), ctypes.byref(dout), lse_ptr, ctypes.byref(dq),
         ctypes.byref(dk), ctypes.byref(dv), workspace_ptr, workspace_bytes, dtype, causal_code(causal), window, sinks, scale,
         stream, device, status_ptr)
+
+
+def paged_append(cache: PagedCache, k: Tensor4, v: Tensor4, q: Tensor4 | None, q_out: Tensor4 | None, cos_ptr: int, sin_ptr: int,
+                 rotary_dim: int, positions: int, interleaved: bool, stream: int, device: int, status_ptr: int = 0) -> int:
+    """Raw append to a paged cache (see b200fa_paged_append); returns the library's status code."""
+    return load().b200fa_paged_append(cache, k, v, q, q_out, cos_ptr, sin_ptr, rotary_dim, positions, 1 if interleaved else 0, stream,
+                                      device, status_ptr)
+
+
+def paged_attention(cache: PagedCache, q: Tensor4, out: Tensor4, lse_ptr: int, window: int, sinks: int, scale: float, longest: int,
+                    stream: int, device: int, status_ptr: int = 0) -> int:
+    """Raw attention over a paged cache (see b200fa_paged_attention); returns the library's status code."""
+    return load().b200fa_paged_attention(cache, q, out, lse_ptr, window, sinks, scale, longest, stream, device, status_ptr)
+
+
+def paged_gather(cache: PagedCache, k: Tensor4, v: Tensor4, stream: int, device: int, status_ptr: int = 0) -> int:
+    """Raw read-back of a paged cache (see b200fa_paged_gather); returns the library's status code."""
+    return load().b200fa_paged_gather(cache, k, v, stream, device, status_ptr)
 
 
 def fwd_splitkv_workspace_bytes(B: int, Hq: int, Hkv: int, Sq: int, Sk: int, D: int, whole_heads: int = 0) -> int:

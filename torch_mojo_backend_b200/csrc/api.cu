@@ -356,6 +356,51 @@ int bwd_impl(const b200fa_tensor4* q, const b200fa_tensor4* k, const b200fa_tens
   return e == cudaSuccess ? B200FA_OK : B200FA_ERR_CUDA;
 }
 
+// Checks a paged cache and fills `c`.  Pages are contiguous; what their indexes are worth only the kernels can see.
+int check_cache(const b200fa_paged_kv* t, uint32_t* status_word, PagedCache* c) {
+  if (!t || !t->k || !t->v || !t->table || !t->lengths) return B200FA_ERR_NULL;
+  if (t->dtype != kBF16 && t->dtype != kF16) return B200FA_ERR_BAD_DTYPE;
+  if (t->bits != 16 && t->bits != 4) return B200FA_ERR_UNSUPPORTED;
+  if (t->bits == 4 && (!t->k_scales || !t->v_scales)) return B200FA_ERR_NULL;
+  if (t->head_dim != 64 && t->head_dim != 128) return B200FA_ERR_UNSUPPORTED;
+  if (t->page_size < 16 || t->page_size > 4096 || (t->page_size & (t->page_size - 1)) != 0) return B200FA_ERR_UNSUPPORTED;
+  if (t->pages <= 0 || t->pages > INT_MAX || t->heads <= 0 || t->heads > 65535 || t->batch <= 0 || t->batch > 65535) return B200FA_ERR_BAD_SHAPE;
+  if (t->table_width <= 0 || t->table_width > (1 << 24) / t->page_size) return B200FA_ERR_BAD_SHAPE;   // 2^24 tokens, as everywhere
+  if (t->table_stride < t->table_width && t->batch > 1) return B200FA_ERR_BAD_STRIDE;
+  for (const void* x : {t->k, t->v, t->k_scales, t->v_scales})
+    if (reinterpret_cast<uintptr_t>(x) % 16 != 0) return B200FA_ERR_MISALIGNED;
+  for (const int32_t* x : {t->table, t->lengths, t->new_lengths})
+    if (reinterpret_cast<uintptr_t>(x) % 4 != 0) return B200FA_ERR_MISALIGNED;
+  c->k = t->k; c->v = t->v; c->k_scales = t->k_scales; c->v_scales = t->v_scales;
+  c->table = t->table; c->lengths = t->lengths; c->new_lengths = t->new_lengths;
+  c->table_stride = t->table_stride;
+  c->B = static_cast<int>(t->batch); c->Hkv = static_cast<int>(t->heads); c->D = static_cast<int>(t->head_dim); c->bits = t->bits;
+  c->shift = 0;
+  while ((int64_t(1) << c->shift) < t->page_size) ++c->shift;
+  c->pages = static_cast<int>(t->pages);
+  c->capacity = static_cast<int>(t->table_width * t->page_size);
+  c->status = status_word;
+  return B200FA_OK;
+}
+
+// What the three calls on a paged cache have in common behind their checks: device, launch, accounting.
+template <typename Launch>
+int run_on(int device, const char* name, Launch launch) {
+  DeviceGuard guard(device);
+  if (!guard.ok) {
+    note_cuda_error("cudaSetDevice", cudaGetLastError());
+    return B200FA_ERR_CUDA;
+  }
+  const int rc = check_device_is_sm100(device);
+  if (rc != B200FA_OK) return rc;
+  int launches = 0;
+  (void)cudaGetLastError();
+  const cudaError_t e = launch(&launches);
+  g_launches += launches;
+  if (e != cudaSuccess) note_cuda_error(name, e);
+  return e == cudaSuccess ? B200FA_OK : B200FA_ERR_CUDA;
+}
+
 // Splits of the split-KV forward: the count up to 64, of at least 256 keys each, that the model
 // below finds cheapest; the first found wins a tie, which is the one with fewer splits.
 // The grid runs in waves of the CTAs that fit: by registers, 3 and 2 per SM of the 16-bit kernel at
@@ -442,6 +487,7 @@ const char* b200fa_strerror(int code) {
     case B200FA_ERR_UNSUPPORTED: return "configuration is not supported (head_dim must be 64 or 128, causal in {0, 1, 2}, scale > 0, 0 <= dropout_p < 1, sm_100 device)";
     case B200FA_ERR_CUDA: return "a CUDA runtime or driver call failed";
     case B200FA_ERR_NULL: return "a required pointer is null";
+    case B200FA_ERR_BAD_INDEX: return "a page, length or position of a paged cache is out of range";
     case B200FA_ERR_TIMEOUT: return "a kernel gave up waiting on an internal barrier";
     default: return "unknown b200fa error";
   }
@@ -672,6 +718,85 @@ int b200fa_fwd_splitkv_piece(const b200fa_tensor4* q, const b200fa_tensor4* k, c
   return e == cudaSuccess ? B200FA_OK : B200FA_ERR_CUDA;
 }
 
+int b200fa_paged_append(const b200fa_paged_kv* cache, const b200fa_tensor4* k, const b200fa_tensor4* v,
+                        const b200fa_tensor4* q, const b200fa_tensor4* q_out, const float* cos, const float* sin,
+                        int64_t rotary_dim, int64_t positions, int interleaved, void* stream, int device,
+                        uint32_t* status_word) {
+  AppendParams p;
+  std::memset(&p, 0, sizeof(p));
+  int rc = check_cache(cache, status_word, &p.c);
+  if (rc != B200FA_OK) return rc;
+  if (!k || !v || (!q) != (!q_out)) return B200FA_ERR_NULL;
+  const int64_t B = p.c.B, S = k->shape[2], D = p.c.D, Hq = q ? q->shape[1] : 0;
+  if (S <= 0 || S > (1 << 24) || Hq < 0 || Hq > 65535 || (q && Hq == 0)) return B200FA_ERR_BAD_SHAPE;
+  if (rotary_dim < 0 || rotary_dim > D || rotary_dim % 16 != 0) return B200FA_ERR_UNSUPPORTED;
+  if (q && rotary_dim == 0) return B200FA_ERR_UNSUPPORTED;   // (nothing would turn them)
+  if (rotary_dim > 0) {
+    if (!cos || !sin) return B200FA_ERR_NULL;
+    if (positions <= 0 || positions > INT_MAX) return B200FA_ERR_BAD_SHAPE;
+    if (reinterpret_cast<uintptr_t>(cos) % 16 != 0 || reinterpret_cast<uintptr_t>(sin) % 16 != 0) return B200FA_ERR_MISALIGNED;
+  }
+  if (B * S * (Hq + 2 * p.c.Hkv) > INT_MAX) return B200FA_ERR_BAD_SHAPE;
+  const int dtype = cache->dtype;
+  if ((rc = check_view(k, B, p.c.Hkv, S, D, dtype, &p.k)) != B200FA_OK) return rc;
+  if ((rc = check_view(v, B, p.c.Hkv, S, D, dtype, &p.v)) != B200FA_OK) return rc;
+  if (q) {
+    if ((rc = check_view(q, B, Hq, S, D, dtype, &p.q)) != B200FA_OK) return rc;
+    if ((rc = check_view(q_out, B, Hq, S, D, dtype, &p.q_out, true)) != B200FA_OK) return rc;
+  }
+  p.cos = cos; p.sin = sin;
+  p.Hq = static_cast<int>(Hq); p.S = static_cast<int>(S);
+  p.rotary = static_cast<int>(rotary_dim); p.positions = static_cast<int>(positions); p.interleaved = interleaved != 0;
+  return run_on(device, "b200fa_paged_append",
+                [&](int* n) { return launch_paged_append(p, dtype, static_cast<cudaStream_t>(stream), n); });
+}
+
+int b200fa_paged_gather(const b200fa_paged_kv* cache, const b200fa_tensor4* k, const b200fa_tensor4* v, void* stream,
+                        int device, uint32_t* status_word) {
+  GatherParams p;
+  std::memset(&p, 0, sizeof(p));
+  int rc = check_cache(cache, status_word, &p.c);
+  if (rc != B200FA_OK) return rc;
+  if (!k || !v) return B200FA_ERR_NULL;
+  const int64_t S = k->shape[2];
+  if (S <= 0 || S > (1 << 24) || static_cast<int64_t>(p.c.B) * p.c.Hkv * S > INT_MAX) return B200FA_ERR_BAD_SHAPE;
+  if ((rc = check_view(k, p.c.B, p.c.Hkv, S, p.c.D, cache->dtype, &p.k, true)) != B200FA_OK) return rc;
+  if ((rc = check_view(v, p.c.B, p.c.Hkv, S, p.c.D, cache->dtype, &p.v, true)) != B200FA_OK) return rc;
+  p.S = static_cast<int>(S);
+  const int dtype = cache->dtype;
+  return run_on(device, "b200fa_paged_gather",
+                [&](int* n) { return launch_paged_gather(p, dtype, static_cast<cudaStream_t>(stream), n); });
+}
+
+int b200fa_paged_attention(const b200fa_paged_kv* cache, const b200fa_tensor4* q, const b200fa_tensor4* out, float* lse,
+                           int64_t window, int64_t sinks, float scale, int64_t longest, void* stream, int device,
+                           uint32_t* status_word) {
+  AttendParams p;
+  std::memset(&p, 0, sizeof(p));
+  int rc = check_cache(cache, status_word, &p.c);
+  if (rc != B200FA_OK) return rc;
+  if (!q || !out || !lse) return B200FA_ERR_NULL;
+  const int64_t B = p.c.B, Hq = q->shape[1], S = q->shape[2];
+  if (Hq <= 0 || Hq > 65535 || S <= 0 || S > (1 << 24) || Hq % p.c.Hkv != 0) return B200FA_ERR_BAD_SHAPE;
+  // one row of thread blocks per KV head and 8 query rows of its group
+  if (Hq * S > INT_MAX / 2 || p.c.Hkv * ((Hq / p.c.Hkv * S + 7) / 8) > 65535) return B200FA_ERR_BAD_SHAPE;
+  if (window < 0 || sinks < 0 || longest < 0) return B200FA_ERR_UNSUPPORTED;
+  if (!(scale > 0.f) || !std::isfinite(scale)) return B200FA_ERR_UNSUPPORTED;
+  if (reinterpret_cast<uintptr_t>(lse) % 4 != 0) return B200FA_ERR_MISALIGNED;
+  if ((rc = check_view(q, B, Hq, S, p.c.D, cache->dtype, &p.q)) != B200FA_OK) return rc;
+  if ((rc = check_view(out, B, Hq, S, p.c.D, cache->dtype, &p.out, true)) != B200FA_OK) return rc;
+  p.lse = lse;
+  p.Hq = static_cast<int>(Hq); p.S = static_cast<int>(S);
+  p.window = static_cast<int>(std::min(window, kMaxWindow));
+  p.sinks = window ? static_cast<int>(std::min(sinks, kMaxWindow)) : 0;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  int64_t keys = longest > 0 && longest < p.c.capacity ? longest : p.c.capacity;
+  if (window) keys = std::min<int64_t>(keys, int64_t(p.window) + p.sinks + S - 1);
+  const int dtype = cache->dtype;
+  return run_on(device, "b200fa_paged_attention",
+                [&](int* n) { return launch_paged_attention(p, dtype, keys, static_cast<cudaStream_t>(stream), n); });
+}
+
 int b200fa_selftest_wait_timeout(uint32_t* status_word, long long budget_cycles, void* stream, int device) {
   if (!status_word) return B200FA_ERR_NULL;
   if (budget_cycles <= 0 || budget_cycles > kWaitBudgetCycles) return B200FA_ERR_UNSUPPORTED;
@@ -703,6 +828,7 @@ void b200fa_dropout_bytes_host(uint64_t philox_seed, uint64_t philox_offset, int
 
 int b200fa_status_to_error(uint32_t status_value) {
   if (status_value == 0) return B200FA_OK;
+  if ((status_value & 0xffff0000u) == kStatusBadIndex) return B200FA_ERR_BAD_INDEX;
   return (status_value & 0xffff0000u) == kStatusWaitTimeout ? B200FA_ERR_TIMEOUT : B200FA_ERR_CUDA;
 }
 

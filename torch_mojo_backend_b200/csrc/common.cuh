@@ -99,6 +99,39 @@ __host__ __device__ __forceinline__ KeyBlocks window_blocks(int p_first, int p_l
 
 constexpr int kSplitkvCluster = 16;   // splits of a KV head that may merge as a cluster
 
+// A validated paged cache of B sequences (see paged.cu).
+struct PagedCache {
+  void *k, *v;                  // (pages, Hkv, page, D) 16-bit elements or D / 2 bytes of codes
+  void *k_scales, *v_scales;    // 4 bits: (pages, Hkv, page, D / 32, 2)
+  const int32_t* table;         // (B, table_stride)
+  const int32_t* lengths;       // (B): tokens in the cache, the new ones included
+  const int32_t* new_lengths;   // (B) or null: all of a call's S tokens are new
+  int64_t table_stride;
+  int B, Hkv, D, bits;
+  int shift;                    // log2 of the page size
+  int pages, capacity;          // of the pool; tokens that a row of the table has pages for
+  uint32_t* status;
+};
+struct AppendParams {
+  PagedCache c;
+  View4 q, k, v, q_out;         // (B, H, S, D); q and q_out only if Hq > 0
+  const float *cos, *sin;       // (positions, rotary / 2)
+  int Hq, S, rotary, positions, interleaved;
+};
+struct GatherParams {
+  PagedCache c;
+  View4 k, v;                   // (B, Hkv, S, D)
+  int S;
+};
+struct AttendParams {
+  PagedCache c;
+  View4 q, out;                 // (B, Hq, S, D)
+  float* lse;                   // (B, Hq, S)
+  int Hq, S, window, sinks;     // window 0: none
+  int row_tiles;                // set by the launcher
+  float scale_log2;
+};
+
 // mask of a tensor-core kernel: every key, the causal diagonal, or the diagonal with a window and sinks
 constexpr int kAll = 0, kCausalMask = 1, kWindowMask = 2;
 
@@ -116,6 +149,10 @@ cudaError_t launch_fwd_splitkv(const SplitKvParams& p, int dtype, cudaStream_t s
 cudaError_t launch_bwd_sm100(const BwdParams& p, int dtype, cudaStream_t stream, int* launches);
 cudaError_t launch_bwd_simt(const BwdParams& p, int dtype, cudaStream_t stream, int* launches);
 int bwd_sink_chunks(const BwdParams& p);   // the tensor-core backward's sink_chunks (host only; sizes, mask, window and sinks are read)
+cudaError_t launch_paged_append(const AppendParams& p, int dtype, cudaStream_t stream, int* launches);
+cudaError_t launch_paged_gather(const GatherParams& p, int dtype, cudaStream_t stream, int* launches);
+// `keys`: the most that a query row can see, as far as the host knows
+cudaError_t launch_paged_attention(const AttendParams& p, int dtype, int64_t keys, cudaStream_t stream, int* launches);
 // A one-warp kernel whose only job is to wait, with `budget` SM cycles, on a barrier nobody
 // arrives at: exercises the bounded-wait give-up path without touching the attention kernels.
 cudaError_t launch_wait_timeout_selftest(uint32_t* status, long long budget, cudaStream_t stream, int* launches);

@@ -17,6 +17,7 @@ namespace b200fa {
 // ---------------------------------------------------------------------------------------
 constexpr uint32_t kStatusOk = 0;
 constexpr uint32_t kStatusWaitTimeout = 0x57410000u;  // | site id in the low 16 bits
+constexpr uint32_t kStatusBadIndex = 0x42490000u;     // | site id: a page, length or position out of range
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

@@ -10,6 +10,7 @@ kernels on torch's current stream.
 from __future__ import annotations
 
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -196,3 +197,159 @@ def window_bwd(dout, q, k, v, out, lse, *, window: int, sinks: int = 0, causal=T
     if rc != _lib.OK:
         raise _lib.B200FAError(rc, "b200fa_window_bwd")
     return dq, dk, dv
+
+
+class PagedKV(NamedTuple):
+    """The pages of a key/value cache: a pool that the sequences' block tables name pages of.
+
+    16 bits: ``k`` and ``v`` are (pages, Hkv, page_size, D) bfloat16 or float16.  4 bits: they are uint8 codes, two to a byte,
+    (pages, Hkv, page_size, D / 2), and ``k_scales`` and ``v_scales`` hold a scale and a minimum of the 16-bit type for every 32
+    elements, (pages, Hkv, page_size, D / 32, 2); an element is code * scale + minimum (the order of the codes: see
+    ``b200fa_paged_kv`` in include/b200fa.h).  ``page_size`` is a power of two from 16 to 4096.
+    """
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scales: torch.Tensor | None = None
+    v_scales: torch.Tensor | None = None
+
+    @classmethod
+    def empty(cls, pages: int, heads: int, page_size: int, head_dim: int, *, dtype=torch.bfloat16, bits: int = 16,
+              device="cuda") -> "PagedKV":
+        """A pool whose contents are not set."""
+        dtype_code(dtype)
+        if bits == 16:
+            return cls(*(torch.empty((pages, heads, page_size, head_dim), dtype=dtype, device=device) for _ in range(2)))
+        if bits != 4 or head_dim % 64:
+            raise NotImplementedError(f"a paged cache has 16 or 4 bits and a head dimension of 64 or 128, got {bits} and {head_dim}")
+        codes = [torch.empty((pages, heads, page_size, head_dim // 2), dtype=torch.uint8, device=device) for _ in range(2)]
+        return cls(*codes, *(torch.empty((pages, heads, page_size, head_dim // 32, 2), dtype=dtype, device=device)
+                             for _ in range(2)))
+
+    @property
+    def dtype(self) -> torch.dtype:
+        """The 16-bit type of the elements, or of the scales."""
+        return (self.k if self.k_scales is None else self.k_scales).dtype
+
+
+def _int32(name, t, shape, device) -> int:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} has to be a contiguous int32 tensor of shape {shape} on {device}")
+    return t.data_ptr()
+
+
+def _paged(cache: PagedKV, block_table, lengths, new_lengths, batch: int) -> _lib.PagedCache:
+    """The cache as the library takes it; pointers are all that it sees, so types, shapes and devices are checked here."""
+    k, v, ks, vs = cache
+    _need_cuda(k)
+    device, four = k.device, ks is not None
+    dtype = dtype_code(cache.dtype)
+    if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or v.device != device or not (k.is_contiguous() and v.is_contiguous()):
+        raise ValueError("the pages of k and v have to be contiguous and alike, (pages, heads, page_size, head_dim)")
+    pages, heads, page_size, width = k.shape
+    if four:
+        if k.dtype != torch.uint8:
+            raise ValueError("4-bit pages are uint8 codes")
+        width *= 2
+        want = (pages, heads, page_size, width // 32, 2)
+        for s in (ks, vs):
+            if s is None or tuple(s.shape) != want or s.dtype != ks.dtype or s.device != device or not s.is_contiguous():
+                raise ValueError(f"the scales of a 4-bit cache have to be contiguous and alike, {want}")
+    elif vs is not None:
+        raise ValueError("16-bit pages have no scales")
+    if (block_table.dim() != 2 or block_table.shape[0] != batch or block_table.dtype != torch.int32 or block_table.device != device
+            or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
+        raise ValueError(f"the block table has to be int32, (batch = {batch}, pages of a sequence), on {device}")
+    return _lib.PagedCache.make(
+        k.data_ptr(), v.data_ptr(), ks.data_ptr() if four else 0, vs.data_ptr() if four else 0, block_table.data_ptr(),
+        _int32("lengths", lengths, (batch,), device),
+        _int32("new_lengths", new_lengths, (batch,), device) if new_lengths is not None else 0,
+        pages, heads, page_size, width, batch, block_table.shape[1], block_table.stride(0), dtype, 4 if four else 16)
+
+
+def paged_append(k, v, cache: PagedKV, block_table, lengths, *, new_lengths=None, rotary=None, interleaved: bool = False, q=None,
+                 q_out=None, status=None):
+    """Writes the new tokens' ``k`` and ``v`` (B, Hkv, S, D) to the pages, k rotated by position, and returns the rotated ``q``.
+
+    ``block_table``: (B, pages of a sequence) int32; ``lengths``: (B,) int32, tokens in the cache with the new ones;
+    ``new_lengths``: (B,) int32, how many of the S tokens are new ones (the first of each row; None: all).  Token s is written at
+    position ``length - new + s``.  ``rotary``: (cos, sin), float32 (positions, R / 2): the first R elements turn, in pairs
+    (i, i + R / 2) or, ``interleaved``, (2 i, 2 i + 1).  ``q``: (B, Hq, S, D), rotated the same way to ``q_out`` (a new tensor by
+    default; q itself will do), whose rows behind a sequence's new tokens are left as they are (zero in a new tensor).  ``status``: see
+    ``include/b200fa.h``.
+    """
+    B, Hkv, S, D = k.shape
+    c = _paged(cache, block_table, lengths, new_lengths, B)
+    if D != c.head_dim or Hkv != c.heads or k.dtype != cache.dtype or k.device != cache.k.device:
+        raise ValueError(f"k and v have to be {cache.dtype} of {c.heads} heads of {c.head_dim} on {cache.k.device}")
+    _same_kind(k, (v, q, q_out))
+    cos_ptr = sin_ptr = rotary_dim = positions = 0
+    if rotary is not None:
+        cos, sin = rotary
+        if cos.dim() != 2 or sin.shape != cos.shape or any(
+                t.dtype != torch.float32 or t.device != k.device or not t.is_contiguous() for t in (cos, sin)):
+            raise ValueError(f"rotary is (cos, sin), contiguous float32 (positions, R / 2) on {k.device}")
+        cos_ptr, sin_ptr, positions, rotary_dim = cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1]
+    if q is None and q_out is not None:
+        raise ValueError("q_out without q")
+    if q is not None and q_out is None:
+        make = torch.empty if new_lengths is None else torch.zeros
+        q_out = make(tuple(q.shape), dtype=q.dtype, device=q.device)
+    stream, dev = _stream_and_device(k)
+    rc = _lib.paged_append(c, t4(k), t4(v), t4(q) if q is not None else None, t4(q_out) if q is not None else None, cos_ptr, sin_ptr,
+                           rotary_dim, positions, interleaved, stream, dev, status.data_ptr() if status is not None else 0)
+    if rc != _lib.OK:
+        raise _lib.B200FAError(rc, "b200fa_paged_append")
+    return q_out
+
+
+def paged_attention(q, cache: PagedKV, block_table, lengths, *, new_lengths=None, window: int = 0, sinks: int = 0,
+                    scale: float | None = None, out=None, lse=None, longest: int = 0, status=None):
+    """out, lse = causal attention of the newest tokens' ``q`` (B, Hq, S, D) over the pages of their sequences.
+
+    ``block_table``, ``lengths`` and ``new_lengths`` as for ``paged_append``, which comes first: the new tokens see each other and
+    themselves.  ``window`` > 0: the last ``window`` keys and the first ``sinks`` ones alone.  Rows behind a sequence's new tokens
+    are left as they are (out zero and lse -inf in new tensors).  ``longest``: a hint, the longest of the lengths, where the block
+    table is much wider.
+    """
+    B, Hq, S, D = q.shape
+    c = _paged(cache, block_table, lengths, new_lengths, B)
+    if D != c.head_dim or q.dtype != cache.dtype or q.device != cache.k.device:
+        raise ValueError(f"q has to be {cache.dtype} of head dimension {c.head_dim} on {cache.k.device}")
+    if scale is None:
+        scale = default_scale(D)
+    if out is None:
+        out = (torch.empty if new_lengths is None else torch.zeros)((B, Hq, S, D), dtype=q.dtype, device=q.device)
+    if lse is None:
+        lse = torch.empty((B, Hq, S), dtype=torch.float32, device=q.device)
+        if new_lengths is not None:
+            lse.fill_(-math.inf)
+    else:
+        _fp32_statistic(lse, (B, Hq, S), q.device)
+    _same_kind(q, (out,))
+    stream, dev = _stream_and_device(q)
+    rc = _lib.paged_attention(c, t4(q), t4(out), lse.data_ptr(), window, sinks, float(scale), longest, stream, dev,
+                              status.data_ptr() if status is not None else 0)
+    if rc != _lib.OK:
+        raise _lib.B200FAError(rc, "b200fa_paged_attention")
+    return out, lse
+
+
+def paged_gather(cache: PagedKV, block_table, lengths, length: int, *, k=None, v=None, status=None):
+    """k, v = the first ``length`` tokens of every sequence, (B, Hkv, length, D) of the cache's 16-bit type; rows behind a
+    sequence's own length are zero.  ``k`` and ``v``: tensors to write to."""
+    B = lengths.shape[0]
+    c = _paged(cache, block_table, lengths, None, B)
+    shape = (B, c.heads, length, c.head_dim)
+    if k is None:
+        k = torch.empty(shape, dtype=cache.dtype, device=cache.k.device)
+    if v is None:
+        v = torch.empty(shape, dtype=cache.dtype, device=cache.k.device)
+    for t in (k, v):
+        if tuple(t.shape) != shape or t.dtype != cache.dtype or t.device != cache.k.device:
+            raise ValueError(f"k and v have to be {cache.dtype} of shape {shape} on {cache.k.device}")
+    stream, dev = _stream_and_device(cache.k)
+    rc = _lib.paged_gather(c, t4(k), t4(v), stream, dev, status.data_ptr() if status is not None else 0)
+    if rc != _lib.OK:
+        raise _lib.B200FAError(rc, "b200fa_paged_gather")
+    return k, v
