@@ -2,7 +2,8 @@
 
 Bounds of the attention, element by element (u half a step of the type, s the relative error of a probability, A = P |V|):
   16 bits: P is rounded to the type before it multiplies V, out after        u A + u |out| + 3 s A
-  4 bits:  P vs is rounded to bf16 (2^-9) before it multiplies the codes     2^-8 sum(P vs c) + u |out| + 3 s (A + sum(P vs c) + sum(P |vm|))
+  4 bits:  P vs is rounded to the type before it multiplies c - 8; the rest, P (vm + 8 vs), is fp32
+           u sum(P vs |c - 8|) + u |out| + 3 s (sum(P vs |c - 8|) + sum(P |vm + 8 vs|));  scores: sums of q ks c and of q km
 A float16 has no step below 2^-24: t = 2^-25 more for each rounding to it.  Appending and reading back round once, in a given
 order: their results are equal to the formula in fp32, bit for bit.
 """
@@ -93,7 +94,8 @@ class Pool:
             scales[page, :, slot] = torch.stack([scale, low], -1)
 
     def held(self, b, n=None):
-        """k, v of sequence b as the cache holds them, (Hkv, n, D) in 32 bits, and of v what the bound needs."""
+        """k, v of sequence b as the cache holds them, (Hkv, n, D) in 32 bits, and with 4 bits the sizes of the two parts that the
+        kernel takes them in: scale * code and minimum (of a value: code - 8 and the minimum + 8 scales)."""
         n = self.k[b].shape[1] if n is None else n
         page, slot = self.place(b, 0, n)
         got = []
@@ -104,9 +106,10 @@ class Pool:
                 got.append((rows.float(), rows.float().abs(), None))
                 continue
             s = scales[page, :, slot].transpose(0, 1).float()
-            scaled = unpacked(rows, element).unflatten(-1, (-1, 32)) * s[..., :1]
-            low = s[..., 1:].expand_as(scaled)
-            got.append(((scaled + low).flatten(-2), scaled.flatten(-2), low.abs().flatten(-2)))
+            codes = unpacked(rows, element).unflatten(-1, (-1, 32))
+            middle = 0 if pages is self.cache.k else 8
+            parts = (codes * s[..., :1] + s[..., 1:], (codes - middle).abs() * s[..., :1], (s[..., 1:] + middle * s[..., :1]).abs().expand_as(codes))
+            got.append(tuple(x.flatten(-2) for x in parts))
         return got
 
 
@@ -129,26 +132,18 @@ def expected(pool, q, b, n, window, sinks):
     p = torch.exp(s - lse.clamp(min=-1e300)[..., None])
     out = p @ v
     a = p @ v.abs()
-    # an fp32 sum of D products, each at most 2^-23 off (4 bits: of code + 16 sixteenths, and of the minimum's part: 4 times the size)
+    # an fp32 sum of D products, each at most 2^-23 off
     size = float((q.abs() @ k.abs().mT).max()) * D ** -0.5
     if pool.bits == 4:
         (_, ks, km), _ = pool.held(b)
-        ks, km = (x.double().repeat_interleave(group, 0) for x in (ks, km))
-        steps = ks + 16 * (ks / unit_codes(pool, b).repeat_interleave(group, 0).clamp(min=1))   # scale * (code + 16) or more
-        size = float((q.abs() @ (steps + km).mT).max()) * D ** -0.5
+        size = float((q.abs() @ (ks + km).double().repeat_interleave(group, 0).mT).max()) * D ** -0.5
     e = size * D * 2 ** -23 + 2.0 ** -20 + int(seen.sum(1).max()) * 2.0 ** -24
     if pool.bits == 16:
         bound = u * (a + out.abs()) + t + t * (seen.double() @ v.abs()) + 3 * e * a
     else:
         low = low.double().repeat_interleave(group, 0)
-        bound = 2.0 ** -8 * (p @ scaled) + u * out.abs() + t + 3 * e * (a + p @ scaled + p @ low)
+        bound = u * (p @ scaled) + u * out.abs() + t + t * 8 * seen.sum(1, keepdim=True) + 3 * e * (p @ scaled + p @ low)
     return (out, bound), (lse, e + 2.0 ** -22 * lse.abs())
-
-
-def unit_codes(pool, b):
-    """The codes of sequence b's keys, (Hkv, n, D)."""
-    page, slot = pool.place(b, 0, pool.k[b].shape[1])
-    return unpacked(pool.cache.k[page, :, slot], k_element(pool.D)).transpose(0, 1).double()
 
 
 def check(name, got, want, bound):

@@ -367,6 +367,8 @@ int check_cache(const b200fa_paged_kv* t, uint32_t* status_word, PagedCache* c) 
   if (t->pages <= 0 || t->pages > INT_MAX || t->heads <= 0 || t->heads > 65535 || t->batch <= 0 || t->batch > 65535) return B200FA_ERR_BAD_SHAPE;
   if (t->table_width <= 0 || t->table_width > (1 << 24) / t->page_size) return B200FA_ERR_BAD_SHAPE;   // 2^24 tokens, as everywhere
   if (t->table_stride < t->table_width && t->batch > 1) return B200FA_ERR_BAD_STRIDE;
+  // rows of the pool are counted in 32 bits (2^32 of the smallest, 40 bytes of k and v each, are more than a GPU holds)
+  if (t->pages * t->heads > (int64_t(1) << 32) / t->page_size - 1) return B200FA_ERR_BAD_SHAPE;
   for (const void* x : {t->k, t->v, t->k_scales, t->v_scales})
     if (reinterpret_cast<uintptr_t>(x) % 16 != 0) return B200FA_ERR_MISALIGNED;
   for (const int32_t* x : {t->table, t->lengths, t->new_lengths})
@@ -790,6 +792,7 @@ int b200fa_paged_attention(const b200fa_paged_kv* cache, const b200fa_tensor4* q
   p.window = static_cast<int>(std::min(window, kMaxWindow));
   p.sinks = window ? static_cast<int>(std::min(sinks, kMaxWindow)) : 0;
   p.scale_log2 = scale * 1.4426950408889634f;
+  p.wait_budget = wait_budget();
   int64_t keys = longest > 0 && longest < p.c.capacity ? longest : p.c.capacity;
   if (window) keys = std::min<int64_t>(keys, int64_t(p.window) + p.sinks + S - 1);
   const int dtype = cache->dtype;

@@ -129,7 +129,9 @@ struct AttendParams {
   float* lse;                   // (B, Hq, S)
   int Hq, S, window, sinks;     // window 0: none
   int row_tiles;                // set by the launcher
+  long long wait_budget;        // SM cycles that a wait for a copy may take
   float scale_log2;
+  uint32_t one_f16, one_bf16;   // kOneF16, kOneBf16 (paged.cu)
 };
 
 // mask of a tensor-core kernel: every key, the causal diagonal, or the diagonal with a window and sinks

@@ -11,7 +11,8 @@
 //
 // Every index that comes from device memory (pages, lengths, positions) is checked before it is used.  What depends on a bad one
 // is not written (append) or is NaN (attention, reading back), and the status word says so.
-#include <atomic>
+#include <algorithm>
+#include <cmath>
 #include <mutex>
 
 #include <cuda_bf16.h>
@@ -260,19 +261,20 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(const GatherParams p)
 //   * 16 bits: K as thread (g, t) reads 16 bytes at (4i + t) 16 of key rows g and g + 8 (any permutation of the contraction
 //     index will do if Q has the same); V as it reads 16 bytes at 128 h + 16 g of rows 2t, 2t+1, 2t+8, 2t+9, whose registers a
 //     byte permute turns into (key, key + 1) pairs.
-//   * 4 bits: a code c goes into the mantissa of 1.0, which makes 1 + c / 16 exactly, two codes per instruction; the scales stay
-//     out of the products.  S = sum over groups G of 16 ks_G (q_G . c_G / 16) + km_G sum(q_G): the accumulator of a group
-//     starts at -sum(q_G), which takes the ones off.  O_G = sum over keys of (P vs_G) c + P vm_G: P vs_G is the B operand, rounded
-//     to bf16 whatever the cache's type (fp16 has not the range for a probability times a small scale), the ones are taken off
-//     the codes, exactly, and sum(P vm_G) is the same for the 32 elements of a group: one fp32 number per row and group.
-// The row maximum moves only when a score exceeds it by 2^8 (a vote per step instead of six shuffles), so P is at most 256.
+//   * 4 bits: the codes are operands, the scales stay out of the products.  S = sum over groups G of ks_G (q_G . c_G) +
+//     km_G sum(q_G), with the codes as fp16 and q as fp16, a row of it multiplied by the power of two that brings its largest
+//     element to 1..2 (exact but for elements below 2^-14 of that one, which are off by 2^-25 of it); sum over G of km_G sum(q_G) is
+//     one more product, keys by groups, of sum(q_G) in three parts of the type.  O_G = sum over keys of (P vs_G) (c - 8) +
+//     P (vm_G + 8 vs_G): P vs_G is the B operand, rounded to the cache's type, c - 8 is exact, and the second sum, the same for
+//     the 32 elements of a group, is one product as well, (vs, vm) of the groups by keys times P as rounded to the type.  (Codes of
+//     0..15 instead would make both sums several times their difference, and the rounding of P vs_G with them.)
+// The row maximum moves only when a score exceeds it by 2^8 (a vote per step instead of six shuffles), so P is at most 256; at
+// most 4 where P vs_G is an fp16, whose largest scale is 8734.
 // Keys that no row of the unit sees are never read, not even into a product with zero: their places in a step re-read a key that is
 // seen (pages behind a window may have been given to another sequence).
 // ------------------------------------------------------------------------------------------
 constexpr int kStepKeys = 16;
-constexpr int kWarps = 4;
 constexpr int kMaxPeers = 16;
-constexpr float kLazy = 8.f;
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -293,59 +295,234 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
 }
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// Codes j of both halves of a word, each as 1 + code / 16
-template <typename T, int j>
-__device__ __forceinline__ uint32_t codes_plus_one(uint32_t w) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {   // 7 bits of mantissa: the code goes to bits 3..6
-    constexpr int s = 4 * j - 3;
-    return ((s < 0 ? w << -s : w >> (s < 0 ? 0 : s)) & 0x00780078u) | 0x3f803f80u;
-  } else {                                                 // 10 bits: to bits 6..9
-    constexpr int s = 4 * j - 6;
-    return ((s < 0 ? w << (s < 0 ? -s : 0) : w >> (s < 0 ? 0 : s)) & 0x03c003c0u) | 0x3c003c00u;
-  }
+// The codes of a word (four in each half) as four pairs, one from each half, of the same place, less `minus` (0 or 8).  The logic
+// unit, at half the rate of the others, binds the unpacking.  An fp16 1024 has ten mantissa bits below it: codes at bits 0..3 or
+// 4..7 make 1024 + c and 1024 + 16 c, and a half-precision FMA takes the rest off, exactly: five logic instructions a word.  A
+// bf16 128 has seven, which take one code: seven instructions a word.
+// `one`: the 1024 or 128 in both halves, kOneF16 or kOneBf16, from the launch: the compiler makes two instructions of a mask and a
+// bit pattern that it knows, since one takes one immediate.
+constexpr uint32_t kOneF16 = 0x64006400u, kOneBf16 = 0x43004300u;
+__device__ __forceinline__ uint32_t masked_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));   // (w & mask) | bits
+  return r;
 }
-__device__ __forceinline__ uint32_t minus_one_bf16x2(uint32_t x) {
-  const __nv_bfloat162 one = __floats2bfloat162_rn(1.f, 1.f);
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), one);
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
-// 16 keys in registers
-template <int kD, int kBits>
-struct Fragments;
-template <int kD>
-struct Fragments<kD, 16> {
-  uint4 k[2][kD / 32];   // key rows g, g + 8
-  uint4 v[4][kD / 64];   // key rows 2t, 2t + 1, 2t + 8, 2t + 9
-};
-template <int kD>
-struct Fragments<kD, 4> {
-  uint32_t k[2][kD / 32];    // codes of key rows g, g + 8
-  uint32_t ks[2][kD / 32];   // (scale, minimum) of their groups
-  uint32_t vs[2][kD / 32];   // ... of the value rows g, g + 8
-  uint32_t v[4][kD / 64];    // codes of value rows 2t, 2t + 1, 2t + 8, 2t + 9
-};
-template <int kN>
-__device__ __forceinline__ void load_words(const uint32_t* p, uint32_t (&w)[kN]) {
-  if constexpr (kN == 4) {
-    const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
-    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-  } else if constexpr (kN == 2) {
-    const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
-    w[0] = x.x; w[1] = x.y;
+template <typename T>
+__device__ __forceinline__ void codes_of(uint32_t w, float minus, uint32_t one, uint32_t (&c)[4]) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const uint32_t w8 = w >> 8;
+    c[0] = masked_or(w, 0x000f000fu, one);
+    c[1] = masked_or(w, 0x00f000f0u, one);
+    c[2] = masked_or(w8, 0x000f000fu, one);
+    c[3] = masked_or(w8, 0x00f000f0u, one);
+    const __half2 lo = __float2half2_rn(-1024.f - minus), hi = __float2half2_rn(-64.f - minus), sixteenth = __float2half2_rn(0.0625f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __half2 x = *reinterpret_cast<const __half2*>(&c[j]);
+      const __half2 y = j & 1 ? __hfma2(x, sixteenth, hi) : __hadd2(x, lo);
+      c[j] = *reinterpret_cast<const uint32_t*>(&y);
+    }
   } else {
-    w[0] = __ldg(p);
+    const __nv_bfloat162 off = __float2bfloat162_rn(-128.f - minus);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      c[j] = masked_or(w >> (4 * j), 0x000f000fu, one);
+      const __nv_bfloat162 y = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&c[j]), off);
+      c[j] = *reinterpret_cast<const uint32_t*>(&y);
+    }
   }
 }
 
-// The last step of a unit: every block has left its unnormalised O of row r at o + r * (kD + 2) and the row's (max, sum) at ml + r, and
-// merges its share of (row, pair of elements) from its peers' shared memory.
-template <typename T, int kD, int kRows>
-__device__ __forceinline__ void merge_peers(const AttendParams& p, int b, int hk, int group, int row0, int rows, int peers, int rank, const float* o,
-                                            const float2* ml) {
-  const int tid = threadIdx.x;
+// The rows and keys of one unit, as a block sees them.
+struct Unit {
+  int b, hk, row0, rows, group;      // rows row0 .. row0 + rows - 1 of the group's (new tokens x query heads)
+  int first_pos, p_first, p_last;    // positions of the first new token, of the unit's first row and of its last
+  KeyBlocks list;                    // steps of keys
+  int hidden_from, hidden_to;        // keys between the sinks and the first row's window
+  int low;                           // a step that begins at or below it holds keys ahead of some row's window; -1 without one
+  int begin, end;                    // the block's share of the steps
+  bool good;                         // the sequence's numbers can be
+};
+template <int kKeys>
+__device__ __forceinline__ Unit unit_of(const AttendParams& p, int max_rows) {
+  Unit u;
+  u.b = blockIdx.z;
+  u.hk = blockIdx.y / p.row_tiles;
+  u.row0 = (blockIdx.y - u.hk * p.row_tiles) * max_rows;
+  u.group = p.Hq / p.c.Hkv;
+  Sequence seq;
+  u.good = sequence_of(p.c, u.b, p.S, &seq);
+  if (!u.good) {   // every row of the sequence is NaN
+    if (threadIdx.x == 0) report_bad_index(p.c.status, 6);
+    seq.len = 0;
+    seq.n = p.S;
+  }
+  u.rows = min(max_rows, seq.n * u.group - u.row0);
+  u.first_pos = seq.len - seq.n;   // negative: the token sees nothing
+  u.p_first = u.first_pos + u.row0 / u.group;
+  u.p_last = u.first_pos + (u.row0 + max(u.rows, 1) - 1) / u.group;
+  u.list = KeyBlocks{0, 0, max(0, u.p_last + kKeys) / kKeys};
+  u.hidden_from = u.hidden_to = 0;
+  u.low = -1;
+  if (p.window) {
+    u.list = window_blocks<kKeys>(u.p_first, u.p_last, seq.len, p.window, p.sinks);
+    u.hidden_from = p.sinks;
+    u.hidden_to = u.p_first - p.window + 1;
+    u.low = u.p_last - p.window;
+  }
+  const int peers = gridDim.x, rank = blockIdx.x;
+  u.begin = static_cast<int>(static_cast<int64_t>(u.list.n) * rank / peers);
+  u.end = static_cast<int>(static_cast<int64_t>(u.list.n) * (rank + 1) / peers);
+  return u;
+}
+// place in a step of the key that is read for key `k` of it
+template <int kKeys>
+__device__ __forceinline__ int place(const Unit& u, int base, int k) {
+  int key = min(base + k, u.p_last);
+  if (key >= u.hidden_from && key < u.hidden_to) key = u.hidden_to < base + kKeys ? u.hidden_to : u.hidden_from - 1;
+  return key - base;
+}
+// every key of the step is one that some row sees
+template <int kKeys>
+__device__ __forceinline__ bool whole_step(const Unit& u, int base) {
+  return base + kKeys - 1 <= u.p_last && (base >= u.hidden_to || base + kKeys - 1 < u.hidden_from);
+}
+// some key of the step is one that some row does not see
+template <int kKeys>
+__device__ __forceinline__ bool edge_step(const Unit& u, const AttendParams& p, int base) {
+  return base + kKeys - 1 > u.p_first || (base <= u.low && base + kKeys - 1 >= p.sinks);
+}
+template <typename T>
+__device__ __forceinline__ const T* query_row(const AttendParams& p, const Unit& u, int r) {
+  const int s = (u.row0 + r) / u.group, h = u.hk * u.group + u.row0 + r - s * u.group;
+  return reinterpret_cast<const T*>(p.q.ptr) + static_cast<int64_t>(u.b) * p.q.sb + static_cast<int64_t>(h) * p.q.sh + static_cast<int64_t>(s) * p.q.ss;
+}
+// row of the pages that holds the first key of a step, which lies in page `page`; page 0 and `bad` for one that is none
+__device__ __forceinline__ uint32_t page_row(const PagedCache& c, int hk, int page, int base, bool* bad) {
+  if (static_cast<unsigned>(page) >= static_cast<unsigned>(c.pages)) {
+    *bad = true;
+    page = 0;
+  }
+  return (static_cast<uint32_t>(page * c.Hkv + hk) << c.shift) + (base & ((1 << c.shift) - 1));
+}
+
+// What a warp holds of its rows: thread (g, t) has rows 2t and 2t + 1 of each tile of eight.
+template <int kNT, int kTiles, bool kZ>
+struct RowState {
+  float m[kNT][2], shift[kNT][2], limit[kNT][2], l[kNT][2];   // shift: -m, 0 as long as there is none; limit: where it moves
+  float o[kNT][kTiles][4];   // O^T: [0] (slot g, row 2t) [1] (slot g, row 2t + 1) [2], [3] slot g + 8
+  float z[kZ ? kNT : 1][4];  // 4 bits: sums of P vs (slots g < D / 32) and P vm (the next D / 32)
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int n = 0; n < kNT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[n][e] = limit[n][e] = -INFINITY;
+        shift[n][e] = l[n][e] = 0.f;
+        if (kZ) z[n][e] = z[n][2 + e] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+    }
+  }
+  // raises the maxima of the rows that have a score above theirs, and rescales what was summed
+  template <int kH>
+  __device__ __forceinline__ void raise(float (&x)[kH][kNT][4], float lazy) {
+    constexpr unsigned kFull = 0xffffffffu;
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float top = fmaxf(x[0][n][e], x[0][n][2 + e]);
+        if (kH == 2) top = fmaxf(top, fmaxf(x[kH - 1][n][e], x[kH - 1][n][2 + e]));
+        top = fmaxf(top, __shfl_xor_sync(kFull, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(kFull, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(kFull, top, 16));   // relative to the standing maximum (to 0 without one)
+        const bool none = m[n][e] == -INFINITY;
+        if (top > (none ? -INFINITY : 0.f)) {
+          const float corr = none ? 0.f : exp2f(-top);
+          m[n][e] = none ? top : m[n][e] + top;
+          shift[n][e] = -m[n][e];
+          limit[n][e] = lazy;
+#pragma unroll
+          for (int h = 0; h < kH; ++h) {
+            x[h][n][e] -= top;
+            x[h][n][2 + e] -= top;
+          }
+          l[n][e] *= corr;
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j) {
+            o[n][j][e] *= corr;
+            o[n][j][2 + e] *= corr;
+          }
+          if (kZ) z[n][e] *= corr;
+        }
+      }
+  }
+  // scores less the rows' maxima, of kH times 16 keys, x[h][n][0] (key g, row 2t) [1] (key g, row 2t + 1) [2], [3] key g + 8, to
+  // probabilities
+  template <int kH>
+  __device__ __forceinline__ void probabilities(float (&x)[kH][kNT][4], float lazy) {
+    bool far = false;
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float top = fmaxf(x[0][n][e], x[0][n][2 + e]);
+        if (kH == 2) top = fmaxf(top, fmaxf(x[kH - 1][n][e], x[kH - 1][n][2 + e]));
+        far |= top > limit[n][e];
+      }
+    if (__any_sync(0xffffffffu, far)) raise(x, lazy);
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int h = 0; h < kH; ++h) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[h][n][e] = ex2_approx(x[h][n][e]);
+        l[n][0] += x[h][n][0] + x[h][n][2];   // this thread's keys; summed over g at the end
+        l[n][1] += x[h][n][1] + x[h][n][3];
+      }
+  }
+  // -inf for the scores of keys (`first` and `second` of this thread) that a row does not see
+  __device__ __forceinline__ void mask(float (&x)[kNT][4], const AttendParams& p, const Unit& u, int first, int second, int t) const {
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = e < 2 ? first : second;
+        const int pos = u.first_pos + (u.row0 + 8 * n + 2 * t + (e & 1)) / u.group;   // (rows behind the last are not written)
+        if (key > pos || (p.window && key <= pos - p.window && key >= p.sinks)) x[n][e] = -INFINITY;
+      }
+  }
+};
+
+// The last steps of a block: every warp has left its unnormalised O of row r at o + warp * stride + r * (kD + 2), and the row's max
+// and sum behind it.  They are merged in the block, then by the blocks of the cluster, each of which takes its share of (row, pair
+// of elements) from its peers' shared memory.
+template <typename T, int kD, int kWarps>
+__device__ __forceinline__ void merge(const AttendParams& p, const Unit& u, float* o, int stride, float2* ml) {
+  const int tid = threadIdx.x, peers = gridDim.x, rank = blockIdx.x;
+  __syncthreads();
+  for (int idx = tid; idx < u.rows * kD; idx += kWarps * 32) {
+    const int r = idx / kD, d = idx % kD;
+    const float* row = o + r * (kD + 2);
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, row[w * stride + kD]);
+    const float m_use = mm == -INFINITY ? 0.f : mm;
+    float acc = 0.f, ls = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float weight = exp2f(row[w * stride + kD] - m_use);
+      acc = fmaf(row[w * stride + d], weight, acc);
+      ls = fmaf(row[w * stride + kD + 1], weight, ls);
+    }
+    o[r * (kD + 2) + d] = acc;   // (this thread alone reads and writes column d of row r)
+    if (d == 0) ml[r] = make_float2(mm, ls);
+  }
   if (peers > 1) cluster_sync(); else __syncthreads();
-  for (int idx = rank * kWarps * 32 + tid; idx < rows * (kD / 2); idx += peers * kWarps * 32) {
+  for (int idx = rank * kWarps * 32 + tid; idx < u.rows * (kD / 2); idx += peers * kWarps * 32) {
     const int r = idx / (kD / 2), d = idx % (kD / 2) * 2;
     const uint32_t a_ml = smem_u32(ml + r), a_o = smem_u32(o + r * (kD + 2) + d);
     float2 v[kMaxPeers], x[kMaxPeers];
@@ -372,266 +549,120 @@ __device__ __forceinline__ void merge_peers(const AttendParams& p, int b, int hk
       }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;   // a row without a key is 0 with lse -inf; a NaN stays one
-    const int row = row0 + r, s = row / group, h = hk * group + row - s * group;
-    T* dst = reinterpret_cast<T*>(p.out.ptr) + static_cast<int64_t>(b) * p.out.sb + static_cast<int64_t>(h) * p.out.sh + static_cast<int64_t>(s) * p.out.ss + d;
+    const int row = u.row0 + r, s = row / u.group, h = u.hk * u.group + row - s * u.group;
+    T* dst = reinterpret_cast<T*>(p.out.ptr) + static_cast<int64_t>(u.b) * p.out.sb + static_cast<int64_t>(h) * p.out.sh + static_cast<int64_t>(s) * p.out.ss + d;
     *reinterpret_cast<uint32_t*>(dst) = pack_t<T>(o0 * inv, o1 * inv);
-    if (d == 0) p.lse[(static_cast<int64_t>(b) * p.Hq + h) * p.S + s] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+    if (d == 0) p.lse[(static_cast<int64_t>(u.b) * p.Hq + h) * p.S + s] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
   }
   if (peers > 1) cluster_sync();   // no block leaves while a peer may still read its shared memory
 }
 
-template <typename T, int kD, int kNT, int kBits>
-__global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? 3 : 2) paged_attention_kernel(const AttendParams p) {
-  constexpr int kRows = 8 * kNT;
-  constexpr int kGroups = kD / kGroup;
-  constexpr int kTiles = kD / 16;   // tiles of O^T
+// Blocks of four warps that an SM takes, by their registers; a block of `kWide` warps has an SM to itself.
+template <int kD, int kNT, int kBits>
+struct AttendCfg {
+  static constexpr int kPerSm = kNT == 2 ? 2 : kD == 128 && kBits == 16 ? 3 : 4;
+  static constexpr int kWide = 4 * kPerSm;
+  // 4 bits: a warp's ring of steps, each the rows of 32 keys: key codes, value codes, key scales, value scales
+  static constexpr int kKeys = kBits == 4 ? 32 : kStepKeys, kStages = kNT == 2 ? 4 : 2;
+  static constexpr int kCodeBytes = kKeys * kD / 2, kScaleBytes = kKeys * kD / kGroup * 4;
+  static constexpr int kStageBytes = 2 * kCodeBytes + 2 * kScaleBytes;
+  static constexpr int kMergeBytes = 8 * kNT * (kD + 2) * 4;   // a warp's results (in its ring, where it has one)
+  static constexpr int kWarpBytes = kBits == 4 ? kStages * kStageBytes : kMergeBytes;
+  static_assert(kWarpBytes >= kMergeBytes && kWarpBytes % 16 == 0, "results fit the ring");
+};
+
+// ---- 16 bits
+template <typename T, int kD, int kNT, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? AttendCfg<kD, kNT, 16>::kPerSm : 1) paged_attention_kernel(const AttendParams p) {
+  using Cfg = AttendCfg<kD, kNT, 16>;
   constexpr unsigned kFull = 0xffffffffu;
-  __shared__ __align__(16) float sMerge[kWarps][kRows][kD + 2];   // per warp and row: O, then max and sum
-  __shared__ float2 sML[kRows];
-  const int peers = gridDim.x, rank = blockIdx.x, b = blockIdx.z;
-  const int row_tiles = p.row_tiles;
-  const int hk = blockIdx.y / row_tiles, row0 = (blockIdx.y - hk * row_tiles) * kRows;
-  const int group = p.Hq / p.c.Hkv;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr float kLazy = 8.f;
+  extern __shared__ __align__(16) float smem_f[];
+  __shared__ float2 sML[8 * kNT];
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
+  const Unit u = unit_of<kStepKeys>(p, 8 * kNT);
+  if (u.rows <= 0) return;   // (all blocks of the cluster do)
 
-  Sequence seq;
-  bool good = sequence_of(p.c, b, p.S, &seq);
-  if (!good) {   // every row of the sequence is NaN
-    if (tid == 0) report_bad_index(p.c.status, 6);
-    seq.len = 0;
-    seq.n = p.S;
-  }
-  const int rows = min(kRows, seq.n * group - row0);   // of this unit
-  if (rows <= 0) return;                               // (all blocks of the cluster do)
-  const int first_pos = seq.len - seq.n;               // position of the first new token; negative: it sees nothing
-  const int p_first = first_pos + row0 / group, p_last = first_pos + (row0 + rows - 1) / group;
-  KeyBlocks list = {0, 0, max(0, p_last + kStepKeys) / kStepKeys};   // steps of 16 keys
-  int hidden_from = 0, hidden_to = 0;                                // keys between the sinks and the first row's window
-  if (p.window) {
-    list = window_blocks<kStepKeys>(p_first, p_last, seq.len, p.window, p.sinks);
-    hidden_from = p.sinks;
-    hidden_to = p_first - p.window + 1;
-  }
-  const int begin = static_cast<int>(static_cast<int64_t>(list.n) * rank / peers), end = static_cast<int>(static_cast<int64_t>(list.n) * (rank + 1) / peers);
-
-  // Q^T fragments of row 8n + g, and (4 bits) the sums of its groups
-  uint32_t qf[kNT][kD / 8];
-  float qs[kNT][2][kBits == 4 ? kGroups : 1];
-#pragma unroll
-  for (int n = 0; n < kNT; ++n) {
-    const int r = 8 * n + g;
-#pragma unroll
-    for (int i = 0; i < kD / 8; ++i) qf[n][i] = 0;
-    if (r < rows) {
-      const int s = (row0 + r) / group, h = hk * group + row0 + r - s * group;
-      const T* qp = reinterpret_cast<const T*>(p.q.ptr) + static_cast<int64_t>(b) * p.q.sb + static_cast<int64_t>(h) * p.q.sh + static_cast<int64_t>(s) * p.q.ss;
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i) {   // 32 elements: this thread's eight
-        const uint4 x = *reinterpret_cast<const uint4*>(qp + 32 * i + 8 * t);
-        if constexpr (kBits == 16) {
-          qf[n][4 * i] = x.x; qf[n][4 * i + 1] = x.y; qf[n][4 * i + 2] = x.z; qf[n][4 * i + 3] = x.w;
-        } else {   // pairs of elements four apart, as the codes of a word come
-          qf[n][4 * i] = __byte_perm(x.x, x.z, 0x5410); qf[n][4 * i + 1] = __byte_perm(x.x, x.z, 0x7632);
-          qf[n][4 * i + 2] = __byte_perm(x.y, x.w, 0x5410); qf[n][4 * i + 3] = __byte_perm(x.y, x.w, 0x7632);
-        }
-      }
-    }
-    if constexpr (kBits == 4) {
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i) {
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sum += lo_f32(qf[n][4 * i + j], T()) + hi_f32(qf[n][4 * i + j], T());
-        sum += __shfl_xor_sync(kFull, sum, 1);
-        sum += __shfl_xor_sync(kFull, sum, 2);   // of row 8n + g, in every thread of the quad
-        qs[n][0][i] = __shfl_sync(kFull, sum, 8 * t);       // row 2t
-        qs[n][1][i] = __shfl_sync(kFull, sum, 8 * t + 4);   // row 2t + 1
-      }
-    }
-  }
-  int pos[kNT][2];   // positions of rows 2t and 2t + 1 of each tile
+  uint4 qf[kNT][kD / 32];   // Q^T fragments: of row 8n + g, the bytes this thread also reads of a key row
 #pragma unroll
   for (int n = 0; n < kNT; ++n)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) pos[n][e] = first_pos + (row0 + 8 * n + 2 * t + e) / group;   // (rows behind the last are not written)
-  float m[kNT][2], shift[kNT][2], limit[kNT][2], l[kNT][2];   // shift: -max, 0 as long as there is none; limit: where it moves
-  float o[kNT][kTiles][4];
-  float z[kNT][2][kBits == 4 ? kGroups : 1];
-#pragma unroll
-  for (int n = 0; n < kNT; ++n) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      m[n][e] = limit[n][e] = -INFINITY;
-      shift[n][e] = l[n][e] = 0.f;
-#pragma unroll
-      for (int i = 0; i < (kBits == 4 ? kGroups : 1); ++i) z[n][e][i] = 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < kTiles; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
-  }
-  const int32_t* table = p.c.table + static_cast<int64_t>(b) * p.c.table_stride;
+    for (int i = 0; i < kD / 32; ++i)
+      qf[n][i] = 8 * n + g < u.rows ? *(reinterpret_cast<const uint4*>(query_row<T>(p, u, 8 * n + g)) + 4 * i + t) : make_uint4(0, 0, 0, 0);
+  RowState<kNT, kD / 16, false> st;
+  st.clear();
+  const int32_t* table = p.c.table + static_cast<int64_t>(u.b) * p.c.table_stride;
+  const int begin = u.begin + warp, end = u.end;
   bool bad_page = false;
 
-  auto base_of = [&](int i) { return list.at(i) * kStepKeys; };
+  auto base_of = [&](int i) { return u.list.at(i) * kStepKeys; };
   auto entry_of = [&](int i) { return __ldg(table + (base_of(min(i, end - 1)) >> p.c.shift)); };   // (used where i < end)
-  // row of the pages that holds the step's first key
-  auto row_of = [&](int i, int page) {
-    if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.c.pages)) {
-      bad_page = true;
-      page = 0;
-    }
-    return ((static_cast<int64_t>(page) * p.c.Hkv + hk) << p.c.shift) + (base_of(i) & ((1 << p.c.shift) - 1));
-  };
-  // place in the step of the key that is read for key `k` of it
-  auto place = [&](int base, int k) {
-    int key = min(base + k, p_last);
-    if (key >= hidden_from && key < hidden_to) key = hidden_to < base + kStepKeys ? hidden_to : hidden_from - 1;
-    return key - base;
-  };
-  const float scale = kBits == 4 ? p.scale_log2 * 16.f : p.scale_log2;
-
-  using Frag = Fragments<kD, kBits>;
-  auto load_k = [&](Frag& f, int i, int64_t row) {
-    const int base = base_of(i);
+  uint4 kf[2][kD / 32];   // key rows g, g + 8
+  uint4 vf[4][kD / 64];   // value rows 2t, 2t + 1, 2t + 8, 2t + 9
+  const T* const kbase = reinterpret_cast<const T*>(p.c.k) + 8 * t;
+  const T* const vbase = reinterpret_cast<const T*>(p.c.v) + 8 * g;
+  auto load_k_at = [&](uint32_t at, int next) {
+    const T* src = kbase + static_cast<uint64_t>(at) * kD;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int64_t at = row + place(base, g + 8 * r);
-      if constexpr (kBits == 16) {
-        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.c.k) + at * kD) + t;
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int j = 0; j < kD / 32; ++j) f.k[r][j] = __ldg(src + 4 * j);
-      } else {
-        load_words<kGroups>(reinterpret_cast<const uint32_t*>(p.c.k) + at * (kD / 8) + t * kGroups, f.k[r]);
-        load_words<kGroups>(reinterpret_cast<const uint32_t*>(p.c.k_scales) + at * kGroups, f.ks[r]);
-      }
+      for (int j = 0; j < kD / 32; ++j) kf[r][j] = __ldg(reinterpret_cast<const uint4*>(src + r * next * kD) + 4 * j);
+  };
+  auto load_v_at = [&](uint32_t at, int d1, int d2, int d3) {
+    const T* src = vbase + static_cast<uint64_t>(at) * kD;
+    const int far[4] = {0, d1, d2, d3};
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < kD / 64; ++j) vf[r][j] = __ldg(reinterpret_cast<const uint4*>(src + far[r] * kD) + 8 * j);
+  };
+  auto load_k = [&](int base, uint32_t row) {
+    if (whole_step<kStepKeys>(u, base)) {
+      load_k_at(row + g, 8);
+    } else {
+      const int at = place<kStepKeys>(u, base, g);
+      load_k_at(row + at, place<kStepKeys>(u, base, g + 8) - at);
     }
   };
-  auto load_v = [&](Frag& f, int i, int64_t row) {
-    const int base = base_of(i);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int64_t at = row + place(base, 2 * t + (r & 1) + 8 * (r >> 1));
-      if constexpr (kBits == 16) {
-        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.c.v) + at * kD) + g;
-#pragma unroll
-        for (int j = 0; j < kD / 64; ++j) f.v[r][j] = __ldg(src + 8 * j);
-      } else {
-        load_words<kD / 64>(reinterpret_cast<const uint32_t*>(p.c.v) + at * (kD / 8) + g * (kD / 64), f.v[r]);
-      }
-    }
-    if constexpr (kBits == 4) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-        load_words<kGroups>(reinterpret_cast<const uint32_t*>(p.c.v_scales) + (row + place(base, g + 8 * r)) * kGroups, f.vs[r]);
+  auto load_v = [&](int base, uint32_t row) {
+    if (whole_step<kStepKeys>(u, base)) {
+      load_v_at(row + 2 * t, 1, 8, 9);
+    } else {
+      const int at = place<kStepKeys>(u, base, 2 * t);
+      load_v_at(row + at, place<kStepKeys>(u, base, 2 * t + 1) - at, place<kStepKeys>(u, base, 2 * t + 8) - at, place<kStepKeys>(u, base, 2 * t + 9) - at);
     }
   };
-  // scores of a step's keys, scaled to the log2 domain less the rows' maxima: x[n][0] (key g, row 2t) [1] (key g, row 2t + 1) [2], [3] key g + 8
-  auto scores = [&](const Frag& f, int i, float (&x)[kNT][4]) {
+  // the next step's keys are loaded as soon as this one's are in the scores, its values behind this one's products
+  if (begin < end) {
+    int base = base_of(begin);
+    uint32_t row = page_row(p.c, u.hk, entry_of(begin), base, &bad_page);
+    load_k(base, row);
+    load_v(base, row);
+    int entry = entry_of(begin + kWarps);
+    for (int i = begin; i < end; i += kWarps) {
+      const int next = min(i + kWarps, end - 1), next_base = base_of(next);
+      row = page_row(p.c, u.hk, entry, next_base, &bad_page);
+      entry = entry_of(next + kWarps);
+      float xs[1][kNT][4];
+      float (&x)[kNT][4] = xs[0];
 #pragma unroll
-    for (int n = 0; n < kNT; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
-    if constexpr (kBits == 16) {
+      for (int n = 0; n < kNT; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
 #pragma unroll
       for (int j = 0; j < kD / 32; ++j)
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
           for (int n = 0; n < kNT; ++n)
-            mma16816<T>(x[n], word_of(f.k[0][j], 2 * half), word_of(f.k[1][j], 2 * half), word_of(f.k[0][j], 2 * half + 1),
-                        word_of(f.k[1][j], 2 * half + 1), qf[n][4 * j + 2 * half], qf[n][4 * j + 2 * half + 1]);
-    } else {
+            mma16816<T>(x[n], word_of(kf[0][j], 2 * half), word_of(kf[1][j], 2 * half), word_of(kf[0][j], 2 * half + 1),
+                        word_of(kf[1][j], 2 * half + 1), word_of(qf[n][j], 2 * half), word_of(qf[n][j], 2 * half + 1));
+      load_k(next_base, row);
 #pragma unroll
-      for (int G = 0; G < kGroups; ++G) {
-        float acc[kNT][4];
+      for (int n = 0; n < kNT; ++n)
 #pragma unroll
-        for (int n = 0; n < kNT; ++n) {
-          acc[n][0] = acc[n][2] = -qs[n][0][G];
-          acc[n][1] = acc[n][3] = -qs[n][1][G];
-        }
-        {
-          const uint32_t a0 = codes_plus_one<T, 0>(f.k[0][G]), a1 = codes_plus_one<T, 0>(f.k[1][G]);
-          const uint32_t a2 = codes_plus_one<T, 1>(f.k[0][G]), a3 = codes_plus_one<T, 1>(f.k[1][G]);
-#pragma unroll
-          for (int n = 0; n < kNT; ++n) mma16816<T>(acc[n], a0, a1, a2, a3, qf[n][4 * G], qf[n][4 * G + 1]);
-        }
-        {
-          const uint32_t a0 = codes_plus_one<T, 2>(f.k[0][G]), a1 = codes_plus_one<T, 2>(f.k[1][G]);
-          const uint32_t a2 = codes_plus_one<T, 3>(f.k[0][G]), a3 = codes_plus_one<T, 3>(f.k[1][G]);
-#pragma unroll
-          for (int n = 0; n < kNT; ++n) mma16816<T>(acc[n], a0, a1, a2, a3, qf[n][4 * G + 2], qf[n][4 * G + 3]);
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float ks = lo_f32(f.ks[r][G], T()), km = hi_f32(f.ks[r][G], T()) * 0.0625f;
-#pragma unroll
-          for (int n = 0; n < kNT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) x[n][2 * r + e] = fmaf(ks, acc[n][2 * r + e], fmaf(km, qs[n][e][G], x[n][2 * r + e]));
-        }
-      }
-    }
-    const int base = base_of(i);
-    // (a step at an edge: of some row's causal range, or of the span that some row's window leaves out)
-    const bool edge = base + kStepKeys - 1 > p_first || (p.window && base <= p_last - p.window && base + kStepKeys - 1 >= p.sinks);
-#pragma unroll
-    for (int n = 0; n < kNT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[n][e] = fmaf(x[n][e], scale, shift[n][e & 1]);
-        if (edge) {
-          const int key = base + g + 8 * (e >> 1), at = pos[n][e & 1];
-          if (key > at || (p.window && key <= at - p.window && key >= p.sinks)) x[n][e] = -INFINITY;
-        }
-      }
-  };
-  // raises the maxima of the rows that have a score too far above theirs, and rescales what was summed
-  auto raise = [&](float (&x)[kNT][4]) {
-#pragma unroll
-    for (int n = 0; n < kNT; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float top = fmaxf(x[n][e], x[n][2 + e]);
-        top = fmaxf(top, __shfl_xor_sync(kFull, top, 4));
-        top = fmaxf(top, __shfl_xor_sync(kFull, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(kFull, top, 16));   // relative to the standing maximum (to 0 without one)
-        const bool none = m[n][e] == -INFINITY;
-        if (top > (none ? -INFINITY : 0.f)) {
-          const float corr = none ? 0.f : exp2f(-top);
-          m[n][e] = none ? top : m[n][e] + top;
-          shift[n][e] = -m[n][e];
-          limit[n][e] = kLazy;
-          x[n][e] -= top;
-          x[n][2 + e] -= top;
-          l[n][e] *= corr;
-#pragma unroll
-          for (int j = 0; j < kTiles; ++j) {
-            o[n][j][e] *= corr;
-            o[n][j][2 + e] *= corr;
-          }
-          if constexpr (kBits == 4) {
-#pragma unroll
-            for (int G = 0; G < kGroups; ++G) z[n][e][G] *= corr;
-          }
-        }
-      }
-  };
-  auto probabilities = [&](float (&x)[kNT][4]) {
-    bool far = false;
-#pragma unroll
-    for (int n = 0; n < kNT; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) far |= fmaxf(x[n][e], x[n][2 + e]) > limit[n][e];
-    if (__any_sync(kFull, far)) raise(x);
-#pragma unroll
-    for (int n = 0; n < kNT; ++n) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[n][e] = ex2_approx(x[n][e]);
-      l[n][0] += x[n][0] + x[n][2];   // this thread's two keys; summed over g at the end
-      l[n][1] += x[n][1] + x[n][3];
-    }
-  };
-  auto add_values = [&](const Frag& f, const float (&x)[kNT][4]) {
-    if constexpr (kBits == 16) {
+        for (int e = 0; e < 4; ++e) x[n][e] = fmaf(x[n][e], p.scale_log2, st.shift[n][e & 1]);
+      if (edge_step<kStepKeys>(u, p, base)) st.mask(x, p, u, base + g, base + g + 8, t);
+      st.probabilities(xs, kLazy);
       uint32_t pb[kNT][2];
 #pragma unroll
       for (int n = 0; n < kNT; ++n) {
@@ -642,185 +673,372 @@ __global__ void __launch_bounds__(kWarps * 32, kNT == 1 ? 3 : 2) paged_attention
       for (int h = 0; h < kD / 64; ++h)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const uint32_t a0 = __byte_perm(word_of(f.v[0][h], q), word_of(f.v[1][h], q), 0x5410);   // element d of keys 2t, 2t + 1
-          const uint32_t a1 = __byte_perm(word_of(f.v[0][h], q), word_of(f.v[1][h], q), 0x7632);   // element d + 1
-          const uint32_t a2 = __byte_perm(word_of(f.v[2][h], q), word_of(f.v[3][h], q), 0x5410);   // keys 2t + 8, 2t + 9
-          const uint32_t a3 = __byte_perm(word_of(f.v[2][h], q), word_of(f.v[3][h], q), 0x7632);
+          const uint32_t a0 = __byte_perm(word_of(vf[0][h], q), word_of(vf[1][h], q), 0x5410);   // element d of keys 2t, 2t + 1
+          const uint32_t a1 = __byte_perm(word_of(vf[0][h], q), word_of(vf[1][h], q), 0x7632);   // element d + 1
+          const uint32_t a2 = __byte_perm(word_of(vf[2][h], q), word_of(vf[3][h], q), 0x5410);   // keys 2t + 8, 2t + 9
+          const uint32_t a3 = __byte_perm(word_of(vf[2][h], q), word_of(vf[3][h], q), 0x7632);
 #pragma unroll
-          for (int n = 0; n < kNT; ++n) mma16816<T>(o[n][4 * h + q], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+          for (int n = 0; n < kNT; ++n) mma16816<T>(st.o[n][4 * h + q], a0, a1, a2, a3, pb[n][0], pb[n][1]);
         }
-    } else {
-#pragma unroll
-      for (int G = 0; G < kGroups; ++G) {
-        uint32_t pb[kNT][2];
-        const float vs0 = lo_f32(f.vs[0][G], T()), vm0 = hi_f32(f.vs[0][G], T());
-        const float vs1 = lo_f32(f.vs[1][G], T()), vm1 = hi_f32(f.vs[1][G], T());
-#pragma unroll
-        for (int n = 0; n < kNT; ++n) {
-          pb[n][0] = transpose8x8(pack2<true>(x[n][0] * vs0, x[n][1] * vs0));
-          pb[n][1] = transpose8x8(pack2<true>(x[n][2] * vs1, x[n][3] * vs1));
-          z[n][0][G] = fmaf(x[n][0], vm0, fmaf(x[n][2], vm1, z[n][0][G]));
-          z[n][1][G] = fmaf(x[n][1], vm0, fmaf(x[n][3], vm1, z[n][1][G]));
-        }
-        // elements 32 G + 4 g + 0..3 of keys (2t, 2t + 1) and (2t + 8, 2t + 9)
-        const uint32_t ya = __byte_perm(f.v[0][G >> 1], f.v[1][G >> 1], G & 1 ? 0x7632 : 0x5410);
-        const uint32_t yb = __byte_perm(f.v[2][G >> 1], f.v[3][G >> 1], G & 1 ? 0x7632 : 0x5410);
-        uint32_t a[4], c[4];
-        a[0] = codes_plus_one<__nv_bfloat16, 0>(ya); a[1] = codes_plus_one<__nv_bfloat16, 1>(ya);
-        a[2] = codes_plus_one<__nv_bfloat16, 2>(ya); a[3] = codes_plus_one<__nv_bfloat16, 3>(ya);
-        c[0] = codes_plus_one<__nv_bfloat16, 0>(yb); c[1] = codes_plus_one<__nv_bfloat16, 1>(yb);
-        c[2] = codes_plus_one<__nv_bfloat16, 2>(yb); c[3] = codes_plus_one<__nv_bfloat16, 3>(yb);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          a[j] = minus_one_bf16x2(a[j]);
-          c[j] = minus_one_bf16x2(c[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int n = 0; n < kNT; ++n)
-            mma16816<__nv_bfloat16>(o[n][2 * G + j], a[2 * j], a[2 * j + 1], c[2 * j], c[2 * j + 1], pb[n][0], pb[n][1]);
-      }
-    }
-  };
-
-  int i = begin + warp;
-  if constexpr (kBits == 16) {
-    // the next step's keys are loaded as soon as this one's are in the scores, its values behind this one's products
-    if (i < end) {
-      Frag f;
-      int64_t row = row_of(i, entry_of(i));
-      load_k(f, i, row);
-      load_v(f, i, row);
-      int entry = entry_of(i + kWarps);
-      for (; i < end; i += kWarps) {
-        const int next = min(i + kWarps, end - 1);
-        row = row_of(next, entry);
-        entry = entry_of(next + kWarps);
-        float x[kNT][4];
-        scores(f, i, x);
-        load_k(f, next, row);
-        probabilities(x);
-        add_values(f, x);
-        load_v(f, next, row);
-      }
-    }
-  } else {
-    // two steps of codes in flight: a step's are a quarter of the bytes
-    if (i < end) {
-      Frag f[2];
-      int64_t row = row_of(i, entry_of(i));
-      load_k(f[0], i, row);
-      load_v(f[0], i, row);
-      const int second = min(i + kWarps, end - 1);
-      row = row_of(second, entry_of(second));
-      load_k(f[1], second, row);
-      load_v(f[1], second, row);
-      int entry = entry_of(i + 2 * kWarps);
-      while (true) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int next = min(i + 2 * kWarps, end - 1);
-          row = row_of(next, entry);
-          entry = entry_of(i + 3 * kWarps);
-          float x[kNT][4];
-          scores(f[u], i, x);
-          load_k(f[u], next, row);
-          probabilities(x);
-          add_values(f[u], x);
-          load_v(f[u], next, row);
-          i += kWarps;
-          if (i >= end) break;
-        }
-        if (i >= end) break;
-      }
+      load_v(next_base, row);
+      base = next_base;
     }
   }
+  bool good = u.good;
   if (__any_sync(kFull, bad_page)) {
     if (lane == 0) report_bad_index(p.c.status, 7);
     good = false;
   }
-  // this warp's results to shared memory
+  float* mine = smem_f + warp * (Cfg::kWarpBytes / 4);
 #pragma unroll
   for (int n = 0; n < kNT; ++n) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float ls = l[n][e];
+      float ls = st.l[n][e];
       ls += __shfl_xor_sync(kFull, ls, 4);
       ls += __shfl_xor_sync(kFull, ls, 8);
       ls += __shfl_xor_sync(kFull, ls, 16);
-      const int r = 8 * n + 2 * t + e;
-      if constexpr (kBits == 16) {
+      float* row = mine + (8 * n + 2 * t + e) * (kD + 2);
 #pragma unroll
-        for (int j = 0; j < kTiles; ++j) {
-          const int d = 64 * (j >> 2) + 8 * g + 2 * (j & 3);
-          sMerge[warp][r][d] = o[n][j][e];
-          sMerge[warp][r][d + 1] = o[n][j][2 + e];
-        }
-      } else {
-#pragma unroll
-        for (int G = 0; G < kGroups; ++G) {
-          float zs = z[n][e][G];
-          zs += __shfl_xor_sync(kFull, zs, 4);
-          zs += __shfl_xor_sync(kFull, zs, 8);
-          zs += __shfl_xor_sync(kFull, zs, 16);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int d = 32 * G + 4 * g + 2 * j;
-            sMerge[warp][r][d] = fmaf(16.f, o[n][2 * G + j][e], zs);
-            sMerge[warp][r][d + 1] = fmaf(16.f, o[n][2 * G + j][2 + e], zs);
-          }
-        }
-      }
-      if (g == 0) {
-        sMerge[warp][r][kD] = good ? m[n][e] : 0.f;
-        sMerge[warp][r][kD + 1] = good ? ls : __uint_as_float(0x7fffffffu);
-      }
+      for (int j = 0; j < kD / 16; ++j)
+        *reinterpret_cast<float2*>(row + 64 * (j >> 2) + 8 * g + 2 * (j & 3)) = make_float2(st.o[n][j][e], st.o[n][j][2 + e]);
+      if (g == 0) *reinterpret_cast<float2*>(row + kD) = good ? make_float2(st.m[n][e], ls) : make_float2(0.f, __uint_as_float(0x7fffffffu));
     }
+  }
+  merge<T, kD, kWarps>(p, u, smem_f, Cfg::kWarpBytes / 4, sML);
+}
+
+// ---- 4 bits.  A step is 32 keys, 5 KB at D = 128, whose halves each lie together in four pieces: eight lanes of a warp fetch them
+// with bulk copies into a ring of the warp's own, and the products read their fragments from there.
+// (Fragments straight from global memory take 14 loads and their addresses for 16 keys, with a step or two in flight.)
+// Shared memory would meet itself four times in a value row's bank if thread t took rows 2t and 2t + 1: slot s of a half is key
+// (s / 2) + 4 (s % 2) of its eight instead, so that t takes rows t, t + 4, t + 8, t + 12.
+template <typename T, int kD, int kNT, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? AttendCfg<kD, kNT, 4>::kPerSm : 1) paged_attention_4bit_kernel(const AttendParams p) {
+  using Cfg = AttendCfg<kD, kNT, 4>;
+  constexpr int kGroups = kD / kGroup, kStages = Cfg::kStages, kKeys = Cfg::kKeys;
+  constexpr unsigned kFull = 0xffffffffu;
+  constexpr float kLazy = std::is_same<T, __half>::value ? 2.f : 8.f;
+  extern __shared__ __align__(16) float smem_f[];
+  __shared__ float2 sML[8 * kNT];
+  __shared__ uint64_t bars[kWarps][kStages];
+  __shared__ uint32_t abort_flag;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const Unit u = unit_of<kKeys>(p, 8 * kNT);
+  if (u.rows <= 0) return;   // (all blocks of the cluster do)
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int w = 0; w < kWarps; ++w)
+      for (int i = 0; i < kStages; ++i) mbar_init(&bars[w][i], 1);
+    fence_mbar_init();
+    fence_proxy_async_smem();
   }
   __syncthreads();
-  // merge the warps
-  for (int idx = tid; idx < rows * kD; idx += kWarps * 32) {
-    const int r = idx / kD, d = idx % kD;
-    float mm = -INFINITY;
+  uint8_t* const ring = reinterpret_cast<uint8_t*>(smem_f) + warp * Cfg::kWarpBytes;
+  const int32_t* table = p.c.table + static_cast<int64_t>(u.b) * p.c.table_stride;
+  const int begin = u.begin + warp, end = u.end;
+  bool bad_page = false;
+  auto base_of = [&](int i) { return u.list.at(i) * kKeys; };
+  // Step i into a slot of the ring: lane l < 8 fetches piece l % 4 of half l / 4, if a row sees a key of that half (the page of one
+  // that none does may not be the sequence's any more).
+  const int my_half = lane >> 2 & 1;
+  const bool scales = lane & 1;
+  const uint8_t* const piece_src = static_cast<const uint8_t*>(lane & 2 ? (scales ? p.c.v_scales : p.c.v) : (scales ? p.c.k_scales : p.c.k));
+  const uint32_t piece_row = scales ? kGroups * 4 : kD / 2, piece_bytes = piece_row * kStepKeys;
+  uint8_t* const piece_dst = ring + (scales ? 2 * Cfg::kCodeBytes : 0) + (lane & 2 ? 2 * static_cast<int>(piece_bytes) : 0) + my_half * piece_bytes;
+  auto half_seen = [&](int from) {
+    return from <= u.p_last && !(from >= u.hidden_from && min(from + kStepKeys - 1, u.p_last) < u.hidden_to);
+  };
+  auto entry_of = [&](int i) {   // (of a step there is; a half that nobody sees takes the other's)
+    const int base = base_of(i), from = base + kStepKeys * my_half;
+    return __ldg(table + ((half_seen(from) ? from : base + kStepKeys * (1 - my_half)) >> p.c.shift));
+  };
+  auto fetch = [&](int i, int entry, int slot) {
+    const int from = base_of(i) + kStepKeys * my_half;
+    const bool seen = half_seen(from);
+    const uint32_t row = page_row(p.c, u.hk, entry, from, &bad_page);
+    const unsigned halves = __ballot_sync(kFull, seen);   // bits 0 and 4
+    uint64_t* bar = &bars[warp][slot];
+    if (lane == 0) mbar_arrive_expect_tx(bar, Cfg::kStageBytes / 2 * ((halves & 1u) + (halves >> 4 & 1u)));
+    __syncwarp();
+    if (lane < 8 && seen) bulk_load_1d(piece_dst + slot * Cfg::kStageBytes, piece_src + static_cast<uint64_t>(row) * piece_row, piece_bytes, bar);
+  };
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sMerge[w][r][kD]);
-    const float m_use = mm == -INFINITY ? 0.f : mm;
-    float acc = 0.f, ls = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float weight = exp2f(sMerge[w][r][kD] - m_use);
-      acc = fmaf(sMerge[w][r][d], weight, acc);
-      ls = fmaf(sMerge[w][r][kD + 1], weight, ls);
-    }
-    sMerge[0][r][d] = acc;   // (this thread alone reads and writes column d of row r)
-    if (d == 0) sML[r] = make_float2(mm, ls);
+  for (int j = 0; j < kStages; ++j) {
+    if (begin + j * kWarps < end) fetch(begin + j * kWarps, entry_of(begin + j * kWarps), j);
   }
-  merge_peers<T, kD, kRows>(p, b, hk, group, row0, rows, peers, rank, &sMerge[0][0][0], sML);
+  int entry = begin + kStages * kWarps < end ? entry_of(begin + kStages * kWarps) : 0;
+
+  // Q^T fragments of row 8n + g, as fp16 times a power of two, and the sums of its groups in three parts
+  uint32_t qf[kNT][kD / 8], qs[kNT][2];   // qs: thread t has the t-th parts of groups (0, 1) and (2, 3)
+  float scale[kNT][2];                    // of the scores of rows 2t and 2t + 1, to the log2 domain
+#pragma unroll
+  for (int n = 0; n < kNT; ++n) {
+    float q[kD / 4], top = 0.f;   // this thread's eight of every 32 elements
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (8 * n + g < u.rows) x = *reinterpret_cast<const uint4*>(query_row<T>(p, u, 8 * n + g) + 32 * i + 8 * t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        q[8 * i + j] = j & 1 ? hi_f32(word_of(x, j >> 1), T()) : lo_f32(word_of(x, j >> 1), T());
+        top = fmaxf(top, fabsf(q[8 * i + j]));
+      }
+    }
+    top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
+    const uint32_t ex = min(__float_as_uint(top) >> 23, 253u);
+    const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23);
+    float part[kGroups];
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {   // pairs of elements four apart, as the codes of a word come
+        const uint32_t w = pack2<false>(q[8 * i + j] * down, q[8 * i + j + 4] * down);
+        qf[n][4 * i + j] = w;
+        sum += lo_f32(w, __half()) + hi_f32(w, __half());
+      }
+      sum += __shfl_xor_sync(kFull, sum, 1);
+      sum += __shfl_xor_sync(kFull, sum, 2);   // of row 8n + g, in every thread of the quad
+#pragma unroll
+      for (int v = 0; v < 3; ++v) {
+        const float r = round_t<T>(sum);
+        part[i] = t == v ? r : v == 0 ? 0.f : part[i];
+        sum -= r;
+      }
+    }
+    qs[n][0] = pack_t<T>(part[0], part[1]);
+    qs[n][1] = kGroups > 2 ? pack_t<T>(part[kGroups - 2], part[kGroups - 1]) : 0;
+    scale[n][0] = p.scale_log2 * __shfl_sync(kFull, up, 8 * t);
+    scale[n][1] = p.scale_log2 * __shfl_sync(kFull, up, 8 * t + 4);
+  }
+  RowState<kNT, kD / 16, true> st;
+  st.clear();
+  const uint32_t one_v = std::is_same<T, __half>::value ? p.one_f16 : p.one_bf16;
+  const uint32_t z_halves = (g / kGroups) & 1 ? 0x7632 : 0x5410;
+  const int k_first = (g >> 1) + 4 * (g & 1);   // key of slot g
+
+  auto step = [&](const uint8_t* stage, int base, auto simple) {
+    constexpr bool kSimple = decltype(simple)::value;   // every row sees every key
+    int kr[2][2], vr[2][4];                             // [half]: rows of the stage
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) kr[h][r] = 16 * h + k_first + 8 * r;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) vr[h][r] = 16 * h + t + 4 * r;
+      if (!kSimple) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) kr[h][r] = place<kKeys>(u, base, kr[h][r]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) vr[h][r] = place<kKeys>(u, base, vr[h][r]);
+      }
+    }
+    const uint8_t* const kc = stage + t * (kD / 8);
+    const uint8_t* const vc = stage + Cfg::kCodeBytes + g * (kD / 16);
+    const uint8_t* const ksc = stage + 2 * Cfg::kCodeBytes;
+    const uint8_t* const vsc = ksc + Cfg::kScaleBytes;
+    auto words = [&](const uint8_t* src, auto& w) {   // 4, 8 or 16 bytes
+      constexpr int n = sizeof(w) / 4;
+      if constexpr (n == 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(src);
+        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+      } else if constexpr (n == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(src);
+        w[0] = x.x; w[1] = x.y;
+      } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(src);
+      }
+    };
+    float x[2][kNT][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) x[h][n][0] = x[h][n][1] = x[h][n][2] = x[h][n][3] = 0.f;
+      uint32_t ks[2][kGroups], k[2][kGroups];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        words(ksc + kr[h][r] * (kGroups * 4), ks[r]);
+        words(kc + kr[h][r] * (kD / 2), k[r]);
+      }
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)   // keys by groups: minima times sums
+        mma16816<T>(x[h][n], __byte_perm(ks[0][0], ks[0][1], 0x7632), __byte_perm(ks[1][0], ks[1][1], 0x7632),
+                    kGroups > 2 ? __byte_perm(ks[0][kGroups - 2], ks[0][kGroups - 1], 0x7632) : 0u,
+                    kGroups > 2 ? __byte_perm(ks[1][kGroups - 2], ks[1][kGroups - 1], 0x7632) : 0u, qs[n][0], qs[n][1]);
+#pragma unroll
+      for (int G = 0; G < kGroups; ++G) {
+        float acc[kNT][4];
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+        uint32_t a[4], c[4];
+        codes_of<__half>(k[0][G], 0.f, p.one_f16, a);
+        codes_of<__half>(k[1][G], 0.f, p.one_f16, c);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int n = 0; n < kNT; ++n)
+            mma16816<__half>(acc[n], a[2 * j], c[2 * j], a[2 * j + 1], c[2 * j + 1], qf[n][4 * G + 2 * j], qf[n][4 * G + 2 * j + 1]);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float s = lo_f32(ks[r][G], T());
+#pragma unroll
+          for (int n = 0; n < kNT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) x[h][n][2 * r + e] = fmaf(s, acc[n][2 * r + e], x[h][n][2 * r + e]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[h][n][e] = fmaf(x[h][n][e], scale[n][e & 1], st.shift[n][e & 1]);
+      if (!kSimple) st.mask(x[h], p, u, base + 16 * h + k_first, base + 16 * h + k_first + 8, t);
+    }
+    st.probabilities(x, kLazy);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t vs[2][kGroups], v[4][kD / 64];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) words(vsc + kr[h][r] * (kGroups * 4), vs[r]);
+      {
+        uint32_t zs[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          words(vc + vr[h][r] * (kD / 2), v[r]);
+          zs[r] = *reinterpret_cast<const uint32_t*>(vsc + vr[h][r] * (kGroups * 4) + (g % kGroups) * 4);
+        }
+        const uint32_t a0 = __byte_perm(zs[0], zs[1], z_halves), a2 = __byte_perm(zs[2], zs[3], z_halves);
+#pragma unroll
+        for (int n = 0; n < kNT; ++n)
+          mma16816<T>(st.z[n], a0, 0u, a2, 0u, transpose8x8(pack_t<T>(x[h][n][0], x[h][n][1])), transpose8x8(pack_t<T>(x[h][n][2], x[h][n][3])));
+      }
+#pragma unroll
+      for (int G = 0; G < kGroups; ++G) {
+        uint32_t pb[kNT][2];
+        const float vs0 = lo_f32(vs[0][G], T()), vs1 = lo_f32(vs[1][G], T());
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+          pb[n][0] = transpose8x8(pack_t<T>(x[h][n][0] * vs0, x[h][n][1] * vs0));
+          pb[n][1] = transpose8x8(pack_t<T>(x[h][n][2] * vs1, x[h][n][3] * vs1));
+        }
+        // elements 32 G + 4 g + 0..3 of the two pairs of keys
+        uint32_t a[4], c[4];
+        codes_of<T>(__byte_perm(v[0][G >> 1], v[1][G >> 1], G & 1 ? 0x7632 : 0x5410), 8.f, one_v, a);
+        codes_of<T>(__byte_perm(v[2][G >> 1], v[3][G >> 1], G & 1 ? 0x7632 : 0x5410), 8.f, one_v, c);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int n = 0; n < kNT; ++n) mma16816<T>(st.o[n][2 * G + j], a[2 * j], a[2 * j + 1], c[2 * j], c[2 * j + 1], pb[n][0], pb[n][1]);
+      }
+    }
+  };
+
+  bool good = u.good;
+  int slot = 0;
+  uint32_t phase = 0;
+  for (int i = begin; i < end; i += kWarps) {
+    if (!mbar_wait_warp(&bars[warp][slot], phase, &abort_flag, p.c.status, 0xc00, p.wait_budget)) {
+      good = false;
+      break;
+    }
+    const uint8_t* stage = ring + slot * Cfg::kStageBytes;
+    const int base = base_of(i);
+    if (edge_step<kKeys>(u, p, base)) step(stage, base, std::false_type());
+    else step(stage, base, std::true_type());
+    __syncwarp();   // every lane is done with the slot
+    const int later = i + kStages * kWarps;
+    if (later < end) {
+      fetch(later, entry, slot);
+      if (later + kWarps < end) entry = entry_of(later + kWarps);
+    }
+    if (++slot == kStages) { slot = 0; phase ^= 1; }
+  }
+  settle_if_aborted(&abort_flag);
+  if (__any_sync(kFull, bad_page)) {
+    if (lane == 0) report_bad_index(p.c.status, 7);
+    good = false;
+  }
+  // (every copy of the warp has arrived: its results take the ring's place)
+  float* mine = reinterpret_cast<float*>(ring);
+#pragma unroll
+  for (int n = 0; n < kNT; ++n) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float ls = st.l[n][e];
+      ls += __shfl_xor_sync(kFull, ls, 4);
+      ls += __shfl_xor_sync(kFull, ls, 8);
+      ls += __shfl_xor_sync(kFull, ls, 16);
+      float* row = mine + (8 * n + 2 * t + e) * (kD + 2);
+#pragma unroll
+      for (int G = 0; G < kGroups; ++G) {
+        const float zs = fmaf(8.f, __shfl_sync(kFull, st.z[n][e], 4 * G + t), __shfl_sync(kFull, st.z[n][e], 4 * (kGroups + G) + t));
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          *reinterpret_cast<float2*>(row + 32 * G + 4 * g + 2 * j) = make_float2(st.o[n][2 * G + j][e] + zs, st.o[n][2 * G + j][2 + e] + zs);
+      }
+      if (g == 0) *reinterpret_cast<float2*>(row + kD) = good ? make_float2(st.m[n][e], ls) : make_float2(0.f, __uint_as_float(0x7fffffffu));
+    }
+  }
+  merge<T, kD, kWarps>(p, u, smem_f, Cfg::kWarpBytes / 4, sML);
 }
 
-// Blocks that share a unit: enough to fill the GPU, of at least four steps for each warp of theirs.
-int choose_peers(int64_t units, int64_t keys, int per_sm) {
-  const int64_t steps = (keys + kStepKeys - 1) / kStepKeys;
-  int64_t peers = 148 * per_sm / std::max<int64_t>(units, 1);
-  peers = std::min(peers, steps / (4 * kWarps));
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(peers, kMaxPeers)));
+// How a unit's keys are shared: `peers` blocks of a cluster, of four warps each or, `wide`, of as many as an SM takes.
+struct Shares {
+  int peers;
+  bool wide;
+};
+// The cheapest by this model, in us and keys of a unit: a block alone works through `alone` (`alone_wide`) keys a us, all of them
+// together through `total`, and the two add up as cubes; clusters do not cross a GPC (seven of 18 SMs and one of 13), and a last wave
+// that is not full costs nearly as much as a full one; a peer costs 0.27 us, a wide block 1.9.  Fitted on 1384 random calls (1-1024
+// units, 64-65536 keys, spread by up to 90 %, which the host does not know, windows among them) with every share of up to 16 forced:
+// the choice takes 5.3 % more time than each call's best (99 in 100: at most 26 %); as many blocks as fit the GPU at once, 17 %.  B200, us, four-warp blocks 1 / 4 / 8 / 16 and 12- or 16-warp blocks 1 / 4 / 8 / 16: B8 Hq32 Hkv8
+// Sk32768 spread 60 % D128 16 bits 468 / 153 / 139 / 149, 267 / 134 / 154 / 202; B1 Hq8 Hkv1 Sk65536 888 / 228 / 120 / 66, 527 / 140 / 76 / 44.
+Shares choose_shares(int64_t units, int64_t keys, int D, int bits, int row_tile, int per_sm) {
+  static constexpr float kRates[2][2][2][3] = {   // [D = 128][16 bits][two tiles of rows]: alone, alone_wide, total
+      {{{97, 270, 20000}, {56, 54, 8100}}, {{120, 380, 26000}, {27, 180, 8000}}},
+      {{{62, 85, 12000}, {45, 59, 4800}}, {{64, 86, 8100}, {64, 46, 12000}}}};
+  const float* rate = kRates[D == 128][bits == 16][row_tile == 2];
+  Shares best = {1, false};
+  double least = -1.0;
+  for (int wide = 0; wide < 2; ++wide) {
+    const int sm = wide ? 1 : per_sm;
+    for (int peers = 1; peers <= kMaxPeers; ++peers) {
+      const int fit = peers <= 2 ? 148 * sm / peers : 7 * (18 * sm / peers) + 13 * sm / peers;
+      const double x = static_cast<double>(units) / fit, waves = 0.87 * std::ceil(x) + 0.13 * x;
+      const double all = static_cast<double>(units) * keys / rate[2], chain = waves * keys / peers / rate[wide];
+      const double cost = (wide ? 1.9 : 0.0) + (peers > 1 ? 0.27 * peers : 0.0) + std::cbrt(all * all * all + chain * chain * chain);
+      if (least < 0.0 || cost < least) {
+        least = cost;
+        best = Shares{peers, wide != 0};
+      }
+    }
+  }
+  return best;
 }
 
-template <typename T, int kD, int kNT, int kBits>
-cudaError_t launch_attend(AttendParams p, int64_t keys, cudaStream_t stream) {
-  auto kern = paged_attention_kernel<T, kD, kNT, kBits>;
+template <typename T, int kD, int kNT, int kBits, int kWarps>
+constexpr auto attention_kernel() {
+  if constexpr (kBits == 4) return &paged_attention_4bit_kernel<T, kD, kNT, kWarps>;
+  else return &paged_attention_kernel<T, kD, kNT, kWarps>;
+}
+
+template <typename T, int kD, int kNT, int kBits, int kWarps>
+cudaError_t launch_attend_warps(const AttendParams& p, int peers, cudaStream_t stream) {
+  constexpr auto kern = attention_kernel<T, kD, kNT, kBits, kWarps>();
+  constexpr int kSmem = kWarps * AttendCfg<kD, kNT, kBits>::kWarpBytes;
   static std::once_flag once[64];
   static cudaError_t result[64];
   int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  const cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  std::call_once(once[dev], [&] { result[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); });
+  std::call_once(once[dev], [&] {
+    result[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (result[dev] == cudaSuccess) result[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  });
   if (result[dev] != cudaSuccess) return result[dev];
-  const int rows = p.Hq / p.c.Hkv * p.S;
-  p.row_tiles = (rows + 8 * kNT - 1) / (8 * kNT);
-  const int peers = choose_peers(static_cast<int64_t>(p.c.B) * p.c.Hkv * p.row_tiles, keys, kNT == 1 ? 3 : 2);
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = peers;
@@ -829,10 +1047,23 @@ cudaError_t launch_attend(AttendParams p, int64_t keys, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(peers, p.c.Hkv * p.row_tiles, p.c.B);
   cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = peers > 1 ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+template <typename T, int kD, int kNT, int kBits>
+cudaError_t launch_attend(AttendParams p, int64_t keys, cudaStream_t stream) {
+  using Cfg = AttendCfg<kD, kNT, kBits>;
+  const int rows = p.Hq / p.c.Hkv * p.S;
+  p.row_tiles = (rows + 8 * kNT - 1) / (8 * kNT);
+  p.one_f16 = kOneF16;
+  p.one_bf16 = kOneBf16;
+  const Shares s = choose_shares(static_cast<int64_t>(p.c.B) * p.c.Hkv * p.row_tiles, keys, kD, kBits, kNT, Cfg::kPerSm);
+  return s.wide ? launch_attend_warps<T, kD, kNT, kBits, Cfg::kWide>(p, s.peers, stream)
+                : launch_attend_warps<T, kD, kNT, kBits, 4>(p, s.peers, stream);
 }
 
 template <typename T, int kD, int kBits>
