@@ -92,11 +92,14 @@ class Tensor4(ctypes.Structure):
         return cls.from_buffer_copy(_pack_tensor4(ptr or 0, *shape, *stride))
 
 
-_pack_paged = struct.Struct("7P7q2i").pack
+#: ``b200fa_tensor4`` as bytes: pointer, (B, H, S, D) shape, element strides
+pack_tensor4 = _pack_tensor4
+#: ``b200fa_paged_kv`` as bytes: its fields in their order, pointers as integers (0: NULL)
+pack_paged_kv = struct.Struct("7P7q2i").pack
 
 
 class PagedCache(ctypes.Structure):
-    """``b200fa_paged_kv``: addresses of a paged cache, its block table and lengths, and their sizes."""
+    """``b200fa_paged_kv``: addresses of a paged cache, its block table and lengths, and their sizes (`pack_paged_kv` makes one)."""
 
     _fields_ = [
         ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p),
@@ -105,11 +108,6 @@ class PagedCache(ctypes.Structure):
         ("batch", ctypes.c_int64), ("table_width", ctypes.c_int64), ("table_stride", ctypes.c_int64),
         ("dtype", ctypes.c_int), ("bits", ctypes.c_int),
     ]
-
-    @classmethod
-    def make(cls, *fields) -> "PagedCache":
-        """The fields in their order, pointers as integers (0: NULL)."""
-        return cls.from_buffer_copy(_pack_paged(*fields))
 
 
 class B200FAError(RuntimeError):
@@ -162,20 +160,21 @@ def load() -> ctypes.CDLL:
     lib.b200fa_fwd_dropout.restype = ctypes.c_int
     lib.b200fa_bwd_dropout.argtypes = bwd_args[:14] + drop_args + bwd_args[14:]
     lib.b200fa_bwd_dropout.restype = ctypes.c_int
-    lib.b200fa_window_fwd.argtypes = fwd_args[:7] + [ctypes.c_int64] * 2 + fwd_args[7:]
+    # (descriptors of these come as packed bytes, which ctypes hands on as they are)
+    packed = ctypes.c_void_p
+    lib.b200fa_window_fwd.argtypes = [packed] * 4 + fwd_args[4:7] + [ctypes.c_int64] * 2 + fwd_args[7:]
     lib.b200fa_window_fwd.restype = ctypes.c_int
-    lib.b200fa_window_bwd.argtypes = bwd_args[:13] + [ctypes.c_int64] * 2 + bwd_args[13:]
+    lib.b200fa_window_bwd.argtypes = [packed] * 5 + bwd_args[5:6] + [packed] * 3 + bwd_args[9:13] + [ctypes.c_int64] * 2 + bwd_args[13:]
     lib.b200fa_window_bwd.restype = ctypes.c_int
     lib.b200fa_window_bwd_workspace_bytes.argtypes = [ctypes.c_int64] * 6 + [ctypes.c_int] + [ctypes.c_int64] * 2
     lib.b200fa_window_bwd_workspace_bytes.restype = ctypes.c_size_t
-    cache = ctypes.POINTER(PagedCache)
-    lib.b200fa_paged_append.argtypes = [cache, t4p, t4p, t4p, t4p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
-                                        ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
+    lib.b200fa_paged_append.argtypes = [packed] * 5 + [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+                                                       ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
     lib.b200fa_paged_append.restype = ctypes.c_int
-    lib.b200fa_paged_attention.argtypes = [cache, t4p, t4p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_float,
+    lib.b200fa_paged_attention.argtypes = [packed, packed, packed, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_float,
                                            ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
     lib.b200fa_paged_attention.restype = ctypes.c_int
-    lib.b200fa_paged_gather.argtypes = [cache, t4p, t4p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
+    lib.b200fa_paged_gather.argtypes = [packed, packed, packed, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
     lib.b200fa_paged_gather.restype = ctypes.c_int
     lib.b200fa_dropout_threshold.argtypes = [ctypes.c_float]
     lib.b200fa_dropout_threshold.restype = ctypes.c_uint32
@@ -282,41 +281,42 @@ def bwd(q: Tensor4, k: Tensor4, v: Tensor4, out: Tensor4, dout: Tensor4, lse_ptr
     return fn(*head, *tail)
 
 
-def window_fwd(q: Tensor4, k: Tensor4, v: Tensor4, out: Tensor4, lse_ptr: int, dtype: int, causal, window: int, sinks: int,
+def window_fwd(q: bytes, k: bytes, v: bytes, out: bytes, lse_ptr: int, dtype: int, causal, window: int, sinks: int,
                scale: float, stream: int, device: int, status_ptr: int = 0) -> int:
-    """Raw forward over a window of keys and the first ones (see b200fa_window_fwd); returns the library's status code."""
-    return load().b200fa_window_fwd(ctypes.byref(q), ctypes.byref(k), ctypes.byref(v), ctypes.byref(out), lse_ptr, dtype,
-                                    causal_code(causal), window, sinks, scale, stream, device, status_ptr)
+    """Raw forward over a window of keys and the first ones (see b200fa_window_fwd), tensors as `pack_tensor4` makes them; returns
+    the library's status code."""
+    return load().b200fa_window_fwd(q, k, v, out, lse_ptr, dtype, causal_code(causal), window, sinks, scale, stream, device,
+                                    status_ptr)
 
 
 def window_bwd_workspace_bytes(B: int, Hq: int, Hkv: int, Sq: int, Sk: int, D: int, dtype: int, window: int, sinks: int) -> int:
     return int(load().b200fa_window_bwd_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, dtype, window, sinks))
 
 
-def window_bwd(q: Tensor4, k: Tensor4, v: Tensor4, out: Tensor4, dout: Tensor4, lse_ptr: int, dq: Tensor4, dk: Tensor4,
-               dv: Tensor4, workspace_ptr: int, workspace_bytes: int, dtype: int, causal, window: int, sinks: int, scale: float,
+def window_bwd(q: bytes, k: bytes, v: bytes, out: bytes, dout: bytes, lse_ptr: int, dq: bytes, dk: bytes,
+               dv: bytes, workspace_ptr: int, workspace_bytes: int, dtype: int, causal, window: int, sinks: int, scale: float,
                stream: int, device: int, status_ptr: int = 0) -> int:
     """Raw backward of `window_fwd`; returns the library's status code."""
     return load().b200fa_window_bwd(
-        ctypes.byref(q), ctypes.byref(k), ctypes.byref(v), ctypes.byref(out), ctypes.byref(dout), lse_ptr, ctypes.byref(dq),
-        ctypes.byref(dk), ctypes.byref(dv), workspace_ptr, workspace_bytes, dtype, causal_code(causal), window, sinks, scale,
+        q, k, v, out, dout, lse_ptr, dq, dk, dv, workspace_ptr, workspace_bytes, dtype, causal_code(causal), window, sinks, scale,
         stream, device, status_ptr)
 
 
-def paged_append(cache: PagedCache, k: Tensor4, v: Tensor4, q: Tensor4 | None, q_out: Tensor4 | None, cos_ptr: int, sin_ptr: int,
+def paged_append(cache: bytes, k: bytes, v: bytes, q: bytes | None, q_out: bytes | None, cos_ptr: int, sin_ptr: int,
                  rotary_dim: int, positions: int, interleaved: bool, stream: int, device: int, status_ptr: int = 0) -> int:
-    """Raw append to a paged cache (see b200fa_paged_append); returns the library's status code."""
+    """Raw append to a paged cache (see b200fa_paged_append), descriptors as `pack_paged_kv` and `pack_tensor4` make them; returns
+    the library's status code."""
     return load().b200fa_paged_append(cache, k, v, q, q_out, cos_ptr, sin_ptr, rotary_dim, positions, 1 if interleaved else 0, stream,
                                       device, status_ptr)
 
 
-def paged_attention(cache: PagedCache, q: Tensor4, out: Tensor4, lse_ptr: int, window: int, sinks: int, scale: float, longest: int,
+def paged_attention(cache: bytes, q: bytes, out: bytes, lse_ptr: int, window: int, sinks: int, scale: float, longest: int,
                     stream: int, device: int, status_ptr: int = 0) -> int:
     """Raw attention over a paged cache (see b200fa_paged_attention); returns the library's status code."""
     return load().b200fa_paged_attention(cache, q, out, lse_ptr, window, sinks, scale, longest, stream, device, status_ptr)
 
 
-def paged_gather(cache: PagedCache, k: Tensor4, v: Tensor4, stream: int, device: int, status_ptr: int = 0) -> int:
+def paged_gather(cache: bytes, k: bytes, v: bytes, stream: int, device: int, status_ptr: int = 0) -> int:
     """Raw read-back of a paged cache (see b200fa_paged_gather); returns the library's status code."""
     return load().b200fa_paged_gather(cache, k, v, stream, device, status_ptr)
 

@@ -51,148 +51,185 @@ __device__ __forceinline__ uint32_t pack_t(float lo, float hi) {
 template <typename T>
 __device__ __forceinline__ float round_t(float x) { return lo_f32(pack_t<T>(x, 0.f), T()); }
 
+template <typename T>
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  const T2 r = __hmin2(*reinterpret_cast<const T2*>(&a), *reinterpret_cast<const T2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  const T2 r = __hmax2(*reinterpret_cast<const T2*>(&a), *reinterpret_cast<const T2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 // ------------------------------------------------------------------------------------------
-// Append.  D / 8 lanes take a row (16 bytes each): one head's query, key or value of one token.  With (a, b) a pair of
-// elements that turn together (i and i + R / 2, or 2 i and 2 i + 1, of the first R) and (c, s) its position's cos and sin,
-// a' = a c - b s, b' = b c + a s: every product and sum rounded to fp32 on its own (no FMA), then to the type, so that the
-// results are those of the formula in fp32 whatever computes it.  Copy-bound: each element is read and written once.
-// A row of 4 bits: scale = (max - min) / 15 rounded to the type, code = round((x - min) / scale), of the elements as rounded to
-// the type.  Where an element of a group is not finite the scale is NaN, and so is the group.
+// Append.  D / 8 lanes take a row (16 bytes each), one head's query, key or value of one token, and a warp kChunk heads of the
+// queries, keys or values of one token, kRows of them in each thread: the token's place and angles are looked up once, and the loads of all its rows are in
+// flight together.  With (a, b) a pair of elements that turn together (i and i + R / 2, or 2 i and 2 i + 1, of the first R) and
+// (c, s) its position's cos and sin, a' = a c - b s, b' = b c + a s: every product and sum rounded to fp32 on its own (no FMA),
+// then to the type, so that the results are those of the formula in fp32 whatever computes it.  Copy-bound: each element is
+// read and written once.  A row of 4 bits: scale = (max - min) / 15 rounded to the type, code = round((x - min) / scale), of the
+// elements as rounded to the type.  Where an element of a group is not finite the scale is NaN, and so is the group.
+// B200, one row a thread / this: 6 prompts of up to 1500 tokens, 16 + 4 heads, D = 64, 4 bits APPEND_FIGURES
 // ------------------------------------------------------------------------------------------
+template <typename T, int kD>
+struct AppendCfg {
+  static constexpr int kLanes = kD / 8, kSide = 32 / kLanes;   // rows side by side
+  static constexpr int kRows = 4, kChunk = kRows * kSide;
+};
+
 template <typename T, int kD, int kBits, bool kInterleaved>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p) {
-  constexpr int kLanes = kD / 8;
+__global__ void __launch_bounds__(128) paged_append_kernel(const AppendParams p) {
+  using Cfg = AppendCfg<T, kD>;
+  constexpr int kLanes = Cfg::kLanes;
   constexpr unsigned kFull = 0xffffffffu;
-  const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int li = static_cast<int>(threadIdx.x) % kLanes;
-  const int64_t row = idx / kLanes;   // (token, head): heads of q, then of k, then of v
-  const int heads = p.Hq + 2 * p.c.Hkv;
-  const int64_t tokens = static_cast<int64_t>(p.c.B) * p.S;
-  const bool inside = row < tokens * heads;
-  const int64_t token = inside ? row / heads : 0;
-  int h = inside ? static_cast<int>(row - token * heads) : 0;
-  const int b = static_cast<int>(token / p.S), s = static_cast<int>(token - static_cast<int64_t>(b) * p.S);
+  const int lane = threadIdx.x & 31, li = lane % kLanes;
+  // the warp's token, and its kChunk heads of q, k or v
+  const int of_q = (p.Hq + Cfg::kChunk - 1) / Cfg::kChunk, of_k = (p.c.Hkv + Cfg::kChunk - 1) / Cfg::kChunk;
+  const unsigned item = blockIdx.x * 4 + static_cast<unsigned>(warp_index());
+  const unsigned token = item / (of_q + 2 * of_k);
+  int chunk = static_cast<int>(item - token * (of_q + 2 * of_k));
+  const int what = chunk < of_q ? 0 : chunk < of_q + of_k ? 1 : 2;
+  chunk -= what == 0 ? 0 : what == 1 ? of_q : of_q + of_k;
+  const int b = static_cast<int>(token / p.S), s = static_cast<int>(token - static_cast<unsigned>(b) * p.S);
+  if (b >= p.c.B) return;
+  const int heads = what == 0 ? p.Hq : p.c.Hkv, h0 = chunk * Cfg::kChunk + lane / kLanes;
+  const View4& from = what == 0 ? p.q : what == 1 ? p.k : p.v;
+  const T* src = reinterpret_cast<const T*>(from.ptr) + static_cast<int64_t>(b) * from.sb + static_cast<int64_t>(h0) * from.sh +
+                 static_cast<int64_t>(s) * from.ss + li * 8;
+  uint4 x[Cfg::kRows];
+#pragma unroll
+  for (int u = 0; u < Cfg::kRows; ++u)
+    x[u] = h0 + u * Cfg::kSide < heads ? __ldg(reinterpret_cast<const uint4*>(src + u * Cfg::kSide * from.sh)) : make_uint4(0, 0, 0, 0);
   Sequence seq;
   const bool good = sequence_of(p.c, b, p.S, &seq);
   const int pos = seq.len - seq.n + s;
-  bool write = inside && good && s < seq.n && pos >= 0;
-  const bool angles = p.rotary == 0 || pos < p.positions;
-  if (inside && (!good || (write && !angles))) {
-    if (li == 0) report_bad_index(p.c.status, good ? 2 : 1);
-    write = false;
+  if (!good) {
+    if (lane == 0) report_bad_index(p.c.status, 1);
+    return;
   }
-  const int what = h < p.Hq ? 0 : h < p.Hq + p.c.Hkv ? 1 : 2;   // q, k, v
-  if (what == 1) h -= p.Hq;
-  if (what == 2) h -= p.Hq + p.c.Hkv;
-  int64_t at = 0;   // the row in the pages
-  if (write && what != 0) {
+  if (s >= seq.n || pos < 0) return;
+  if (p.rotary != 0 && pos >= p.positions) {
+    if (lane == 0) report_bad_index(p.c.status, 2);
+    return;
+  }
+  uint32_t row0 = 0;   // of head h0 in the pages
+  if (what != 0) {
     const int page = __ldg(p.c.table + static_cast<int64_t>(b) * p.c.table_stride + (pos >> p.c.shift));
     if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.c.pages)) {
-      if (li == 0) report_bad_index(p.c.status, 3);
-      write = false;
-    } else {
-      at = ((static_cast<int64_t>(page) * p.c.Hkv + h) << p.c.shift) + (pos & ((1 << p.c.shift) - 1));
+      if (lane == 0) report_bad_index(p.c.status, 3);
+      return;
+    }
+    row0 = (static_cast<uint32_t>(page * p.c.Hkv + h0) << p.c.shift) + (pos & ((1 << p.c.shift) - 1));
+  }
+  const int e0 = li * 8, half = p.rotary / 2;
+  const bool first = e0 < half;
+  constexpr int kAngles = kInterleaved ? 4 : 8;
+  float cs[kAngles], sn[kAngles];
+  if (what != 2 && e0 < p.rotary) {
+    const int64_t angle = static_cast<int64_t>(pos) * half + (kInterleaved ? e0 / 2 : first ? e0 : e0 - half);
+#pragma unroll
+    for (int i = 0; i < kAngles / 4; ++i) {
+      const float4 c4 = __ldg(reinterpret_cast<const float4*>(p.cos + angle) + i), s4 = __ldg(reinterpret_cast<const float4*>(p.sin + angle) + i);
+      cs[4 * i] = c4.x; cs[4 * i + 1] = c4.y; cs[4 * i + 2] = c4.z; cs[4 * i + 3] = c4.w;
+      sn[4 * i] = s4.x; sn[4 * i + 1] = s4.y; sn[4 * i + 2] = s4.z; sn[4 * i + 3] = s4.w;
     }
   }
-  const View4& src = what == 0 ? p.q : what == 1 ? p.k : p.v;
-  uint4 x = make_uint4(0, 0, 0, 0);
-  if (write)
-    x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(src.ptr) + static_cast<int64_t>(b) * src.sb + static_cast<int64_t>(h) * src.sh +
-                                        static_cast<int64_t>(s) * src.ss + li * 8);
-  uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  if (p.rotary) {
-    const int e0 = li * 8, half = p.rotary / 2;
-    const bool turn = write && what != 2 && e0 < p.rotary;
-    if constexpr (kInterleaved) {
-      if (turn) {
-        const float4 c4 = __ldg(reinterpret_cast<const float4*>(p.cos + static_cast<int64_t>(pos) * half + e0 / 2));
-        const float4 s4 = __ldg(reinterpret_cast<const float4*>(p.sin + static_cast<int64_t>(pos) * half + e0 / 2));
-        const float cs[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float a = lo_f32(w[i], T()), d = hi_f32(w[i], T());
-          w[i] = pack_t<T>(__fsub_rn(__fmul_rn(a, cs[i]), __fmul_rn(d, sn[i])), __fadd_rn(__fmul_rn(d, cs[i]), __fmul_rn(a, sn[i])));
-        }
-      }
-    } else {
-      // the other elements of the pairs are half / 8 lanes away
-      const bool first = e0 < half;
-      const int lane = threadIdx.x & 31;
-      const int from = e0 < p.rotary ? (first ? lane + half / 8 : lane - half / 8) : lane;
-      uint32_t o[4];
+  for (int u = 0; u < Cfg::kRows; ++u) {
+    if (chunk * Cfg::kChunk + u * Cfg::kSide >= heads) break;
+    const bool write = h0 + u * Cfg::kSide < heads;
+    uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+    if (p.rotary && what != 2) {
+      const bool turn = e0 < p.rotary;
+      if constexpr (kInterleaved) {
+        if (turn) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = __shfl_sync(kFull, w[i], from);
-      if (turn) {
-        const int64_t angle = static_cast<int64_t>(pos) * half + (first ? e0 : e0 - half);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float4 c4 = __ldg(reinterpret_cast<const float4*>(p.cos + angle) + i);
-          const float4 s4 = __ldg(reinterpret_cast<const float4*>(p.sin + angle) + i);
-          const float cs[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
-          float y[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t mine = w[2 * i + (j >> 1)], other = o[2 * i + (j >> 1)];
-            const float a = j & 1 ? hi_f32(mine, T()) : lo_f32(mine, T()), d = j & 1 ? hi_f32(other, T()) : lo_f32(other, T());
-            const float ac = __fmul_rn(a, cs[j]), ds = __fmul_rn(d, sn[j]);
-            y[j] = first ? __fsub_rn(ac, ds) : __fadd_rn(ac, ds);
+          for (int i = 0; i < 4; ++i) {
+            const float a = lo_f32(w[i], T()), d = hi_f32(w[i], T());
+            w[i] = pack_t<T>(__fsub_rn(__fmul_rn(a, cs[i]), __fmul_rn(d, sn[i])), __fadd_rn(__fmul_rn(d, cs[i]), __fmul_rn(a, sn[i])));
           }
-          w[2 * i] = pack_t<T>(y[0], y[1]);
-          w[2 * i + 1] = pack_t<T>(y[2], y[3]);
+        }
+      } else {
+        // the other elements of the pairs are half / 8 lanes away
+        const int from = e0 < p.rotary ? (first ? lane + half / 8 : lane - half / 8) : lane;
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = __shfl_sync(kFull, w[i], from);
+        if (turn) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float y[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float a = j ? hi_f32(w[i], T()) : lo_f32(w[i], T()), d = j ? hi_f32(o[i], T()) : lo_f32(o[i], T());
+              const float ac = __fmul_rn(a, cs[2 * i + j]), ds = __fmul_rn(d, sn[2 * i + j]);
+              y[j] = first ? __fsub_rn(ac, ds) : __fadd_rn(ac, ds);
+            }
+            w[i] = pack_t<T>(y[0], y[1]);
+          }
         }
       }
     }
-  }
-  if (what == 0) {
-    if (write)
-      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.q_out.ptr) + static_cast<int64_t>(b) * p.q_out.sb + static_cast<int64_t>(h) * p.q_out.sh +
-                                static_cast<int64_t>(s) * p.q_out.ss + li * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  if constexpr (kBits == 16) {
-    if (write && what != 0) {
-      void* pages = what == 1 ? p.c.k : p.c.v;
-      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(pages) + at * kD + li * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (what == 0) {
+      if (write)
+        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.q_out.ptr) + static_cast<int64_t>(b) * p.q_out.sb + static_cast<int64_t>(h0 + u * Cfg::kSide) * p.q_out.sh +
+                                  static_cast<int64_t>(s) * p.q_out.ss + li * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+      continue;
     }
-  } else {
-    // the four lanes of a group find its minimum and maximum
-    float v[8], low = INFINITY, high = -INFINITY;
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = i & 1 ? hi_f32(w[i >> 1], T()) : lo_f32(w[i >> 1], T());
-      odd |= !(fabsf(v[i]) <= 3.402823466e38f);
-      low = fminf(low, v[i]);
-      high = fmaxf(high, v[i]);
-    }
-#pragma unroll
-    for (int off = 1; off <= 2; off <<= 1) {
-      low = fminf(low, __shfl_xor_sync(kFull, low, off));
-      high = fmaxf(high, __shfl_xor_sync(kFull, high, off));
-    }
-    const unsigned odd_lanes = __ballot_sync(kFull, odd);
-    if (!write || what == 0) return;
-    float scale = round_t<T>(__fdiv_rn(__fsub_rn(high, low), 15.f));
-    if ((odd_lanes >> ((threadIdx.x & 31) & ~3)) & 15u) scale = __uint_as_float(0x7fffffffu);
-    uint32_t codes = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float q = rintf(__fdiv_rn(__fsub_rn(v[i], low), scale));
-      const int code = scale > 0.f ? static_cast<int>(fminf(fmaxf(q, 0.f), 15.f)) : 0;
-      codes |= static_cast<uint32_t>(code) << (4 * i);
-    }
-    const int G = li >> 2, t = li & 3;
-    constexpr int kGroups = kD / kGroup;
-    uint32_t* row_words = reinterpret_cast<uint32_t*>(what == 1 ? p.c.k : p.c.v) + at * (kD / 8);
-    if (what == 1) {
-      row_words[t * kGroups + G] = codes;
+    const uint64_t at = row0 + (static_cast<uint32_t>(u * Cfg::kSide) << p.c.shift);   // the row in the pages
+    if constexpr (kBits == 16) {
+      if (write) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(what == 1 ? p.c.k : p.c.v) + at * kD + li * 8) = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
-      uint16_t* halves = reinterpret_cast<uint16_t*>(row_words);
-      halves[2 * t * kGroups + G] = static_cast<uint16_t>(codes);
-      halves[(2 * t + 1) * kGroups + G] = static_cast<uint16_t>(codes >> 16);
-    }
-    if (t == 0) {
-      uint32_t* scales = reinterpret_cast<uint32_t*>(what == 1 ? p.c.k_scales : p.c.v_scales) + at * kGroups;
-      scales[G] = pack_t<T>(scale, low);
+      // the four lanes of a group find its minimum and maximum, two elements at a time
+      uint32_t lo2 = min2<T>(min2<T>(w[0], w[1]), min2<T>(w[2], w[3])), hi2 = max2<T>(max2<T>(w[0], w[1]), max2<T>(w[2], w[3]));
+#pragma unroll
+      for (int off = 1; off <= 2; off <<= 1) {
+        lo2 = min2<T>(lo2, __shfl_xor_sync(kFull, lo2, off));
+        hi2 = max2<T>(hi2, __shfl_xor_sync(kFull, hi2, off));
+      }
+      float v[8], odd = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = i & 1 ? hi_f32(w[i >> 1], T()) : lo_f32(w[i >> 1], T());
+        odd = fmaf(v[i], 0.f, odd);   // NaN if an element is not finite
+      }
+      const unsigned odd_lanes = __ballot_sync(kFull, odd != 0.f);
+      if (!write) continue;   // (nothing below needs the other lanes; the next row's shuffles wait for all)
+      const float low = fminf(lo_f32(lo2, T()), hi_f32(lo2, T())), high = fmaxf(lo_f32(hi2, T()), hi_f32(hi2, T()));
+      float scale = round_t<T>(__fdiv_rn(__fsub_rn(high, low), 15.f));
+      if ((odd_lanes >> (lane & ~3)) & 15u) scale = __uint_as_float(0x7fffffffu);
+      // round((x - low) / scale), the division rounded to nearest, at most 15.  The product with the reciprocal is within 3e-6 of
+      // that quotient and rounds as it does unless it is that near to a half; then the division decides.  (A division for each
+      // element was most of the kernel's instructions.)
+      const float inverse = __fdiv_rn(1.f, scale);
+      const bool tiny = !(scale >= 1e-37f);   // (its reciprocal may be infinite)
+      uint32_t codes = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        constexpr float kInts = 12582912.f;   // 1.5 * 2^23: the sum's last bits are the rounded number
+        const float d = __fsub_rn(v[i], low);
+        float q = fminf(__fmul_rn(d, inverse), 15.f), r = __fadd_rn(q, kInts);
+        if (tiny || !(fabsf(q - __fsub_rn(r, kInts)) < 0.4999f)) r = __fadd_rn(fminf(__fdiv_rn(d, scale), 15.f), kInts);
+        codes |= (__float_as_uint(r) & 15u) << (4 * i);
+      }
+      if (!(scale > 0.f)) codes = 0;
+      const int G = li >> 2, t = li & 3;
+      constexpr int kGroups = kD / kGroup;
+      uint32_t* row_words = reinterpret_cast<uint32_t*>(what == 1 ? p.c.k : p.c.v) + at * (kD / 8);
+      if (what == 1) {
+        row_words[t * kGroups + G] = codes;
+      } else {
+        uint16_t* halves = reinterpret_cast<uint16_t*>(row_words);
+        halves[2 * t * kGroups + G] = static_cast<uint16_t>(codes);
+        halves[(2 * t + 1) * kGroups + G] = static_cast<uint16_t>(codes >> 16);
+      }
+      if (t == 0) {
+        uint32_t* scales = reinterpret_cast<uint32_t*>(what == 1 ? p.c.k_scales : p.c.v_scales) + at * kGroups;
+        scales[G] = pack_t<T>(scale, low);
+      }
     }
   }
 }
@@ -1089,10 +1126,11 @@ cudaError_t with_cache(const PagedCache& c, int dtype, F f) {
 cudaError_t launch_paged_append(const AppendParams& p, int dtype, cudaStream_t stream, int* launches) {
   const cudaError_t e = with_cache(p.c, dtype, [&](auto type, auto d, auto bits) {
     using T = decltype(type);
-    const int64_t threads = static_cast<int64_t>(p.c.B) * p.S * (p.Hq + 2 * p.c.Hkv) * (d / 8);
-    const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
-    if (p.interleaved) paged_append_kernel<T, d, bits, true><<<blocks, 256, 0, stream>>>(p);
-    else paged_append_kernel<T, d, bits, false><<<blocks, 256, 0, stream>>>(p);
+    constexpr int kChunk = AppendCfg<T, d>::kChunk;
+    const int64_t warps = static_cast<int64_t>(p.c.B) * p.S * ((p.Hq + kChunk - 1) / kChunk + 2 * ((p.c.Hkv + kChunk - 1) / kChunk));
+    const unsigned blocks = static_cast<unsigned>((warps + 3) / 4);
+    if (p.interleaved) paged_append_kernel<T, d, bits, true><<<blocks, 128, 0, stream>>>(p);
+    else paged_append_kernel<T, d, bits, false><<<blocks, 128, 0, stream>>>(p);
     return cudaGetLastError();
   });
   if (e == cudaSuccess && launches) *launches += 1;

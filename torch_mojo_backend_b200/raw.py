@@ -30,6 +30,13 @@ def t4(t: torch.Tensor) -> _lib.Tensor4:
     return _lib.Tensor4.make(t.data_ptr(), tuple(t.shape), tuple(t.stride()))
 
 
+def _t4b(t: torch.Tensor) -> bytes:
+    """`t4` as the packed bytes that the newer entry points take (a third of the time)."""
+    if t.dim() != 4:
+        raise ValueError("b200fa tensors are 4-D (batch, heads, seq, head_dim)")
+    return _lib.pack_tensor4(t.data_ptr(), *t.shape, *t.stride())
+
+
 def _stream_and_device(t: torch.Tensor) -> tuple[int, int]:
     dev = t.device.index if t.device.index is not None else torch.cuda.current_device()
     return torch._C._cuda_getCurrentRawStream(dev), dev
@@ -132,9 +139,10 @@ def _need_cuda(q) -> None:
 
 def _same_kind(q, others) -> None:
     """Pointers are all that the library sees of a tensor: its type and device are checked here."""
+    dtype, device = q.dtype, q.device
     for t in others:
-        if t is not None and (t.dtype != q.dtype or t.device != q.device):
-            raise ValueError(f"expected {q.dtype} tensors on {q.device}, got {t.dtype} on {t.device}")
+        if t is not None and (t.dtype is not dtype or t.device != device):
+            raise ValueError(f"expected {dtype} tensors on {device}, got {t.dtype} on {t.device}")
 
 
 def _fp32_statistic(lse, shape, device) -> None:
@@ -163,7 +171,7 @@ def window_fwd(q, k, v, *, window: int, sinks: int = 0, causal=True, scale: floa
         _fp32_statistic(lse, (B, Hq, Sq), q.device)
     _same_kind(q, (k, v, out))
     stream, dev = _stream_and_device(q)
-    rc = _lib.window_fwd(t4(q), t4(k), t4(v), t4(out), lse.data_ptr(), dtype_code(q.dtype), causal, window, sinks,
+    rc = _lib.window_fwd(_t4b(q), _t4b(k), _t4b(v), _t4b(out), lse.data_ptr(), dtype_code(q.dtype), causal, window, sinks,
                          float(scale), stream, dev, status.data_ptr() if status is not None else 0)
     if rc != _lib.OK:
         raise _lib.B200FAError(rc, "b200fa_window_fwd")
@@ -191,7 +199,7 @@ def window_bwd(dout, q, k, v, out, lse, *, window: int, sinks: int = 0, causal=T
     if workspace is None:
         workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
     stream, dev = _stream_and_device(q)
-    rc = _lib.window_bwd(t4(q), t4(k), t4(v), t4(out), t4(dout), lse.data_ptr(), t4(dq), t4(dk), t4(dv),
+    rc = _lib.window_bwd(_t4b(q), _t4b(k), _t4b(v), _t4b(out), _t4b(dout), lse.data_ptr(), _t4b(dq), _t4b(dk), _t4b(dv),
                          workspace.data_ptr(), workspace.numel() * workspace.element_size(), code, causal, window, sinks,
                          float(scale), stream, dev, status.data_ptr() if status is not None else 0)
     if rc != _lib.OK:
@@ -232,39 +240,44 @@ class PagedKV(NamedTuple):
         return (self.k if self.k_scales is None else self.k_scales).dtype
 
 
-def _int32(name, t, shape, device) -> int:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} has to be a contiguous int32 tensor of shape {shape} on {device}")
+def _int32(name, t, batch: int, device) -> int:
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != batch or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} has to be a contiguous int32 tensor of shape {(batch,)} on {device}")
     return t.data_ptr()
 
 
-def _paged(cache: PagedKV, block_table, lengths, new_lengths, batch: int) -> _lib.PagedCache:
-    """The cache as the library takes it; pointers are all that it sees, so types, shapes and devices are checked here."""
+def _paged(cache: PagedKV, block_table, lengths, new_lengths, batch: int):
+    """(the cache as the library takes it, its 16-bit type, KV heads, head dimension, device); pointers are all that the library
+    sees, so types, shapes and devices are checked here."""
     k, v, ks, vs = cache
-    _need_cuda(k)
-    device, four = k.device, ks is not None
-    dtype = dtype_code(cache.dtype)
-    if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or v.device != device or not (k.is_contiguous() and v.is_contiguous()):
+    device, shape = k.device, k.shape
+    if device.type != "cuda":
+        raise RuntimeError("b200fa kernels need CUDA memory; there is no CPU implementation")
+    if len(shape) != 4 or v.shape != shape or v.dtype is not k.dtype or v.device != device or not (k.is_contiguous() and v.is_contiguous()):
         raise ValueError("the pages of k and v have to be contiguous and alike, (pages, heads, page_size, head_dim)")
-    pages, heads, page_size, width = k.shape
-    if four:
-        if k.dtype != torch.uint8:
+    pages, heads, page_size, width = shape
+    if ks is None:
+        dtype, bits, ks_ptr, vs_ptr = k.dtype, 16, 0, 0
+        if vs is not None:
+            raise ValueError("16-bit pages have no scales")
+    else:
+        if k.dtype is not torch.uint8:
             raise ValueError("4-bit pages are uint8 codes")
         width *= 2
         want = (pages, heads, page_size, width // 32, 2)
-        for s in (ks, vs):
-            if s is None or tuple(s.shape) != want or s.dtype != ks.dtype or s.device != device or not s.is_contiguous():
-                raise ValueError(f"the scales of a 4-bit cache have to be contiguous and alike, {want}")
-    elif vs is not None:
-        raise ValueError("16-bit pages have no scales")
-    if (block_table.dim() != 2 or block_table.shape[0] != batch or block_table.dtype != torch.int32 or block_table.device != device
-            or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
+        if vs is None or vs.dtype is not ks.dtype or any(
+                tuple(s.shape) != want or s.device != device or not s.is_contiguous() for s in (ks, vs)):
+            raise ValueError(f"the scales of a 4-bit cache have to be contiguous and alike, {want}")
+        dtype, bits, ks_ptr, vs_ptr = ks.dtype, 4, ks.data_ptr(), vs.data_ptr()
+    table_shape = block_table.shape
+    if (len(table_shape) != 2 or table_shape[0] != batch or block_table.dtype is not torch.int32 or block_table.device != device
+            or (table_shape[1] > 1 and block_table.stride(1) != 1)):
         raise ValueError(f"the block table has to be int32, (batch = {batch}, pages of a sequence), on {device}")
-    return _lib.PagedCache.make(
-        k.data_ptr(), v.data_ptr(), ks.data_ptr() if four else 0, vs.data_ptr() if four else 0, block_table.data_ptr(),
-        _int32("lengths", lengths, (batch,), device),
-        _int32("new_lengths", new_lengths, (batch,), device) if new_lengths is not None else 0,
-        pages, heads, page_size, width, batch, block_table.shape[1], block_table.stride(0), dtype, 4 if four else 16)
+    packed = _lib.pack_paged_kv(
+        k.data_ptr(), v.data_ptr(), ks_ptr, vs_ptr, block_table.data_ptr(), _int32("lengths", lengths, batch, device),
+        _int32("new_lengths", new_lengths, batch, device) if new_lengths is not None else 0,
+        pages, heads, page_size, width, batch, table_shape[1], block_table.stride(0), dtype_code(dtype), bits)
+    return packed, dtype, heads, width, device
 
 
 def paged_append(k, v, cache: PagedKV, block_table, lengths, *, new_lengths=None, rotary=None, interleaved: bool = False, q=None,
@@ -279,15 +292,15 @@ def paged_append(k, v, cache: PagedKV, block_table, lengths, *, new_lengths=None
     ``include/b200fa.h``.
     """
     B, Hkv, S, D = k.shape
-    c = _paged(cache, block_table, lengths, new_lengths, B)
-    if D != c.head_dim or Hkv != c.heads or k.dtype != cache.dtype or k.device != cache.k.device:
-        raise ValueError(f"k and v have to be {cache.dtype} of {c.heads} heads of {c.head_dim} on {cache.k.device}")
+    c, dtype, heads, head_dim, device = _paged(cache, block_table, lengths, new_lengths, B)
+    if D != head_dim or Hkv != heads or k.dtype is not dtype or k.device != device:
+        raise ValueError(f"k and v have to be {dtype} of {heads} heads of {head_dim} on {device}")
     _same_kind(k, (v, q, q_out))
     cos_ptr = sin_ptr = rotary_dim = positions = 0
     if rotary is not None:
         cos, sin = rotary
-        if cos.dim() != 2 or sin.shape != cos.shape or any(
-                t.dtype != torch.float32 or t.device != k.device or not t.is_contiguous() for t in (cos, sin)):
+        if (cos.dim() != 2 or sin.shape != cos.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32
+                or cos.device != device or sin.device != device or not (cos.is_contiguous() and sin.is_contiguous())):
             raise ValueError(f"rotary is (cos, sin), contiguous float32 (positions, R / 2) on {k.device}")
         cos_ptr, sin_ptr, positions, rotary_dim = cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1]
     if q is None and q_out is not None:
@@ -296,7 +309,7 @@ def paged_append(k, v, cache: PagedKV, block_table, lengths, *, new_lengths=None
         make = torch.empty if new_lengths is None else torch.zeros
         q_out = make(tuple(q.shape), dtype=q.dtype, device=q.device)
     stream, dev = _stream_and_device(k)
-    rc = _lib.paged_append(c, t4(k), t4(v), t4(q) if q is not None else None, t4(q_out) if q is not None else None, cos_ptr, sin_ptr,
+    rc = _lib.paged_append(c, _t4b(k), _t4b(v), _t4b(q) if q is not None else None, _t4b(q_out) if q is not None else None, cos_ptr, sin_ptr,
                            rotary_dim, positions, interleaved, stream, dev, status.data_ptr() if status is not None else 0)
     if rc != _lib.OK:
         raise _lib.B200FAError(rc, "b200fa_paged_append")
@@ -313,9 +326,9 @@ def paged_attention(q, cache: PagedKV, block_table, lengths, *, new_lengths=None
     table is much wider.
     """
     B, Hq, S, D = q.shape
-    c = _paged(cache, block_table, lengths, new_lengths, B)
-    if D != c.head_dim or q.dtype != cache.dtype or q.device != cache.k.device:
-        raise ValueError(f"q has to be {cache.dtype} of head dimension {c.head_dim} on {cache.k.device}")
+    c, dtype, _, head_dim, device = _paged(cache, block_table, lengths, new_lengths, B)
+    if D != head_dim or q.dtype is not dtype or q.device != device:
+        raise ValueError(f"q has to be {dtype} of head dimension {head_dim} on {device}")
     if scale is None:
         scale = default_scale(D)
     if out is None:
@@ -328,7 +341,7 @@ def paged_attention(q, cache: PagedKV, block_table, lengths, *, new_lengths=None
         _fp32_statistic(lse, (B, Hq, S), q.device)
     _same_kind(q, (out,))
     stream, dev = _stream_and_device(q)
-    rc = _lib.paged_attention(c, t4(q), t4(out), lse.data_ptr(), window, sinks, float(scale), longest, stream, dev,
+    rc = _lib.paged_attention(c, _t4b(q), _t4b(out), lse.data_ptr(), window, sinks, float(scale), longest, stream, dev,
                               status.data_ptr() if status is not None else 0)
     if rc != _lib.OK:
         raise _lib.B200FAError(rc, "b200fa_paged_attention")
@@ -339,17 +352,17 @@ def paged_gather(cache: PagedKV, block_table, lengths, length: int, *, k=None, v
     """k, v = the first ``length`` tokens of every sequence, (B, Hkv, length, D) of the cache's 16-bit type; rows behind a
     sequence's own length are zero.  ``k`` and ``v``: tensors to write to."""
     B = lengths.shape[0]
-    c = _paged(cache, block_table, lengths, None, B)
-    shape = (B, c.heads, length, c.head_dim)
+    c, dtype, heads, head_dim, device = _paged(cache, block_table, lengths, None, B)
+    shape = (B, heads, length, head_dim)
     if k is None:
-        k = torch.empty(shape, dtype=cache.dtype, device=cache.k.device)
+        k = torch.empty(shape, dtype=dtype, device=device)
     if v is None:
-        v = torch.empty(shape, dtype=cache.dtype, device=cache.k.device)
+        v = torch.empty(shape, dtype=dtype, device=device)
     for t in (k, v):
-        if tuple(t.shape) != shape or t.dtype != cache.dtype or t.device != cache.k.device:
-            raise ValueError(f"k and v have to be {cache.dtype} of shape {shape} on {cache.k.device}")
-    stream, dev = _stream_and_device(cache.k)
-    rc = _lib.paged_gather(c, t4(k), t4(v), stream, dev, status.data_ptr() if status is not None else 0)
+        if tuple(t.shape) != shape or t.dtype is not dtype or t.device != device:
+            raise ValueError(f"k and v have to be {dtype} of shape {shape} on {device}")
+    stream, dev = _stream_and_device(k)
+    rc = _lib.paged_gather(c, _t4b(k), _t4b(v), stream, dev, status.data_ptr() if status is not None else 0)
     if rc != _lib.OK:
         raise _lib.B200FAError(rc, "b200fa_paged_gather")
     return k, v
