@@ -108,6 +108,11 @@ CASES = [
     (1, 4, 2, 900, 200, 128, TL, 64, 3),      # ... and who see the sinks alone
     (1, 1, 1, 2900, 2900, 128, TL, 64, 4),    # few heads: the sinks' tile is shared by several blocks
     (1, 8, 2, 2100, 2100, 64, TL, 256, 200),
+    (1, 4, 2, 200, 3000, 128, BR, 1500, 4),   # few heads, which share K/V: their keys are shared by several blocks
+    (1, 8, 1, 70, 2500, 128, BR, 1024, 130),
+    (2, 6, 2, 1100, 1100, 128, TL, 150, 64),  # three heads to a K/V head; sinks of half a block
+    (1, 4, 2, 1100, 1100, 128, TL, 150, 65),
+    (1, 4, 2, 1100, 1100, 64, TL, 100, 192),
 ]
 
 

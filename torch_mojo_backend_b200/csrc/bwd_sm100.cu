@@ -682,9 +682,16 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ 
         }
         if (kWindow && col0 <= m0 + kTile - 1 + p.causal_off - p.window && col0 + 31 >= p.sinks) {
           const int before = m0 + r + p.causal_off - p.window - col0;   // the last column ahead of the row's window
+          if (col0 >= p.sinks) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            if (e <= before && e >= p.sinks - col0) pf[ch * 32 + e] = 0.f;
+            for (int e = 0; e < 32; ++e) {
+              if (e <= before) pf[ch * 32 + e] = 0.f;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              if (e <= before && e >= p.sinks - col0) pf[ch * 32 + e] = 0.f;
+            }
           }
         }
       }

@@ -71,6 +71,7 @@ struct FwdSched {
   int group;       // heads scheduled together so their K/V stay L2-resident
   int nkv_total;   // ceil(Sk / 128)
   bool one_tile;   // the one-tile-per-CTA kernel (two CTAs per SM)
+  bool paired;     // window, two tiles: of two heads that share K/V, the same rows (else of one head, one below the other)
   int splits;      // CTAs (one cluster) that share a query unit's K/V blocks; 1: no cluster
 };
 
@@ -81,10 +82,13 @@ struct FwdSched {
 // are then summed with eight 16-byte loads in flight per thread (one row and peer at a time, with
 // the statistics read row by row, the merge took 25 us at kPeers = 2).  Where a peer's abort flag
 // is up nothing is written: no wait runs behind the barrier before this, so all peers see the same.
-template <int kD, int kTiles, bool kBf16, int kPeers>
+template <int kD, int kTiles, bool kBf16, int kPeers, bool kWindow>
 __device__ __forceinline__ void merge_split(const FwdParams& p, const uint8_t* s_o, const float* s_l, const float* s_m,
-                                            uint8_t* s_w, const volatile uint32_t* abort_flag, int rank, int b, int h,
-                                            int row0) {
+                                            uint8_t* s_w, const volatile uint32_t* abort_flag, int rank, int b, int h0,
+                                            int row0, bool paired) {
+  // row `lr` of the unit: its head and query row
+  auto head_of = [&](int lr) { return kWindow && paired ? h0 + lr / kBM : h0; };
+  auto row_of = [&](int lr) { return kWindow && paired ? row0 + lr % kBM : row0 + lr; };
   constexpr int kShare = kTiles * kBM / kPeers;   // rows, at most the 128 threads
   const int tid = threadIdx.x & 127;
   uint32_t aborted = 0;
@@ -115,8 +119,8 @@ __device__ __forceinline__ void merge_split(const FwdParams& p, const uint8_t* s
     const float inv = sum == 0.f ? 0.f : 1.f / sum;   // (a NaN stays one)
 #pragma unroll
     for (int r = 0; r < kPeers; ++r) weights[tid * kPeers + r] = (wrote >> r) & 1u ? m[r] * inv : -0.f;
-    if (row0 + lr < p.Sq) {
-      p.lse[(static_cast<int64_t>(b) * p.Hq + h) * p.Sq + row0 + lr] = sum > 0.f ? top * p.scale + logf(sum) : -INFINITY;
+    if (row_of(lr) < p.Sq) {
+      p.lse[(static_cast<int64_t>(b) * p.Hq + head_of(lr)) * p.Sq + row_of(lr)] = sum > 0.f ? top * p.scale + logf(sum) : -INFINITY;
     }
   }
   named_bar_sync(1, 128);
@@ -128,7 +132,7 @@ __device__ __forceinline__ void merge_split(const FwdParams& p, const uint8_t* s
   static_assert(kShare % (kStep * kBatch) == 0, "whole batches");
 #pragma unroll 1
   for (int i0 = tid / kLanes; i0 < kShare; i0 += kStep * kBatch) {
-    if (row0 + rank * kShare + i0 >= p.Sq) break;
+    if (!(kWindow && paired) && row0 + rank * kShare + i0 >= p.Sq) break;
     float4 o[kBatch][kPeers];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
@@ -138,7 +142,7 @@ __device__ __forceinline__ void merge_split(const FwdParams& p, const uint8_t* s
     }
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const int i = i0 + u * kStep, q_row = row0 + rank * kShare + i;
+      const int i = i0 + u * kStep, q_row = row_of(rank * kShare + i), h = head_of(rank * kShare + i);
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int r = 0; r < kPeers; ++r) {
@@ -204,7 +208,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
 
   // ---- which (pair, head, batch) this CTA owns: head groups keep K/V in L2, and inside a
   // group the heaviest (latest) causal pairs are scheduled first.
-  const int total_bh = p.B * p.Hq;
+  const int total_bh = kWindow && sched.paired ? p.B * p.Hq / 2 : p.B * p.Hq;
   int pair, bh;
   {
     const int per_group = sched.group * sched.npairs;
@@ -214,18 +218,22 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
     pair = sched.npairs - 1 - within / gsize;
     bh = g * sched.group + within % gsize;
   }
+  const bool paired = kWindow && kTiles == 2 && sched.paired;
+  if (paired) bh *= 2;
   const int b = bh / p.Hq;
-  const int h = bh - b * p.Hq;
-  const int hk = h / (p.Hq / p.Hkv);
-  const int row0 = pair * kTiles * kBM;  // first query row of tile 0
+  const int h0 = bh - b * p.Hq;
+  const int hk = h0 / (p.Hq / p.Hkv);
+  const int row0 = pair * (paired ? 1 : kTiles) * kBM;  // first query row of tile 0
+  const int tile_rows = paired ? 0 : kBM;               // from a tile's first row to the next tile's
+  auto head_of = [&](int t) { return paired ? h0 + t : h0; };
 
   // KV tiles each query tile visits
   int n_t[2] = {0, 0};
   KeyBlocks list = {0, 0, 0};   // under a window: the blocks of this unit, in order; a tile visits the first n_t of them
-  if constexpr (kWindow) list = window_blocks<kBN>(row0 + p.causal_off, min(row0 + kTiles * kBM, p.Sq) - 1 + p.causal_off, p.Sk, p.window, p.sinks);
+  if constexpr (kWindow) list = window_blocks<kBN>(row0 + p.causal_off, min(row0 + (kTiles - 1) * tile_rows + kBM, p.Sq) - 1 + p.causal_off, p.Sk, p.window, p.sinks);
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) {
-    const int r0 = row0 + t * kBM;
+    const int r0 = row0 + t * tile_rows;
     if (r0 >= p.Sq) {
       n_t[t] = 0;
     } else if constexpr (kWindow) {
@@ -250,6 +258,14 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
     for (int t = 0; t < kTiles; ++t) n_t[t] = max(0, min(n_t[t], j_end) - j_first);
   }
   const int n_max = max(n_t[0], n_t[1]);
+  // The second half of the last block of sinks, where it has none (nor a window's keys: a gap follows), is not computed: block
+  // `half_block` of this CTA has one half.  `whole` half-blocks come before half-block (j, half) of a tile.
+  int half_block = -1;
+  if constexpr (kWindow) {
+    if (list.n_sink > 0 && (p.sinks - 1) % kBN < kBN / 2) half_block = list.n_sink - 1 - j_first;
+  }
+  auto is_left_out = [&](int j, int half) { return kWindow && half == 1 && j == half_block; };
+  auto left_out = [&](int j) { return kWindow && half_block >= 0 && j > half_block ? 1 : 0; };   // half-blocks ahead of block j
   // first key row of this CTA's K/V block j
   auto key_row = [&](int j) { return (kWindow ? list.at(j_first + j) : j_first + j) * kBN; };
 
@@ -269,9 +285,9 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
     const int krow = key_row(seq >> 1);
     if (seq == 0) {
       // Q tile 0 rides ahead of K_0, Q tile 1 right behind it
-      if (n_t[0] > 0) load_tile(&mapQ, sQ, &q_full[0], row0, h);
+      if (n_t[0] > 0) load_tile(&mapQ, sQ, &q_full[0], row0, h0);
       load_tile(&mapK, sKV + slot * Cfg::kTileBytes, &kv_full[slot], krow, hk);
-      if (kTiles == 2 && n_t[1] > 0) load_tile(&mapQ, sQ + Cfg::kTileBytes, &q_full[1], row0 + kBM, h);
+      if (kTiles == 2 && n_t[1] > 0) load_tile(&mapQ, sQ + Cfg::kTileBytes, &q_full[1], row0 + tile_rows, head_of(1));
     } else {
       load_tile((seq & 1) ? &mapV : &mapK, sKV + slot * Cfg::kTileBytes, &kv_full[slot], krow, hk);
     }
@@ -329,7 +345,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem_base + lane_off + (t == 0 ? Cfg::kTmemS0 : Cfg::kTmemS1);
     const float c = p.scale_log2;
-    const int q_row = row0 + t * kBM + row;  // global query row
+    const int r0 = row0 + t * tile_rows;     // the tile's first query row
+    const int q_row = r0 + row;              // global query row
     // m: the row maximum the exponentials are taken against.  It is only raised when the
     // true maximum has grown by more than 2^kRescaleLog2 (lazy rescaling), so most KV
     // tiles need no correction of O; l is the row sum relative to that same m.
@@ -339,26 +356,23 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
     for (int j = 0; j < nblk; ++j) {
       uint32_t keep_bits[4] = {0, 0, 0, 0};   // dropout: one bit per column of this row of the KV block
       if constexpr (kDropout) {
-        dropout_row_bits(p.drop, b * p.Hq + h, q_row, key_row(j), keep_bits);
+        dropout_row_bits(p.drop, b * p.Hq + h0, q_row, key_row(j), keep_bits);
       }
       // The 128 key columns of a block are scored, exponentiated and fed to P V in two halves of
       // 64, each with its own S columns: while this warp works on one half, the tensor pipe runs
       // P V of the other half and then the next block's Q K^T into the columns that P V just freed.
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
+        if (is_left_out(j, half)) continue;
         const uint32_t tSh = tS + half * 64;
-        B200FA_WAIT(&s_full[t * 2 + half], j & 1, 0x100 + t * 2 + half);
+        B200FA_WAIT(&s_full[t * 2 + half], (half == 1 ? j - left_out(j) : j) & 1, 0x100 + t * 2 + half);
         tc_fence_after();
         uint32_t s[64];
         float* sf = reinterpret_cast<float*>(s);
         const int col0 = key_row(j) + half * 64;
         // mask: causal diagonal and/or columns beyond Sk, columns between the sinks and the window
-        bool need_mask = (kCausal && (col0 + 63 > row0 + t * kBM + p.causal_off)) || (col0 + 64 > p.Sk);
-        bool need_low = false;
-        if constexpr (kWindow) {
-          need_low = col0 <= row0 + t * kBM + kBM - 1 + p.causal_off - p.window && col0 + 63 >= p.sinks;
-          need_mask |= need_low;
-        }
+        const bool need_mask = (kCausal && (col0 + 63 > r0 + p.causal_off)) || (col0 + 64 > p.Sk);
+        const bool need_low = kWindow && col0 <= r0 + kBM - 1 + p.causal_off - p.window && col0 + 63 >= p.sinks;
         auto load_scores = [&]() {
           tmem_ld32(tSh + 0, s + 0);
           tmem_ld32(tSh + 32, s + 32);
@@ -369,8 +383,15 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
             for (int i = 0; i < 64; ++i) {
               if (col0 + i > limit) sf[i] = -INFINITY;
             }
-            if (kWindow && need_low) {
-              const int before = q_row + p.causal_off - p.window;   // the last column ahead of the row's window
+          }
+          if (kWindow && need_low) {
+            const int before = q_row + p.causal_off - p.window;   // the last column ahead of the row's window
+            if (col0 >= p.sinks) {
+#pragma unroll
+              for (int i = 0; i < 64; ++i) {
+                if (col0 + i <= before) sf[i] = -INFINITY;
+              }
+            } else {
 #pragma unroll
               for (int i = 0; i < 64; ++i) {
                 if (col0 + i <= before && col0 + i >= p.sinks) sf[i] = -INFINITY;
@@ -407,7 +428,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
           sc = ex2_approx((m - m_new) * c);
           m = m_new;
         }
-        const int hb = 2 * j + half;   // half-block index
+        const int hb = 2 * j + half - left_out(j);   // half-block index
         if (hb > 0 && any_moved) {
           B200FA_WAIT(&pv_done[t], (hb - 1) & 1, 0x108 + t);
           tc_fence_after();
@@ -430,9 +451,9 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
         // leaving it idle together.  (Only the overlap depends on the turns, no result does.)
         if constexpr (kTiles == 2) {
           if (t == 0) {
-            if (hb > 0 && hb - 1 < 2 * n_t[1]) { B200FA_WAIT(&xturn[warp & 3], (hb - 1) & 1, 0x110); }
+            if (hb > 0 && hb - 1 < 2 * n_t[1] - left_out(n_t[1])) { B200FA_WAIT(&xturn[warp & 3], (hb - 1) & 1, 0x110); }
           } else {
-            if (hb < 2 * n_t[0]) { B200FA_WAIT(&xturn[4 + (warp & 3)], hb & 1, 0x111); }
+            if (hb < 2 * n_t[0] - left_out(n_t[0])) { B200FA_WAIT(&xturn[4 + (warp & 3)], hb & 1, 0x111); }
           }
         }
         const float mc = kWindow && m == -INFINITY ? 0.f : m * c;
@@ -485,7 +506,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
       // a row that saw no key at all (possible under a bottom-right aligned mask) is 0 with lse -inf
       float inv_l = l > 0.f ? 1.f / l : 0.f;
       if constexpr (kDropout) inv_l *= p.drop.inv_keep;
-      const int q_row = row0 + t * kBM + row;
+      const int h = head_of(t), r0 = row0 + t * tile_rows, q_row = r0 + row;
       const uint32_t tO = tmem_base + lane_off + (t == 0 ? Cfg::kTmemO0 : Cfg::kTmemO1);
       // The 16-bit output tile is staged in this query tile's own Q buffer (every MMA that
       // read it has completed), in the swizzled box layout, and leaves through TMA stores:
@@ -519,7 +540,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
         if (!mbar_wait(&o_ready[t], 0, abort_flag, p.status, 0x218 + t, p.wait_budget)) return false;
 #pragma unroll
         for (int cs = 0; cs < Cfg::kSub; ++cs) {
-          tma_store_4d(&mapO, stage + cs * kSubTileBytes, cs * 64, row0 + t * kBM, h, b);
+          tma_store_4d(&mapO, stage + cs * kSubTileBytes, cs * 64, r0, h, b);
         }
         tma_store_commit();
       }
@@ -562,9 +583,9 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
       }
       cluster_sync();
       peers_met = true;
-      if (sched.splits == 2) merge_split<kD, kTiles, kBf16, 2>(p, sKV, sMsg, sMax, sQ, abort_flag, rank, b, h, row0);
-      else if (sched.splits == 4) merge_split<kD, kTiles, kBf16, 4>(p, sKV, sMsg, sMax, sQ, abort_flag, rank, b, h, row0);
-      else merge_split<kD, kTiles, kBf16, 8>(p, sKV, sMsg, sMax, sQ, abort_flag, rank, b, h, row0);
+      if (sched.splits == 2) merge_split<kD, kTiles, kBf16, 2, kWindow>(p, sKV, sMsg, sMax, sQ, abort_flag, rank, b, h0, row0, paired);
+      else if (sched.splits == 4) merge_split<kD, kTiles, kBf16, 4, kWindow>(p, sKV, sMsg, sMax, sQ, abort_flag, rank, b, h0, row0, paired);
+      else merge_split<kD, kTiles, kBf16, 8, kWindow>(p, sKV, sMsg, sMax, sQ, abort_flag, rank, b, h0, row0, paired);
     } else {
       // (a tile that sees its last KV block a step before the other is written out while the other still runs)
       if (!epilogue(0)) goto teardown;
@@ -620,8 +641,10 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
         tc_fence_after();
         issue_qk(0, 0);
         umma_commit(&s_full[t * 2]);
-        issue_qk(0, 1);
-        umma_commit(&s_full[t * 2 + 1]);
+        if (!is_left_out(0, 1)) {
+          issue_qk(0, 1);
+          umma_commit(&s_full[t * 2 + 1]);
+        }
         umma_commit(&kv_empty[0]);
         int slot = 1;         // ring slot of V_j; K_{j+1} follows in the next slot
         uint32_t phase = 0;   // parity of the ring pass V_j's slot is in
@@ -635,11 +658,13 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             // one half-block: P V of this half, then the next block's Q K^T into the S columns it frees
-            B200FA_WAIT(&p_full[t * 2 + half], j & 1, 0x320 + t * 2 + half);
-            tc_fence_after();
-            issue_pv(vslot * umma_off(Cfg::kTileBytes), j == 0 && half == 0, half);
-            umma_commit(&pv_done[t]);
-            if (has_next) {
+            if (!is_left_out(j, half)) {
+              B200FA_WAIT(&p_full[t * 2 + half], (half == 1 ? j - left_out(j) : j) & 1, 0x320 + t * 2 + half);
+              tc_fence_after();
+              issue_pv(vslot * umma_off(Cfg::kTileBytes), j == 0 && half == 0, half);
+              umma_commit(&pv_done[t]);
+            }
+            if (has_next && !is_left_out(j + 1, half)) {
               issue_qk(slot * umma_off(Cfg::kTileBytes), half);
               umma_commit(&s_full[t * 2 + half]);
             }
@@ -733,7 +758,7 @@ cudaError_t launch_tiles(const CUtensorMap& mq, const CUtensorMap& mk, const CUt
     e = result[dev];
   }
   if (e != cudaSuccess) return e;
-  const int grid = sched.npairs * p.B * p.Hq;
+  const int grid = sched.npairs * p.B * (sched.paired ? p.Hq / 2 : p.Hq);
   if constexpr (kSplit) {
     cudaLaunchAttribute cluster;
     cluster.id = cudaLaunchAttributeClusterDimension;
@@ -768,13 +793,13 @@ cudaError_t launch_tiles(const CUtensorMap& mq, const CUtensorMap& mk, const CUt
 //   B4 Hq16 S300 unmasked (128)           [14] / 29 / 48 / 100      D=64 B2 Hq16 Sq256 Sk8192  86 / 49 / [38] / 45
 int choose_splits(const FwdParams& p, const FwdSched& sched) {
   if (p.drop.threshold != 0 || p.tiles_per_cta != 0) return 1;   // (no split form with dropout, nor of a forced shape)
-  const int rows = (sched.one_tile ? 1 : 2) * kBM;
+  const int rows = (sched.one_tile || sched.paired ? 1 : 2) * kBM;
   const int per_sm = sched.one_tile ? 2 : 1;
   // SMs that clusters of 1, 2, 4 and 8 CTAs of one per SM can fill: they do not cross a GPC (measured: the
   // 34th cluster of 4 and the 16th of 8 wait for a second wave)
   constexpr int kSMs[4] = {148, 148, 132, 120};
   const double fixed = p.D == 64 ? 4.0 : 3.0;   // in K/V blocks; the merge costs about as much again
-  const int64_t heads = p.whole_heads;   // a piece of a problem is split as the whole is: the same bits
+  const int64_t heads = sched.paired ? p.whole_heads / 2 : p.whole_heads;   // a piece of a problem is split as the whole is: the same bits
   if (heads > kSMs[0] * per_sm || heads * sched.npairs > kSMs[0] * per_sm) return 1;
   int best = 1;
   double best_cost = 0.0;
@@ -848,13 +873,14 @@ cudaError_t launch_mask(const CUtensorMap& mq, const CUtensorMap& mk, const CUte
 FwdSched schedule(const FwdParams& p) {
   FwdSched sched;
   sched.one_tile = choose_one_tile(p, p.tiles_per_cta);
-  const int rows = (sched.one_tile ? 1 : 2) * kBM;
+  sched.paired = p.window && !sched.one_tile && p.Hq / p.Hkv % 2 == 0;
+  const int rows = (sched.one_tile || sched.paired ? 1 : 2) * kBM;
   sched.npairs = (p.Sq + rows - 1) / rows;
   sched.nkv_total = (p.Sk + kBN - 1) / kBN;
   // keep roughly 32 MiB of K/V hot in L2: that many heads are walked together
   const int64_t kv_bytes_per_head = static_cast<int64_t>(p.Sk) * p.D * 2 * 2;
   int64_t group = (32ll << 20) / (kv_bytes_per_head > 0 ? kv_bytes_per_head : 1);
-  const int64_t total_bh = static_cast<int64_t>(p.B) * p.Hq;
+  const int64_t total_bh = static_cast<int64_t>(p.B) * (sched.paired ? p.Hq / 2 : p.Hq);
   if (group < 1) group = 1;
   if (group > total_bh) group = total_bh;
   sched.group = static_cast<int>(group);
