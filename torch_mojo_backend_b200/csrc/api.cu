@@ -336,7 +336,8 @@ int bwd_impl(const b200fa_tensor4* q, const b200fa_tensor4* k, const b200fa_tens
   p.status = status_word;
   p.wait_budget = wait_budget();
   p.parts = opt.parts;
-  p.sink_chunks = p.window && dtype != kF32 ? bwd_sink_chunks(p) : 1;
+  int sink_rows = 0;
+  p.sink_chunks = dtype == kF32 ? simt_sink_chunks(p, &sink_rows) : bwd_sink_chunks(p, &sink_rows);
   p.sink_part = reinterpret_cast<float*>(ws + statistics);
 
   DeviceGuard guard(device);
@@ -617,17 +618,18 @@ size_t b200fa_window_bwd_workspace_bytes(int64_t batch, int64_t heads_q, int64_t
                                          int64_t seqlen_k, int64_t head_dim, int dtype, int64_t window, int64_t sinks) {
   if (heads_kv <= 0 || heads_q < heads_kv || seqlen_k <= 0 || window <= 0 || sinks < 0) return 0;
   const size_t statistics = b200fa_bwd_workspace_bytes(batch, heads_q, heads_kv, seqlen_q, head_dim, dtype);
-  if (statistics == 0 || dtype == kF32 || batch > 65535 || heads_q > 65535 || seqlen_q > (1 << 24) || seqlen_k > (1 << 24)) return statistics;
+  if (statistics == 0 || batch > 65535 || heads_q > 65535 || seqlen_q > (1 << 24) || seqlen_k > (1 << 24)) return statistics;
   BwdParams p;
   std::memset(&p, 0, sizeof(p));
   p.B = static_cast<int>(batch); p.Hq = static_cast<int>(heads_q); p.Hkv = static_cast<int>(heads_kv);
   p.S = static_cast<int>(seqlen_q); p.Sk = static_cast<int>(seqlen_k);
   p.window = static_cast<int>(std::min(window, kMaxWindow));
   p.sinks = static_cast<int>(std::min(sinks, kMaxWindow));
-  const int64_t chunks = bwd_sink_chunks(p);
+  int rows = 0;
+  const int64_t chunks = dtype == kF32 ? simt_sink_chunks(p, &rows) : bwd_sink_chunks(p, &rows);
   if (chunks <= 1) return statistics;
-  const int64_t tiles = std::min<int64_t>((seqlen_k + 127) / 128, (p.sinks + 127) / 128);
-  return statistics + static_cast<size_t>(batch * heads_kv * tiles * chunks * 2 * 128 * head_dim) * 4;
+  const int64_t tiles = std::min((seqlen_k + rows - 1) / rows, static_cast<int64_t>(p.sinks + rows - 1) / rows);
+  return statistics + static_cast<size_t>(batch * heads_kv * tiles * chunks * 2 * rows * head_dim) * 4;
 }
 
 int b200fa_window_bwd(const b200fa_tensor4* q, const b200fa_tensor4* k, const b200fa_tensor4* v,

@@ -1065,20 +1065,13 @@ cudaError_t launch_mask(const CUtensorMap& mq, const CUtensorMap& mk, const CUte
 
 }  // namespace
 
-// How many blocks share the steps of a K/V tile with sinks in it.  Every query row behind such a tile sees it, so its block runs
-// (rows / 128) steps per head where the others run a window's; with few heads it would outlast all of them.  A share is at most a
-// quarter of what each SM has to do in all, and at least eight steps (the sums of a share are 128 KB at head dimension 128).
-int bwd_sink_chunks(const BwdParams& p) {
-  const int64_t m_tiles = (p.S + kTile - 1) / kTile, n_tiles = (p.Sk + kTile - 1) / kTile, pairs = static_cast<int64_t>(p.B) * p.Hkv;
-  const int64_t sink_tiles = std::min<int64_t>(n_tiles, (p.sinks + kTile - 1) / kTile);
-  if (!p.window || sink_tiles == 0) return 1;
-  const int64_t group = p.Hq / p.Hkv;
-  const int64_t sink_steps = group * m_tiles;
-  const int64_t others = group * std::min<int64_t>(m_tiles, (p.window + kTile - 1) / kTile + 1);
-  const int64_t all = pairs * (sink_tiles * sink_steps + (n_tiles - sink_tiles) * others);
-  int64_t chunks = (4 * 148 * sink_steps + all - 1) / all;
-  chunks = std::min(chunks, sink_steps / 8);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(chunks, 64)));
+// (the fp32 sums of a share are 128 KB at head dimension 128)
+int bwd_sink_chunks(const BwdParams& p, int* tile_rows) {
+  *tile_rows = kTile;
+  if (!p.window) return 1;
+  const int64_t m_tiles = (p.S + kTile - 1) / kTile, n_tiles = (p.Sk + kTile - 1) / kTile, group = p.Hq / p.Hkv;
+  return sink_chunks_for(static_cast<int64_t>(p.B) * p.Hkv, n_tiles, std::min<int64_t>(n_tiles, (p.sinks + kTile - 1) / kTile), group * m_tiles,
+                         group * std::min<int64_t>(m_tiles, (p.window + kTile - 1) / kTile + 1), 148, 8);
 }
 
 cudaError_t launch_bwd_sm100(const BwdParams& p, int dtype, cudaStream_t stream, int* launches) {

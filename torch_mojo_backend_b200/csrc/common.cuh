@@ -150,7 +150,19 @@ cudaError_t launch_bwd_fp32(const BwdParams& p, cudaStream_t stream, int* launch
 cudaError_t launch_fwd_splitkv(const SplitKvParams& p, int dtype, cudaStream_t stream, int* launches);
 cudaError_t launch_bwd_sm100(const BwdParams& p, int dtype, cudaStream_t stream, int* launches);
 cudaError_t launch_bwd_simt(const BwdParams& p, int dtype, cudaStream_t stream, int* launches);
-int bwd_sink_chunks(const BwdParams& p);   // the tensor-core backward's sink_chunks (host only; sizes, mask, window and sinks are read)
+// sink_chunks of the tensor-core and the SIMT backward, and the key rows of a tile of theirs (host only; sizes, window and sinks are read)
+int bwd_sink_chunks(const BwdParams& p, int* tile_rows);
+int simt_sink_chunks(const BwdParams& p, int* tile_rows);
+// How many blocks share the steps of a key tile with sinks in it.  Every query row behind such a tile sees it, so its block runs a step
+// for every tile of query rows where the others run a window's; with few heads it would outlast all of them.  A share is at most
+// a quarter of what each of `slots` blocks has to do in all, and at least `least` steps (it leaves two fp32 tiles to be added up).
+inline int sink_chunks_for(int64_t pairs, int64_t tiles, int64_t sink_tiles, int64_t sink_steps, int64_t other_steps, int64_t slots, int64_t least) {
+  if (sink_tiles == 0) return 1;
+  const int64_t all = pairs * (sink_tiles * sink_steps + (tiles - sink_tiles) * other_steps);
+  int64_t chunks = (4 * slots * sink_steps + all - 1) / all;
+  if (chunks > sink_steps / least) chunks = sink_steps / least;
+  return static_cast<int>(chunks < 1 ? 1 : chunks > 64 ? 64 : chunks);
+}
 cudaError_t launch_paged_append(const AppendParams& p, int dtype, cudaStream_t stream, int* launches);
 cudaError_t launch_paged_gather(const GatherParams& p, int dtype, cudaStream_t stream, int* launches);
 // `keys`: the most that a query row can see, as far as the host knows

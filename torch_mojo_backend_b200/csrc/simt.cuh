@@ -33,6 +33,8 @@
 // One translation unit per storage type (simt.cu, simt_bf16.cu, simt_f16.cu): together they are most of the
 // library's compile time.
 #pragma once
+#include <algorithm>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -370,7 +372,18 @@ __global__ void __launch_bounds__(S::NT, 1) bwd_dkdv_simt_kernel(const BwdParams
   float* sDps = sLse + kBN;                                              // [64]
   const int tx = threadIdx.x % kTX, ty = threadIdx.x / kTX;
   int tile, bh;
-  tile_and_head((p.Sk + S::BM - 1) / S::BM, p.B * p.Hkv, false, &tile, &bh);
+  const int tiles = (p.Sk + S::BM - 1) / S::BM, sink_tiles = kWin ? min(tiles, (p.sinks + S::BM - 1) / S::BM) : 0;
+  tile_and_head(kWin ? tiles + sink_tiles * (p.sink_chunks - 1) : tiles, p.B * p.Hkv, false, &tile, &bh);
+  int chunk = 0, chunks = 1;   // of a tile with sinks in it, which every later row sees: several blocks share its steps
+  if constexpr (kWin) {
+    if (tile < sink_tiles * p.sink_chunks) {
+      chunks = p.sink_chunks;
+      chunk = tile % chunks;
+      tile /= chunks;
+    } else {
+      tile -= sink_tiles * (p.sink_chunks - 1);
+    }
+  }
   const int n0 = tile * S::BM;
   const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const int group = p.Hq / p.Hkv;
@@ -386,12 +399,14 @@ __global__ void __launch_bounds__(S::NT, 1) bwd_dkdv_simt_kernel(const BwdParams
   int m_end = p.S;
   if (kWin && n0 >= p.sinks) m_end = min(p.S, max(0, min(n0 + S::BM, p.Sk) - 1 + p.window - p.causal_off));   // behind the last row that sees the tile
   const int per_head = max(0, (m_end - m_begin + kBN - 1) / kBN);
-  const int steps = group * per_head;
+  const int steps_end = kWin ? static_cast<int>(static_cast<int64_t>(group * per_head) * (chunk + 1) / chunks) : group * per_head;
+  const int steps_begin = kWin ? static_cast<int>(static_cast<int64_t>(group * per_head) * chunk / chunks) : 0;
   stage_tile<T, kD, S::BM, S::NT, 2>(sK, p.k, b, hk, n0, p.Sk);
   stage_tile<T, kD, S::BM, S::NT, 2>(sV, p.v, b, hk, n0, p.Sk);
-  if (steps > 0) stage_tile<T, kD, kBN, S::NT, 0>(sdO, p.dout, b, hk * group, m_begin, p.S);
+  if (steps_begin < steps_end)
+    stage_tile<T, kD, kBN, S::NT, 0>(sdO, p.dout, b, hk * group + steps_begin / per_head, m_begin + steps_begin % per_head * kBN, p.S);
   cp_commit();
-  for (int step = 0; step < steps; ++step) {
+  for (int step = steps_begin; step < steps_end; ++step) {
     const int h = hk * group + step / per_head;
     const int m0 = m_begin + step % per_head * kBN;
     cp_wait<0>();
@@ -441,7 +456,7 @@ __global__ void __launch_bounds__(S::NT, 1) bwd_dkdv_simt_kernel(const BwdParams
     __syncthreads();
     rows_by_dim<S, kD>(sX, sdO, tx, ty, dv);     // dV[key] += P[query][key] dO[query]
     __syncthreads();   // everyone is done with P and dO
-    if (step + 1 < steps)
+    if (step + 1 < steps_end)
       stage_tile<T, kD, kBN, S::NT, 0>(sdO, p.dout, b, hk * group + (step + 1) / per_head,
                                        m_begin + (step + 1) % per_head * kBN, p.S);
     cp_commit();
@@ -455,6 +470,13 @@ __global__ void __launch_bounds__(S::NT, 1) bwd_dkdv_simt_kernel(const BwdParams
   for (int i = 0; i < S::TM; ++i) {
     one[i] = 1.f;
     scale[i] = p.scale;
+  }
+  if (kWin && chunks > 1) {   // fp32 sums for the last kernel to add up, rows past the end among them
+    float* part = p.sink_part + ((static_cast<int64_t>(bh) * sink_tiles + tile) * chunks + chunk) * 2 * S::BM * kD;
+    const View4 sums[2] = {{part, 0, 0, kD}, {part + S::BM * kD, 0, 0, kD}};
+    store_rows<S, float, kD>(sums[0], 0, 0, 0, S::BM, tx, ty, dv, one);
+    store_rows<S, float, kD>(sums[1], 0, 0, 0, S::BM, tx, ty, dk, scale);
+    return;
   }
   store_rows<S, T, kD>(p.dk, b, hk, n0, p.Sk, tx, ty, dk, scale);
   store_rows<S, T, kD>(p.dv, b, hk, n0, p.Sk, tx, ty, dv, one);
@@ -565,6 +587,25 @@ __global__ void dpsum_simt_kernel(const BwdParams p) {
   if (lane == 0) p.dpsum[((int64_t)b * p.Hq + h) * p.Spad + s] = acc;
 }
 
+// dV and dK of the key tiles whose steps several blocks shared: the sum of their parts, in their order.  One thread per four elements.
+template <int kD>
+__global__ void sink_sum_simt_kernel(const BwdParams p, int rows, int sink_tiles) {
+  const int64_t idx = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int c = static_cast<int>(idx % (kD / 4)) * 4, row = static_cast<int>(idx / (kD / 4) % rows);
+  const int which = static_cast<int>(idx / (kD / 4) / rows % 2);
+  const int64_t slot = idx / (kD / 4) / rows / 2;   // (batch, kv head, tile)
+  const int tile = static_cast<int>(slot % sink_tiles), s = tile * rows + row;
+  const int64_t bh = slot / sink_tiles;
+  if (bh >= static_cast<int64_t>(p.B) * p.Hkv || s >= p.Sk) return;
+  const float* part = p.sink_part + ((slot * p.sink_chunks * 2 + which) * rows + row) * kD + c;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < p.sink_chunks; ++i) {
+    const float4 x = *reinterpret_cast<const float4*>(part + static_cast<int64_t>(i) * 2 * rows * kD);
+    sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+  }
+  store4(row_ptr_mut<float>(which == 0 ? p.dv : p.dk, static_cast<int>(bh / p.Hkv), static_cast<int>(bh % p.Hkv), s) + c, sum.x, sum.y, sum.z, sum.w);
+}
+
 template <typename Kernel, typename Params>
 cudaError_t launch(Kernel kern, int64_t blocks, int threads, int smem, cudaStream_t stream, const Params& p) {
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -585,6 +626,9 @@ cudaError_t launch(Kernel kern, int64_t blocks, int threads, int smem, cudaStrea
 template <int kD> using Tall = Shape<kD == 64 ? 8 : 4, kD == 64 ? 8 : 16>;
 using Short = Shape<4, 8>;
 bool short_blocks(int64_t heads, int rows) { return heads * ((rows + 63) / 64) < 3 * 148; }
+// keys of a dK/dV block
+inline int key_rows(const BwdParams& p) { return short_blocks((int64_t)p.B * p.Hkv, p.Sk) ? Short::BM : 64; }
+static_assert(Tall<64>::BM == 64 && Tall<128>::BM == 64, "key_rows");
 
 template <class S, typename T, int kD>
 cudaError_t launch_fwd_s(const FwdParams& p, cudaStream_t stream) {
@@ -605,9 +649,10 @@ cudaError_t launch_fwd_t(const FwdParams& p, cudaStream_t stream) {
 
 template <class S, typename T, int kD>
 cudaError_t launch_dkdv_s(const BwdParams& p, cudaStream_t stream) {
-  const int64_t blocks = (int64_t)p.B * p.Hkv * ((p.Sk + S::BM - 1) / S::BM);
+  int64_t blocks = (int64_t)p.B * p.Hkv * ((p.Sk + S::BM - 1) / S::BM);
   constexpr int smem = smem_bytes<S, kD>(2);
   if constexpr (sizeof(T) == 4) {
+    if (p.window) blocks += (int64_t)p.B * p.Hkv * std::min((p.Sk + S::BM - 1) / S::BM, (p.sinks + S::BM - 1) / S::BM) * (p.sink_chunks - 1);
     if (p.window) return launch(bwd_dkdv_simt_kernel<S, T, kD, false, true>, blocks, S::NT, smem, stream, p);
   }
   return p.drop.threshold != 0 ? launch(bwd_dkdv_simt_kernel<S, T, kD, true, false>, blocks, S::NT, smem, stream, p)
@@ -634,6 +679,14 @@ cudaError_t launch_bwd_t(const BwdParams& p, cudaStream_t stream) {
   e = short_blocks((int64_t)p.B * p.Hkv, p.Sk) ? launch_dkdv_s<Short, T, kD>(p, stream)
                                                    : launch_dkdv_s<Tall<kD>, T, kD>(p, stream);
   if (e != cudaSuccess) return e;
+  if constexpr (sizeof(T) == 4) {
+    if (p.window && p.sink_chunks > 1) {
+      const int rows = key_rows(p), sink_tiles = std::min((p.Sk + rows - 1) / rows, (p.sinks + rows - 1) / rows);
+      const int64_t threads = (int64_t)p.B * p.Hkv * sink_tiles * 2 * rows * (kD / 4);
+      sink_sum_simt_kernel<kD><<<(unsigned)((threads + 255) / 256), 256, 0, stream>>>(p, rows, sink_tiles);
+      if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
+  }
   return short_blocks((int64_t)p.B * p.Hq, p.S) ? launch_dq_s<Short, T, kD>(p, stream)
                                                     : launch_dq_s<Tall<kD>, T, kD>(p, stream);
 }
