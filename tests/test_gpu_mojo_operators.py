@@ -1,0 +1,140 @@
+"""Window attention and the paged cache through the `mojo` device (``-m gpu``): the same kernels as the calls in ``raw``, so the same
+bits, with autograd, streams and the device's status word around them."""
+
+import pytest
+import torch
+
+import torch_mojo_backend_b200 as tmb
+from tests.test_gpu_window import TL, BR, inputs, run_both
+from torch_mojo_backend_b200 import _lib, raw
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def mojo():
+    tmb.register_mojo_devices()
+
+
+def leaves(*ts):
+    return [tmb.from_cuda(t).requires_grad_() for t in ts]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("Sq,Sk,causal", [(500, 500, TL), (200, 700, BR)])
+def test_window_attention_and_its_gradients_are_the_kernels(Sq, Sk, causal, dtype):
+    q, k, v, grad = inputs(1, 2, 4, 2, Sq, Sk, 64, dtype)
+    want = run_both(q, k, v, grad, causal, 100, 3)
+    mq, mk, mv = leaves(q, k, v)
+    out, lse = tmb.window_attention(mq, mk, mv, 100, sinks=3, bottom_right=causal == BR, enable_gqa=True, return_lse=True)
+    assert out.requires_grad and not lse.requires_grad
+    out.backward(tmb.from_cuda(grad))
+    torch.mojo.synchronize()
+    for name, got in (("out", out.detach()), ("lse", lse), ("dq", mq.grad), ("dk", mk.grad), ("dv", mv.grad)):
+        assert torch.equal(tmb.to_cuda(got), want[name]), name
+
+
+def test_window_attention_of_a_fused_projection_keeps_its_layout():
+    B, H, S, D = 2, 4, 300, 64
+    g = torch.Generator(device="cuda").manual_seed(3)
+    fused = torch.randn(B, S, 3 * H * D, generator=g, device="cuda").bfloat16()
+    views = [t.unflatten(2, (H, D)).transpose(1, 2) for t in fused.split(H * D, 2)]
+    grad = torch.randn(B, S, H, D, generator=g, device="cuda").bfloat16().transpose(1, 2)
+    want = run_both(*(t.contiguous() for t in views), grad.contiguous(), TL, 64, 2)
+    q, k, v = leaves(*views)
+    out = tmb.window_attention(q, k, v, 64, sinks=2)
+    assert tmb.to_cuda(out.detach()).transpose(1, 2).is_contiguous()
+    grads = torch.autograd.grad(out, (q, k, v), tmb.from_cuda(grad))
+    assert torch.equal(tmb.to_cuda(out.detach()), want["out"])
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        assert torch.equal(tmb.to_cuda(got), want[name]) and tmb.to_cuda(got).transpose(1, 2).is_contiguous()
+
+
+def test_the_same_tensor_as_key_and_value_and_a_result_that_nobody_differentiates():
+    q, k, _, grad = inputs(4, 1, 2, 2, 200, 200, 64, torch.bfloat16)
+    want = run_both(q, k, k, grad, TL, 50, 0)
+    mq, mk = leaves(q, k)
+    out = tmb.window_attention(mq, mk, mk, 50)
+    out.backward(tmb.from_cuda(grad))
+    torch.mojo.synchronize()
+    assert torch.equal(tmb.to_cuda(mk.grad), want["dk"] + want["dv"])
+    with torch.no_grad():
+        assert torch.equal(tmb.to_cuda(tmb.window_attention(mq, mk, mk, 50)), want["out"])
+
+
+def test_autocast_casts_the_tensors():
+    q, k, v, _ = inputs(6, 1, 2, 2, 200, 200, 64, torch.float32)
+    want, _ = raw.window_fwd(q.bfloat16(), k.bfloat16(), v.bfloat16(), window=50)
+    mq, mk, mv = leaves(q, k, v)
+    with torch.autocast("mojo", dtype=torch.bfloat16):
+        out = tmb.window_attention(mq, mk, mv, 50)
+    assert out.dtype == torch.bfloat16 and torch.equal(tmb.to_cuda(out.detach()), want)
+    out.backward(torch.ones(out.shape, dtype=torch.bfloat16).to("mojo"))
+    assert mq.grad.dtype == torch.float32
+
+
+def test_a_training_step_on_a_side_stream_and_in_a_graph():
+    """The backward runs on the stream of the forward, whichever thread the engine calls it from."""
+    q, k, v, grad = inputs(5, 1, 4, 2, 1500, 1500, 128, torch.bfloat16)
+    want = run_both(q, k, v, grad, TL, 200, 4)
+    mq, mk, mv = leaves(q, k, v)
+    g = tmb.from_cuda(grad)
+
+    def step():
+        out = tmb.window_attention(mq, mk, mv, 200, sinks=4, enable_gqa=True)
+        return [tmb.to_cuda(t) for t in (out.detach(), *torch.autograd.grad(out, (mq, mk, mv), g))]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    side.synchronize()
+    for name, t in zip(("out", "dq", "dk", "dv"), got):
+        assert torch.equal(t, want[name]), name
+    alive = tmb.window_attention(mq, mk, mv, 200, sinks=4, enable_gqa=True)   # an eager graph of the same leaves
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for t in got:
+        t.zero_()
+    q.mul_(0.5)
+    graph.replay()
+    want = run_both(q, k, v, grad, TL, 200, 4)
+    for name, t in zip(("out", "dq", "dk", "dv"), got):
+        assert torch.equal(t, want[name]), name
+    assert alive.requires_grad
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_paged_cache_on_the_device(bits):
+    B, Hq, Hkv, D, page = 2, 8, 2, 128, 16
+    cache = tmb.PagedKVCache(12, Hkv, page, D, dtype=torch.float16, bits=bits)
+    assert cache.dtype == torch.float16
+    table = torch.tensor([[3, 5, 7, 9, 11, 0], [1, 2, 4, 6, 8, 10]], dtype=torch.int32)
+    lengths = torch.tensor([70, 33], dtype=torch.int32)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v = (torch.randn(B, h, 70, D, generator=g, device="cuda").half() for h in (Hq, Hkv, Hkv))
+    angle = torch.rand(96, 64, device="cuda", generator=g)
+    rotary = angle.cos(), angle.sin()
+    plain = raw.PagedKV.empty(12, Hkv, page, D, dtype=torch.float16, bits=bits)
+    tq = raw.paged_append(k, v, plain, table.cuda(), lengths.cuda(), new_lengths=lengths.cuda(), rotary=rotary, q=q)
+    want, want_lse = raw.paged_attention(tq, plain, table.cuda(), lengths.cuda(), new_lengths=lengths.cuda(), window=20, sinks=1)
+    gk, gv = raw.paged_gather(plain, table.cuda(), lengths.cuda(), 80)
+    m = [t.to("mojo") for t in (table, lengths)]
+    turned = cache.append(tmb.from_cuda(k), tmb.from_cuda(v), *m, new_lengths=m[1], rotary=[tmb.from_cuda(t) for t in rotary],
+                          query=tmb.from_cuda(q))
+    out, lse = cache.attention(turned, *m, new_lengths=m[1], window=20, sinks=1, return_lse=True)
+    mk, mv = cache.gather(*m, 80)
+    torch.mojo.synchronize()
+    for got, ref in ((turned, tq), (out, want), (lse, want_lse), (mk, gk), (mv, gv)):
+        assert torch.equal(tmb.to_cuda(got), ref)
+    with pytest.raises(RuntimeError, match="mojo tensor"):
+        cache.attention(tq, *m)
+    # an index out of range surfaces where the device is synchronised
+    cache.attention(turned, m[0], torch.tensor([97, 33], dtype=torch.int32).to("mojo"))
+    with pytest.raises(_lib.B200FAError) as err:
+        torch.mojo.synchronize()
+    assert err.value.code == _lib.ERR_BAD_INDEX
+    again = cache.attention(turned, *m, new_lengths=m[1], window=20, sinks=1)
+    torch.mojo.synchronize()
+    assert torch.equal(tmb.to_cuda(again), want)

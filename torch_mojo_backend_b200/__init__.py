@@ -56,7 +56,16 @@ def __getattr__(name):
         from .host_pipeline import HostAttentionPipeline
 
         return HostAttentionPipeline
+    if name == "window_attention":
+        from .window import window_attention
+
+        return window_attention
+    if name == "PagedKVCache":
+        from .paged import PagedKVCache
+
+        return PagedKVCache
     raise AttributeError(name)
 
 
-__all__ = ["register_mojo_devices", "from_cuda", "to_cuda", "pinned_empty", "HostAttentionPipeline"]
+__all__ = ["register_mojo_devices", "from_cuda", "to_cuda", "pinned_empty", "HostAttentionPipeline", "window_attention",
+           "PagedKVCache"]

@@ -288,8 +288,8 @@ def paged_append(k, v, cache: PagedKV, block_table, lengths, *, new_lengths=None
     ``new_lengths``: (B,) int32, how many of the S tokens are new ones (the first of each row; None: all).  Token s is written at
     position ``length - new + s``.  ``rotary``: (cos, sin), float32 (positions, R / 2): the first R elements turn, in pairs
     (i, i + R / 2) or, ``interleaved``, (2 i, 2 i + 1).  ``q``: (B, Hq, S, D), rotated the same way to ``q_out`` (a new tensor by
-    default; q itself will do), whose rows behind a sequence's new tokens are left as they are (zero in a new tensor).  ``status``: see
-    ``include/b200fa.h``.
+    default; q itself will do), whose rows behind a sequence's new tokens are left as they are (zero in a new tensor).  ``status``: an
+    int32 tensor of one element, zero, that reports a page, length or position out of range (include/b200fa.h).
     """
     B, Hkv, S, D = k.shape
     c, dtype, heads, head_dim, device = _paged(cache, block_table, lengths, new_lengths, B)
