@@ -384,9 +384,9 @@ template <int kKeys>
 __device__ __forceinline__ Unit unit_of(const AttendParams& p, int max_rows) {
   Unit u;
   u.b = blockIdx.z;
-  u.hk = blockIdx.y / p.row_tiles;
+  u.hk = blockIdx.y / static_cast<unsigned>(p.row_tiles);
   u.row0 = (blockIdx.y - u.hk * p.row_tiles) * max_rows;
-  u.group = p.Hq / p.c.Hkv;
+  u.group = p.group;
   Sequence seq;
   u.good = sequence_of(p.c, u.b, p.S, &seq);
   if (!u.good) {   // every row of the sequence is NaN
@@ -408,8 +408,9 @@ __device__ __forceinline__ Unit unit_of(const AttendParams& p, int max_rows) {
     u.low = u.p_last - p.window;
   }
   const int peers = gridDim.x, rank = blockIdx.x;
-  u.begin = static_cast<int>(static_cast<int64_t>(u.list.n) * rank / peers);
-  u.end = static_cast<int>(static_cast<int64_t>(u.list.n) * (rank + 1) / peers);
+  // (at most 2^20 steps and 16 peers)
+  u.begin = static_cast<int>(static_cast<unsigned>(u.list.n * rank) / static_cast<unsigned>(peers));
+  u.end = static_cast<int>(static_cast<unsigned>(u.list.n * (rank + 1)) / static_cast<unsigned>(peers));
   return u;
 }
 // place in a step of the key that is read for key `k` of it
@@ -431,7 +432,7 @@ __device__ __forceinline__ bool edge_step(const Unit& u, const AttendParams& p, 
 }
 template <typename T>
 __device__ __forceinline__ const T* query_row(const AttendParams& p, const Unit& u, int r) {
-  const int s = (u.row0 + r) / u.group, h = u.hk * u.group + u.row0 + r - s * u.group;
+  const int s = static_cast<int>(static_cast<unsigned>(u.row0 + r) / static_cast<unsigned>(u.group)), h = u.hk * u.group + u.row0 + r - s * u.group;
   return reinterpret_cast<const T*>(p.q.ptr) + static_cast<int64_t>(u.b) * p.q.sb + static_cast<int64_t>(h) * p.q.sh + static_cast<int64_t>(s) * p.q.ss;
 }
 // row of the pages that holds the first key of a step, which lies in page `page`; page 0 and `bad` for one that is none
@@ -449,10 +450,13 @@ struct RowState {
   float m[kNT][2], shift[kNT][2], limit[kNT][2], l[kNT][2];   // shift: -m, 0 as long as there is none; limit: where it moves
   float o[kNT][kTiles][4];   // O^T: [0] (slot g, row 2t) [1] (slot g, row 2t + 1) [2], [3] slot g + 8
   float z[kZ ? kNT : 1][4];  // 4 bits: sums of P vs (slots g < D / 32) and P vm (the next D / 32)
+  int pos[kNT][2];           // positions of the rows (of those behind the last, too, which are not written)
 
-  __device__ __forceinline__ void clear() {
+  __device__ __forceinline__ void clear(const Unit& u, int t) {
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) pos[n][e] = u.first_pos + static_cast<int>(static_cast<unsigned>(u.row0 + 8 * n + 2 * t + e) / static_cast<unsigned>(u.group));
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         m[n][e] = limit[n][e] = -INFINITY;
@@ -522,76 +526,118 @@ struct RowState {
       }
   }
   // -inf for the scores of keys (`first` and `second` of this thread) that a row does not see
-  __device__ __forceinline__ void mask(float (&x)[kNT][4], const AttendParams& p, const Unit& u, int first, int second, int t) const {
+  __device__ __forceinline__ void mask(float (&x)[kNT][4], const AttendParams& p, int first, int second) const {
 #pragma unroll
     for (int n = 0; n < kNT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int key = e < 2 ? first : second;
-        const int pos = u.first_pos + (u.row0 + 8 * n + 2 * t + (e & 1)) / u.group;   // (rows behind the last are not written)
-        if (key > pos || (p.window && key <= pos - p.window && key >= p.sinks)) x[n][e] = -INFINITY;
+        const int key = e < 2 ? first : second, at = pos[n][e & 1];
+        if (key > at || (p.window && key <= at - p.window && key >= p.sinks)) x[n][e] = -INFINITY;
       }
   }
 };
 
-// The last steps of a block: every warp has left its unnormalised O of row r at o + warp * stride + r * (kD + 2), and the row's max
-// and sum behind it.  They are merged in the block, then by the blocks of the cluster, each of which takes its share of (row, pair
-// of elements) from its peers' shared memory.
-template <typename T, int kD, int kWarps>
-__device__ __forceinline__ void merge(const AttendParams& p, const Unit& u, float* o, int stride, float2* ml) {
+// The last steps of a block: every warp has left its unnormalised O of row r at o + warp * stride + r * kRow, and the row's max and sum
+// behind it.  They are merged in the block, then by the blocks of the cluster, each of which takes its share of the rows'
+// 16-byte pieces from its peers' shared memory.  A row's weights are made once, by one thread.  (With each thread's own weights for
+// each pair of elements the fixed cost of a call of 16 rows was 14 us; MERGE_FIGURES.)
+template <int kD>
+constexpr int kRow = kD + 4;   // floats: a row, its max and sum, 16-byte aligned
+
+template <typename T, int kD, int kNT, int kWarps>
+__device__ __forceinline__ void merge(const AttendParams& p, const Unit& u, float* o, int stride) {
+  constexpr int kPieces = kD / 4, kRows = 8 * kNT, kThreads = kWarps * 32;
+  __shared__ float sWeight[kRows][kWarps > kMaxPeers ? kWarps : kMaxPeers];
+  __shared__ float2 sML[kRows];
   const int tid = threadIdx.x, peers = gridDim.x, rank = blockIdx.x;
+  auto write = [&](int r, int c, float4 x) {
+    const int row = u.row0 + r, s = static_cast<int>(static_cast<unsigned>(row) / static_cast<unsigned>(u.group)), h = u.hk * u.group + row - s * u.group;
+    T* dst = reinterpret_cast<T*>(p.out.ptr) + static_cast<int64_t>(u.b) * p.out.sb + static_cast<int64_t>(h) * p.out.sh + static_cast<int64_t>(s) * p.out.ss + c * 4;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_t<T>(x.x, x.y), pack_t<T>(x.z, x.w));
+  };
+  // 1 / sum, and the row's lse; a row without a key is 0 with lse -inf; a NaN stays one
+  auto finish = [&](int r, float m, float l, bool lse) {
+    if (lse) {
+      const int row = u.row0 + r, s = static_cast<int>(static_cast<unsigned>(row) / static_cast<unsigned>(u.group)), h = u.hk * u.group + row - s * u.group;
+      p.lse[(static_cast<int64_t>(u.b) * p.Hq + h) * p.S + s] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+    }
+    return l == 0.f ? 0.f : 1.f / l;
+  };
   __syncthreads();
-  for (int idx = tid; idx < u.rows * kD; idx += kWarps * 32) {
-    const int r = idx / kD, d = idx % kD;
-    const float* row = o + r * (kD + 2);
-    float mm = -INFINITY;
+  if (tid < u.rows) {
+    const float* row = o + tid * kRow<kD> + kD;
+    float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, row[w * stride + kD]);
-    const float m_use = mm == -INFINITY ? 0.f : mm;
-    float acc = 0.f, ls = 0.f;
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, row[w * stride]);
+    const float m_use = m == -INFINITY ? 0.f : m;
+    float weight[kWarps];
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float weight = exp2f(row[w * stride + kD] - m_use);
-      acc = fmaf(row[w * stride + d], weight, acc);
-      ls = fmaf(row[w * stride + kD + 1], weight, ls);
+      weight[w] = ex2_approx(row[w * stride] - m_use);   // 0 for a warp that saw no key of the row
+      l = fmaf(row[w * stride + 1], weight[w], l);
     }
-    o[r * (kD + 2) + d] = acc;   // (this thread alone reads and writes column d of row r)
-    if (d == 0) ml[r] = make_float2(mm, ls);
+    const float inv = peers == 1 ? finish(tid, m, l, true) : 1.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) sWeight[tid][w] = weight[w] * inv;
+    sML[tid] = make_float2(m, l);
   }
-  if (peers > 1) cluster_sync(); else __syncthreads();
-  for (int idx = rank * kWarps * 32 + tid; idx < u.rows * (kD / 2); idx += peers * kWarps * 32) {
-    const int r = idx / (kD / 2), d = idx % (kD / 2) * 2;
-    const uint32_t a_ml = smem_u32(ml + r), a_o = smem_u32(o + r * (kD + 2) + d);
-    float2 v[kMaxPeers], x[kMaxPeers];
+  __syncthreads();
+  for (int i = tid; i < u.rows * kPieces; i += kThreads) {
+    const int r = i / kPieces, c = i % kPieces;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < kMaxPeers; ++i) {
-      if (i < peers) {
-        v[i] = peer_load_f32x2(a_ml, i);
-        x[i] = peer_load_f32x2(a_o, i);
-      }
+    for (int w = 0; w < kWarps; ++w) {
+      const float4 x = *reinterpret_cast<const float4*>(o + w * stride + r * kRow<kD> + c * 4);
+      const float a = sWeight[r][w];
+      acc.x = fmaf(x.x, a, acc.x); acc.y = fmaf(x.y, a, acc.y); acc.z = fmaf(x.z, a, acc.z); acc.w = fmaf(x.w, a, acc.w);
     }
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+    if (peers == 1) write(r, c, acc);
+    else *reinterpret_cast<float4*>(o + r * kRow<kD> + c * 4) = acc;   // (this thread alone reads and writes the piece)
+  }
+  if (peers == 1) return;
+  cluster_sync();
+  if (tid < u.rows) {
+    const uint32_t a_ml = smem_u32(sML + tid);
+    float2 v[kMaxPeers];
+    float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int i = 0; i < kMaxPeers; ++i) {
-      if (i < peers) m = fmaxf(m, v[i].x);
-    }
+    for (int i = 0; i < kMaxPeers; ++i) v[i] = i < peers ? peer_load_f32x2(a_ml, i) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (int i = 0; i < kMaxPeers; ++i) m = fmaxf(m, v[i].x);
     const float m_use = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int i = 0; i < kMaxPeers; ++i) {
-      if (i < peers) {
-        const float w = exp2f(v[i].x - m_use);   // 0 for a peer that saw no key of the row
-        l = fmaf(v[i].y, w, l);
-        o0 = fmaf(x[i].x, w, o0);
-        o1 = fmaf(x[i].y, w, o1);
+      v[i].x = ex2_approx(v[i].x - m_use);
+      l = fmaf(v[i].y, v[i].x, l);
+    }
+    const float inv = finish(tid, m, l, rank == 0);
+#pragma unroll
+    for (int i = 0; i < kMaxPeers; ++i) sWeight[tid][i] = v[i].x * inv;
+  }
+  __syncthreads();
+  for (int i = rank * kThreads + tid; i < u.rows * kPieces; i += peers * kThreads) {
+    const int r = i / kPieces, c = i % kPieces;
+    const uint32_t at = smem_u32(o + r * kRow<kD> + c * 4);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int first = 0; first < kMaxPeers; first += 8) {   // eight loads in flight
+      if (first >= peers) break;
+      float4 x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (first + j < peers) x[j] = peer_load_f32x4(at, first + j);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (first + j < peers) {
+          const float a = sWeight[r][first + j];
+          acc.x = fmaf(x[j].x, a, acc.x); acc.y = fmaf(x[j].y, a, acc.y); acc.z = fmaf(x[j].z, a, acc.z); acc.w = fmaf(x[j].w, a, acc.w);
+        }
       }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;   // a row without a key is 0 with lse -inf; a NaN stays one
-    const int row = u.row0 + r, s = row / u.group, h = u.hk * u.group + row - s * u.group;
-    T* dst = reinterpret_cast<T*>(p.out.ptr) + static_cast<int64_t>(u.b) * p.out.sb + static_cast<int64_t>(h) * p.out.sh + static_cast<int64_t>(s) * p.out.ss + d;
-    *reinterpret_cast<uint32_t*>(dst) = pack_t<T>(o0 * inv, o1 * inv);
-    if (d == 0) p.lse[(static_cast<int64_t>(u.b) * p.Hq + h) * p.S + s] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+    write(r, c, acc);
   }
-  if (peers > 1) cluster_sync();   // no block leaves while a peer may still read its shared memory
+  cluster_sync();   // no block leaves while a peer may still read its shared memory
 }
 
 // Blocks of four warps that an SM takes, by their registers; a block of `kWide` warps has an SM to itself.
@@ -603,7 +649,7 @@ struct AttendCfg {
   static constexpr int kKeys = kBits == 4 ? 32 : kStepKeys, kStages = kNT == 2 ? 4 : 2;
   static constexpr int kCodeBytes = kKeys * kD / 2, kScaleBytes = kKeys * kD / kGroup * 4;
   static constexpr int kStageBytes = 2 * kCodeBytes + 2 * kScaleBytes;
-  static constexpr int kMergeBytes = 8 * kNT * (kD + 2) * 4;   // a warp's results (in its ring, where it has one)
+  static constexpr int kMergeBytes = 8 * kNT * kRow<kD> * 4;   // a warp's results (in its ring, where it has one)
   static constexpr int kWarpBytes = kBits == 4 ? kStages * kStageBytes : kMergeBytes;
   static_assert(kWarpBytes >= kMergeBytes && kWarpBytes % 16 == 0, "results fit the ring");
 };
@@ -615,7 +661,6 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? AttendCfg<kD, kNT, 
   constexpr unsigned kFull = 0xffffffffu;
   constexpr float kLazy = 8.f;
   extern __shared__ __align__(16) float smem_f[];
-  __shared__ float2 sML[8 * kNT];
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const Unit u = unit_of<kStepKeys>(p, 8 * kNT);
@@ -628,7 +673,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? AttendCfg<kD, kNT, 
     for (int i = 0; i < kD / 32; ++i)
       qf[n][i] = 8 * n + g < u.rows ? *(reinterpret_cast<const uint4*>(query_row<T>(p, u, 8 * n + g)) + 4 * i + t) : make_uint4(0, 0, 0, 0);
   RowState<kNT, kD / 16, false> st;
-  st.clear();
+  st.clear(u, t);
   const int32_t* table = p.c.table + static_cast<int64_t>(u.b) * p.c.table_stride;
   const int begin = u.begin + warp, end = u.end;
   bool bad_page = false;
@@ -698,7 +743,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? AttendCfg<kD, kNT, 
       for (int n = 0; n < kNT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[n][e] = fmaf(x[n][e], p.scale_log2, st.shift[n][e & 1]);
-      if (edge_step<kStepKeys>(u, p, base)) st.mask(x, p, u, base + g, base + g + 8, t);
+      if (edge_step<kStepKeys>(u, p, base)) st.mask(x, p, base + g, base + g + 8);
       st.probabilities(xs, kLazy);
       uint32_t pb[kNT][2];
 #pragma unroll
@@ -735,14 +780,14 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? AttendCfg<kD, kNT, 
       ls += __shfl_xor_sync(kFull, ls, 4);
       ls += __shfl_xor_sync(kFull, ls, 8);
       ls += __shfl_xor_sync(kFull, ls, 16);
-      float* row = mine + (8 * n + 2 * t + e) * (kD + 2);
+      float* row = mine + (8 * n + 2 * t + e) * kRow<kD>;
 #pragma unroll
       for (int j = 0; j < kD / 16; ++j)
         *reinterpret_cast<float2*>(row + 64 * (j >> 2) + 8 * g + 2 * (j & 3)) = make_float2(st.o[n][j][e], st.o[n][j][2 + e]);
       if (g == 0) *reinterpret_cast<float2*>(row + kD) = good ? make_float2(st.m[n][e], ls) : make_float2(0.f, __uint_as_float(0x7fffffffu));
     }
   }
-  merge<T, kD, kWarps>(p, u, smem_f, Cfg::kWarpBytes / 4, sML);
+  merge<T, kD, kNT, kWarps>(p, u, smem_f, Cfg::kWarpBytes / 4);
 }
 
 // ---- 4 bits.  A step is 32 keys, 5 KB at D = 128, whose halves each lie together in four pieces: eight lanes of a warp fetch them
@@ -757,7 +802,6 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? AttendCfg<kD, kNT, 
   constexpr unsigned kFull = 0xffffffffu;
   constexpr float kLazy = std::is_same<T, __half>::value ? 2.f : 8.f;
   extern __shared__ __align__(16) float smem_f[];
-  __shared__ float2 sML[8 * kNT];
   __shared__ uint64_t bars[kWarps][kStages];
   __shared__ uint32_t abort_flag;
   const int warp = warp_index(), lane = threadIdx.x & 31;
@@ -852,7 +896,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? AttendCfg<kD, kNT, 
     scale[n][1] = p.scale_log2 * __shfl_sync(kFull, up, 8 * t + 4);
   }
   RowState<kNT, kD / 16, true> st;
-  st.clear();
+  st.clear(u, t);
   const uint32_t one_v = std::is_same<T, __half>::value ? p.one_f16 : p.one_bf16;
   const uint32_t z_halves = (g / kGroups) & 1 ? 0x7632 : 0x5410;
   const int k_first = (g >> 1) + 4 * (g & 1);   // key of slot g
@@ -931,7 +975,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? AttendCfg<kD, kNT, 
       for (int n = 0; n < kNT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[h][n][e] = fmaf(x[h][n][e], scale[n][e & 1], st.shift[n][e & 1]);
-      if (!kSimple) st.mask(x[h], p, u, base + 16 * h + k_first, base + 16 * h + k_first + 8, t);
+      if (!kSimple) st.mask(x[h], p, base + 16 * h + k_first, base + 16 * h + k_first + 8);
     }
     st.probabilities(x, kLazy);
 #pragma unroll
@@ -1007,7 +1051,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? AttendCfg<kD, kNT, 
       ls += __shfl_xor_sync(kFull, ls, 4);
       ls += __shfl_xor_sync(kFull, ls, 8);
       ls += __shfl_xor_sync(kFull, ls, 16);
-      float* row = mine + (8 * n + 2 * t + e) * (kD + 2);
+      float* row = mine + (8 * n + 2 * t + e) * kRow<kD>;
 #pragma unroll
       for (int G = 0; G < kGroups; ++G) {
         const float zs = fmaf(8.f, __shfl_sync(kFull, st.z[n][e], 4 * G + t), __shfl_sync(kFull, st.z[n][e], 4 * (kGroups + G) + t));
@@ -1018,7 +1062,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? AttendCfg<kD, kNT, 
       if (g == 0) *reinterpret_cast<float2*>(row + kD) = good ? make_float2(st.m[n][e], ls) : make_float2(0.f, __uint_as_float(0x7fffffffu));
     }
   }
-  merge<T, kD, kWarps>(p, u, smem_f, Cfg::kWarpBytes / 4, sML);
+  merge<T, kD, kNT, kWarps>(p, u, smem_f, Cfg::kWarpBytes / 4);
 }
 
 // How a unit's keys are shared: `peers` blocks of a cluster, of four warps each or, `wide`, of as many as an SM takes.
@@ -1095,6 +1139,7 @@ template <typename T, int kD, int kNT, int kBits>
 cudaError_t launch_attend(AttendParams p, int64_t keys, cudaStream_t stream) {
   using Cfg = AttendCfg<kD, kNT, kBits>;
   const int rows = p.Hq / p.c.Hkv * p.S;
+  p.group = p.Hq / p.c.Hkv;
   p.row_tiles = (rows + 8 * kNT - 1) / (8 * kNT);
   p.one_f16 = kOneF16;
   p.one_bf16 = kOneBf16;
