@@ -1071,25 +1071,26 @@ struct Shares {
   bool wide;
 };
 // The cheapest by this model, in us and keys of a unit: a block alone works through `alone` (`alone_wide`) keys a us, all of them
-// together through `total`, and the two add up as cubes; clusters do not cross a GPC (seven of 18 SMs and one of 13), and a last wave
-// that is not full costs nearly as much as a full one; a peer costs 0.27 us, a wide block 1.9.  Fitted on 1384 random calls (1-1024
-// units, 64-65536 keys, spread by up to 90 %, which the host does not know, windows among them) with every share of up to 16 forced:
-// the choice takes 5.3 % more time than each call's best (99 in 100: at most 26 %); as many blocks as fit the GPU at once, 17 %.  B200, us, four-warp blocks 1 / 4 / 8 / 16 and 12- or 16-warp blocks 1 / 4 / 8 / 16: B8 Hq32 Hkv8
-// Sk32768 spread 60 % D128 16 bits 468 / 153 / 139 / 149, 267 / 134 / 154 / 202; B1 Hq8 Hkv1 Sk65536 888 / 228 / 120 / 66, 527 / 140 / 76 / 44.
-Shares choose_shares(int64_t units, int64_t keys, int D, int bits, int row_tile, int per_sm) {
+// together through `total`, and the two add up as cubes; `fits` clusters run at once (they do not cross a GPC: asked of the device),
+// and a last wave that is not full costs nearly as much as a full one; a peer costs 0.39 us, a wide block 1.9.  Fitted on 7037 random
+// calls (1-1024 units, 64-65536 keys, spread by up to 90 %, which the host does not know, windows among them) with every share of up to
+// 16 forced: the choice takes 4.7 % more time than each call's best (99 in 100: at most 26 %); as many blocks as fit at once, 21 %.
+// B200, us, four-warp blocks 1 / 4 / 8 / 16 and 12-warp blocks 1 / 4 / 8 / 16: B8 Hq32 Hkv8 Sk32768 spread 60 % D128 16 bits 468 / 153 / 139 /
+// 149, 267 / 134 / 154 / 202; B1 Hq8 Hkv1 Sk65536 888 / 228 / 120 / 66, 527 / 140 / 76 / 44.
+Shares choose_shares(int64_t units, int64_t keys, int D, int bits, int row_tile, const int* fits, const int* fits_wide) {
   static constexpr float kRates[2][2][2][3] = {   // [D = 128][16 bits][two tiles of rows]: alone, alone_wide, total
-      {{{97, 270, 20000}, {56, 54, 8100}}, {{120, 380, 26000}, {27, 180, 8000}}},
-      {{{62, 85, 12000}, {45, 59, 4800}}, {{64, 86, 8100}, {64, 46, 12000}}}};
+      {{{92, 240, 33000}, {99, 56, 18000}}, {{130, 280, 63000}, {100, 200, 17000}}},
+      {{{56, 120, 11000}, {57, 91, 5700}}, {{75, 130, 15000}, {90, 33, 12000}}}};
   const float* rate = kRates[D == 128][bits == 16][row_tile == 2];
   Shares best = {1, false};
   double least = -1.0;
   for (int wide = 0; wide < 2; ++wide) {
-    const int sm = wide ? 1 : per_sm;
     for (int peers = 1; peers <= kMaxPeers; ++peers) {
-      const int fit = peers <= 2 ? 148 * sm / peers : 7 * (18 * sm / peers) + 13 * sm / peers;
-      const double x = static_cast<double>(units) / fit, waves = 0.87 * std::ceil(x) + 0.13 * x;
+      const int fit = (wide ? fits_wide : fits)[peers];
+      if (fit < 1) continue;
+      const double x = static_cast<double>(units) / fit, waves = 0.89 * std::ceil(x) + 0.11 * x;
       const double all = static_cast<double>(units) * keys / rate[2], chain = waves * keys / peers / rate[wide];
-      const double cost = (wide ? 1.9 : 0.0) + (peers > 1 ? 0.27 * peers : 0.0) + std::cbrt(all * all * all + chain * chain * chain);
+      const double cost = (wide ? 1.9 : 0.0) + (peers > 1 ? 0.39 * peers : 0.0) + std::cbrt(all * all * all + chain * chain * chain);
       if (least < 0.0 || cost < least) {
         least = cost;
         best = Shares{peers, wide != 0};
@@ -1105,47 +1106,72 @@ constexpr auto attention_kernel() {
   else return &paged_attention_kernel<T, kD, kNT, kWarps>;
 }
 
+template <int kD, int kNT, int kBits, int kWarps>
+void config_of(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, dim3 grid, cudaStream_t stream) {
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = grid.x;
+  attr->val.clusterDim.y = 1;
+  attr->val.clusterDim.z = 1;
+  *cfg = cudaLaunchConfig_t{};
+  cfg->gridDim = grid;
+  cfg->blockDim = dim3(kWarps * 32);
+  cfg->dynamicSmemBytes = kWarps * AttendCfg<kD, kNT, kBits>::kWarpBytes;
+  cfg->stream = stream;
+  cfg->attrs = attr;
+  cfg->numAttrs = grid.x > 1 ? 1 : 0;
+}
+
+// Clusters of 1 .. 16 blocks of a kernel that the current device runs at once; the kernel is made ready for them.  Once per device.
 template <typename T, int kD, int kNT, int kBits, int kWarps>
-cudaError_t launch_attend_warps(const AttendParams& p, int peers, cudaStream_t stream) {
+cudaError_t clusters_that_fit(const int** fits) {
   constexpr auto kern = attention_kernel<T, kD, kNT, kBits, kWarps>();
-  constexpr int kSmem = kWarps * AttendCfg<kD, kNT, kBits>::kWarpBytes;
   static std::once_flag once[64];
   static cudaError_t result[64];
+  static int count[64][kMaxPeers + 1];
   int dev = 0;
   const cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   std::call_once(once[dev], [&] {
-    result[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (result[dev] == cudaSuccess) result[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr;
+    cudaError_t r = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (r == cudaSuccess) r = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarps * AttendCfg<kD, kNT, kBits>::kWarpBytes);
+    for (int peers = 1; peers <= kMaxPeers && r == cudaSuccess; ++peers) {
+      config_of<kD, kNT, kBits, kWarps>(&cfg, &attr, dim3(peers), nullptr);
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&count[dev][peers], kern, &cfg) != cudaSuccess) {   // then never of this size
+        (void)cudaGetLastError();
+        count[dev][peers] = 0;
+      }
+    }
+    result[dev] = r;
   });
-  if (result[dev] != cudaSuccess) return result[dev];
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = peers;
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(peers, p.c.Hkv * p.row_tiles, p.c.B);
-  cfg.blockDim = dim3(kWarps * 32);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = peers > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kern, p);
+  *fits = count[dev];
+  return result[dev];
 }
 
 template <typename T, int kD, int kNT, int kBits>
 cudaError_t launch_attend(AttendParams p, int64_t keys, cudaStream_t stream) {
-  using Cfg = AttendCfg<kD, kNT, kBits>;
-  const int rows = p.Hq / p.c.Hkv * p.S;
+  constexpr int kWide = AttendCfg<kD, kNT, kBits>::kWide;
+  const int *fits = nullptr, *fits_wide = nullptr;
+  cudaError_t e = clusters_that_fit<T, kD, kNT, kBits, 4>(&fits);
+  if (e == cudaSuccess) e = clusters_that_fit<T, kD, kNT, kBits, kWide>(&fits_wide);
+  if (e != cudaSuccess) return e;
   p.group = p.Hq / p.c.Hkv;
-  p.row_tiles = (rows + 8 * kNT - 1) / (8 * kNT);
+  p.row_tiles = (p.group * p.S + 8 * kNT - 1) / (8 * kNT);
   p.one_f16 = kOneF16;
   p.one_bf16 = kOneBf16;
-  const Shares s = choose_shares(static_cast<int64_t>(p.c.B) * p.c.Hkv * p.row_tiles, keys, kD, kBits, kNT, Cfg::kPerSm);
-  return s.wide ? launch_attend_warps<T, kD, kNT, kBits, Cfg::kWide>(p, s.peers, stream)
-                : launch_attend_warps<T, kD, kNT, kBits, 4>(p, s.peers, stream);
+  const Shares s = choose_shares(static_cast<int64_t>(p.c.B) * p.c.Hkv * p.row_tiles, keys, kD, kBits, kNT, fits, fits_wide);
+  const dim3 grid(s.peers, p.c.Hkv * p.row_tiles, p.c.B);
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr;
+  if (s.wide) {
+    config_of<kD, kNT, kBits, kWide>(&cfg, &attr, grid, stream);
+    return cudaLaunchKernelEx(&cfg, attention_kernel<T, kD, kNT, kBits, kWide>(), p);
+  }
+  config_of<kD, kNT, kBits, 4>(&cfg, &attr, grid, stream);
+  return cudaLaunchKernelEx(&cfg, attention_kernel<T, kD, kNT, kBits, 4>(), p);
 }
 
 template <typename T, int kD, int kBits>
