@@ -243,7 +243,8 @@ int b200fa_paged_append(const b200fa_paged_kv* cache, const b200fa_tensor4* k, c
  * Rows behind a sequence's new tokens are left as they are; a row that sees no key gets out = 0, lse = -inf.  Keys that no
  * new token of the sequence sees are not read: pages that hold none of the others may be given away.  `longest` (0: not
  * known, table_width * page_size then) is no bound but a hint, how many keys to spread over the GPU.  Sums of a row depend
- * on how many blocks share its keys, which goes by the sizes and that hint, not by the contents of the device tensors.  No
+ * on how many blocks share its keys, which goes by the sizes, that hint and the GPU, not by the contents of the device tensors.
+ * What a query does not see but another of the same call does has to have finite values (0 * inf is NaN).  No
  * workspace: the blocks that share the keys of a KV head are a cluster.  16-bit pages and 4-bit pages; rows beyond 16 of a
  * KV head's group (Hq / heads * S) read the pages again, 16 at a time (long prompts: b200fa_paged_gather, then b200fa_window_fwd
  * or b200fa_fwd).

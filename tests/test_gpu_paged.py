@@ -164,6 +164,7 @@ ATTEND = [
     ([900, 70], None, 3, 40, 2, 128, 16, 0, 0),                   # four tiles of rows
     ([513, 100, 7], [4, 1, 2], 4, 8, 2, 128, 16, 0, 0),           # padded rows
     ([40, 3, 0], [37, 3, 0], 37, 4, 2, 64, 16, 0, 0),             # a prompt; nothing at all
+    ([1500], None, 1300, 8, 2, 64, 64, 0, 0),                     # a long prompt: 325 tiles of rows
     ([1000, 30, 1], None, 1, 8, 2, 128, 16, 100, 4),              # window and sinks
     ([1000, 130, 129, 128], None, 1, 4, 4, 64, 32, 128, 0),
     ([700, 20, 40], [3, 2, 3], 3, 8, 2, 128, 16, 17, 5),          # a gap between sinks and window inside a step

@@ -114,7 +114,7 @@ def test_calls_on_a_paged_cache_validate_the_rest_before_launch():
     assert attend(t4(FAKE, (3, 3, 2, 64))) == _lib.ERR_BAD_SHAPE          # heads of q
     assert attend(t4(FAKE, (2, 4, 2, 64))) == _lib.ERR_BAD_SHAPE          # batch
     assert attend(t4(FAKE, (3, 4, 2, 128))) == _lib.ERR_BAD_SHAPE         # head dimension
-    assert attend(t4(FAKE, (3, 4, 1 << 18, 64))) == _lib.ERR_BAD_SHAPE    # grid
+    assert attend(t4(FAKE, (3, 64, 1 << 24, 64))) == _lib.ERR_BAD_SHAPE   # grid
     assert attend(out=t4(FAKE, (3, 4, 2, 64), (512, 64, 64, 1))) == _lib.ERR_BAD_STRIDE   # output rows overlap
     append = lambda k=k, v=k, q=q, q_out=q, cos=FAKE, sin=FAKE, R=64, positions=10: _lib.paged_append(
         c, k, v, q, q_out, cos, sin, R, positions, False, 0, 0)

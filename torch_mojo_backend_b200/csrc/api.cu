@@ -782,8 +782,7 @@ int b200fa_paged_attention(const b200fa_paged_kv* cache, const b200fa_tensor4* q
   if (!q || !out || !lse) return B200FA_ERR_NULL;
   const int64_t B = p.c.B, Hq = q->shape[1], S = q->shape[2];
   if (Hq <= 0 || Hq > 65535 || S <= 0 || S > (1 << 24) || Hq % p.c.Hkv != 0) return B200FA_ERR_BAD_SHAPE;
-  // one row of thread blocks per KV head and 8 query rows of its group
-  if (Hq * S > INT_MAX / 2 || p.c.Hkv * ((Hq / p.c.Hkv * S + 7) / 8) > 65535) return B200FA_ERR_BAD_SHAPE;
+  if (Hq * S > INT_MAX / 16) return B200FA_ERR_BAD_SHAPE;   // rows, and up to 16 thread blocks for 16 of them
   if (window < 0 || sinks < 0 || longest < 0) return B200FA_ERR_UNSUPPORTED;
   if (!(scale > 0.f) || !std::isfinite(scale)) return B200FA_ERR_UNSUPPORTED;
   if (reinterpret_cast<uintptr_t>(lse) % 4 != 0) return B200FA_ERR_MISALIGNED;

@@ -128,7 +128,7 @@ struct AttendParams {
   View4 q, out;                 // (B, Hq, S, D)
   float* lse;                   // (B, Hq, S)
   int Hq, S, window, sinks;     // window 0: none
-  int row_tiles, group;         // set by the launcher: tiles of rows and query heads of a KV head
+  int peers, group;             // set by the launcher: blocks that share a unit, query heads of a KV head
   long long wait_budget;        // SM cycles that a wait for a copy may take
   float scale_log2;
   uint32_t one_f16, one_bf16;   // kOneF16, kOneBf16 (paged.cu)

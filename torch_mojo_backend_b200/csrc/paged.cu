@@ -372,7 +372,8 @@ __device__ __forceinline__ void codes_of(uint32_t w, float minus, uint32_t one, 
 
 // The rows and keys of one unit, as a block sees them.
 struct Unit {
-  int b, hk, row0, rows, group;      // rows row0 .. row0 + rows - 1 of the group's (new tokens x query heads)
+  int b, hk, rank;                   // sequence, KV head, place in the cluster
+  int row0, rows, group;             // rows row0 .. row0 + rows - 1 of the group's (new tokens x query heads)
   int first_pos, p_first, p_last;    // positions of the first new token, of the unit's first row and of its last
   KeyBlocks list;                    // steps of keys
   int hidden_from, hidden_to;        // keys between the sinks and the first row's window
@@ -384,8 +385,10 @@ template <int kKeys>
 __device__ __forceinline__ Unit unit_of(const AttendParams& p, int max_rows) {
   Unit u;
   u.b = blockIdx.z;
-  u.hk = blockIdx.y / static_cast<unsigned>(p.row_tiles);
-  u.row0 = (blockIdx.y - u.hk * p.row_tiles) * max_rows;
+  u.hk = blockIdx.y;
+  const unsigned tile = blockIdx.x / static_cast<unsigned>(p.peers);
+  u.rank = blockIdx.x - tile * p.peers;
+  u.row0 = tile * max_rows;
   u.group = p.group;
   Sequence seq;
   u.good = sequence_of(p.c, u.b, p.S, &seq);
@@ -407,10 +410,9 @@ __device__ __forceinline__ Unit unit_of(const AttendParams& p, int max_rows) {
     u.hidden_to = u.p_first - p.window + 1;
     u.low = u.p_last - p.window;
   }
-  const int peers = gridDim.x, rank = blockIdx.x;
   // (at most 2^20 steps and 16 peers)
-  u.begin = static_cast<int>(static_cast<unsigned>(u.list.n * rank) / static_cast<unsigned>(peers));
-  u.end = static_cast<int>(static_cast<unsigned>(u.list.n * (rank + 1)) / static_cast<unsigned>(peers));
+  u.begin = static_cast<int>(static_cast<unsigned>(u.list.n * u.rank) / static_cast<unsigned>(p.peers));
+  u.end = static_cast<int>(static_cast<unsigned>(u.list.n * (u.rank + 1)) / static_cast<unsigned>(p.peers));
   return u;
 }
 // place in a step of the key that is read for key `k` of it
@@ -549,7 +551,7 @@ __device__ __forceinline__ void merge(const AttendParams& p, const Unit& u, floa
   constexpr int kPieces = kD / 4, kRows = 8 * kNT, kThreads = kWarps * 32;
   __shared__ float sWeight[kRows][kWarps > kMaxPeers ? kWarps : kMaxPeers];
   __shared__ float2 sML[kRows];
-  const int tid = threadIdx.x, peers = gridDim.x, rank = blockIdx.x;
+  const int tid = threadIdx.x, peers = p.peers, rank = u.rank;
   auto write = [&](int r, int c, float4 x) {
     const int row = u.row0 + r, s = static_cast<int>(static_cast<unsigned>(row) / static_cast<unsigned>(u.group)), h = u.hk * u.group + row - s * u.group;
     T* dst = reinterpret_cast<T*>(p.out.ptr) + static_cast<int64_t>(u.b) * p.out.sb + static_cast<int64_t>(h) * p.out.sh + static_cast<int64_t>(s) * p.out.ss + c * 4;
@@ -1107,9 +1109,9 @@ constexpr auto attention_kernel() {
 }
 
 template <int kD, int kNT, int kBits, int kWarps>
-void config_of(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, dim3 grid, cudaStream_t stream) {
+void config_of(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, dim3 grid, int peers, cudaStream_t stream) {
   attr->id = cudaLaunchAttributeClusterDimension;
-  attr->val.clusterDim.x = grid.x;
+  attr->val.clusterDim.x = peers;
   attr->val.clusterDim.y = 1;
   attr->val.clusterDim.z = 1;
   *cfg = cudaLaunchConfig_t{};
@@ -1118,7 +1120,7 @@ void config_of(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, dim3 grid, cu
   cfg->dynamicSmemBytes = kWarps * AttendCfg<kD, kNT, kBits>::kWarpBytes;
   cfg->stream = stream;
   cfg->attrs = attr;
-  cfg->numAttrs = grid.x > 1 ? 1 : 0;
+  cfg->numAttrs = peers > 1 ? 1 : 0;
 }
 
 // Clusters of 1 .. 16 blocks of a kernel that the current device runs at once; the kernel is made ready for them.  Once per device.
@@ -1138,7 +1140,7 @@ cudaError_t clusters_that_fit(const int** fits) {
     cudaError_t r = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (r == cudaSuccess) r = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarps * AttendCfg<kD, kNT, kBits>::kWarpBytes);
     for (int peers = 1; peers <= kMaxPeers && r == cudaSuccess; ++peers) {
-      config_of<kD, kNT, kBits, kWarps>(&cfg, &attr, dim3(peers), nullptr);
+      config_of<kD, kNT, kBits, kWarps>(&cfg, &attr, dim3(peers), peers, nullptr);
       cfg.numAttrs = 1;
       if (cudaOccupancyMaxActiveClusters(&count[dev][peers], kern, &cfg) != cudaSuccess) {   // then never of this size
         (void)cudaGetLastError();
@@ -1159,18 +1161,19 @@ cudaError_t launch_attend(AttendParams p, int64_t keys, cudaStream_t stream) {
   if (e == cudaSuccess) e = clusters_that_fit<T, kD, kNT, kBits, kWide>(&fits_wide);
   if (e != cudaSuccess) return e;
   p.group = p.Hq / p.c.Hkv;
-  p.row_tiles = (p.group * p.S + 8 * kNT - 1) / (8 * kNT);
+  const int row_tiles = (p.group * p.S + 8 * kNT - 1) / (8 * kNT);
   p.one_f16 = kOneF16;
   p.one_bf16 = kOneBf16;
-  const Shares s = choose_shares(static_cast<int64_t>(p.c.B) * p.c.Hkv * p.row_tiles, keys, kD, kBits, kNT, fits, fits_wide);
-  const dim3 grid(s.peers, p.c.Hkv * p.row_tiles, p.c.B);
+  const Shares s = choose_shares(static_cast<int64_t>(p.c.B) * p.c.Hkv * row_tiles, keys, kD, kBits, kNT, fits, fits_wide);
+  p.peers = s.peers;
+  const dim3 grid(s.peers * row_tiles, p.c.Hkv, p.c.B);
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr;
   if (s.wide) {
-    config_of<kD, kNT, kBits, kWide>(&cfg, &attr, grid, stream);
+    config_of<kD, kNT, kBits, kWide>(&cfg, &attr, grid, s.peers, stream);
     return cudaLaunchKernelEx(&cfg, attention_kernel<T, kD, kNT, kBits, kWide>(), p);
   }
-  config_of<kD, kNT, kBits, 4>(&cfg, &attr, grid, stream);
+  config_of<kD, kNT, kBits, 4>(&cfg, &attr, grid, s.peers, stream);
   return cudaLaunchKernelEx(&cfg, attention_kernel<T, kD, kNT, kBits, 4>(), p);
 }
 
