@@ -2,8 +2,10 @@
 
 Bounds of the attention, element by element (u half a step of the type, s the relative error of a probability, A = P |V|):
   16 bits: P is rounded to the type before it multiplies V, out after        u A + u |out| + 3 s A
-  4 bits:  P vs is rounded to the type before it multiplies c - 8; the rest, P (vm + 8 vs), is fp32
-           u sum(P vs |c - 8|) + u |out| + 3 s (sum(P vs |c - 8|) + sum(P |vm + 8 vs|));  scores: sums of q ks c and of q km
+  4 bits:  P vs is rounded to the type before it multiplies c - 8, and P is before it multiplies vs and vm, whose sums make that
+           of P (vm + 8 vs).  With F = sum(P vs |c - 8|), G = sum(P |vm + 8 vs|):    u (F + G) + u |out| + 3 s (F + G)
+           scores: sums of q ks c and of q km
+All but u |out| times 1 + u, since it is the sum with these errors that is rounded to the type.
 A float16 has no step below 2^-24: t = 2^-25 more for each rounding to it.  Appending and reading back round once, in a given
 order: their results are equal to the formula in fp32, bit for bit.
 """
@@ -139,10 +141,11 @@ def expected(pool, q, b, n, window, sinks):
         size = float((q.abs() @ (ks + km).double().repeat_interleave(group, 0).mT).max()) * D ** -0.5
     e = size * D * 2 ** -23 + 2.0 ** -20 + int(seen.sum(1).max()) * 2.0 ** -24
     if pool.bits == 16:
-        bound = u * (a + out.abs()) + t + t * (seen.double() @ v.abs()) + 3 * e * a
+        bound = (1 + u) * ((u + 3 * e) * a + t * (seen.double() @ v.abs())) + u * out.abs() + t
     else:
         low = low.double().repeat_interleave(group, 0)
-        bound = u * (p @ scaled) + u * out.abs() + t + t * 8 * seen.sum(1, keepdim=True) + 3 * e * (p @ scaled + p @ low)
+        bound = (u + 3 * e) * (p @ scaled + p @ low) + t * 8 * seen.sum(1, keepdim=True) + t * (seen.double() @ low)
+        bound = (1 + u) * bound + u * out.abs() + t
     return (out, bound), (lse, e + 2.0 ** -22 * lse.abs())
 
 

@@ -106,6 +106,8 @@ CASES = [
     (1, 4, 2, 600, 200, 128, BR, 50, 2),      # 400 rows without a key
     (1, 4, 2, 900, 200, 64, TL, 64, 0),       # rows whose window lies behind the last key
     (1, 4, 2, 900, 200, 128, TL, 64, 3),      # ... and who see the sinks alone
+    (2, 4, 2, 900, 100, 64, TL, 64, 129),     # ... more sinks than keys
+    (2, 4, 2, 900, 230, 128, TL, 5, 300),
     (1, 1, 1, 2900, 2900, 128, TL, 64, 4),    # few heads: the sinks' tile is shared by several blocks
     (1, 8, 2, 2100, 2100, 64, TL, 256, 200),
     (1, 4, 2, 200, 3000, 128, BR, 1500, 4),   # few heads, which share K/V: their keys are shared by several blocks

@@ -262,7 +262,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
   // `half_block` of this CTA has one half.  `whole` half-blocks come before half-block (j, half) of a tile.
   int half_block = -1;
   if constexpr (kWindow) {
-    if (list.n_sink > 0 && (p.sinks - 1) % kBN < kBN / 2) half_block = list.n_sink - 1 - j_first;
+    if (list.n_sink > 0 && (min(p.sinks, p.Sk) - 1) % kBN < kBN / 2) half_block = list.n_sink - 1 - j_first;
   }
   auto is_left_out = [&](int j, int half) { return kWindow && half == 1 && j == half_block; };
   auto left_out = [&](int j) { return kWindow && half_block >= 0 && j > half_block ? 1 : 0; };   // half-blocks ahead of block j

@@ -72,7 +72,8 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
 // then to the type, so that the results are those of the formula in fp32 whatever computes it.  Copy-bound: each element is
 // read and written once.  A row of 4 bits: scale = (max - min) / 15 rounded to the type, code = round((x - min) / scale), of the
 // elements as rounded to the type.  Where an element of a group is not finite the scale is NaN, and so is the group.
-// B200, one row a thread / this: 6 prompts of up to 1500 tokens, 16 + 4 heads, D = 64, 4 bits APPEND_FIGURES
+// B200, one row a thread / this: 6 prompts of up to 1500 tokens, 16 + 4 heads, D = 64, 4 bits: 21 / 12.9 us, most of it by the
+// reciprocal; 64 single tokens, 32 + 8 heads, D = 128, 16 bits: 2.8 us.
 // ------------------------------------------------------------------------------------------
 template <typename T, int kD>
 struct AppendCfg {
@@ -542,7 +543,7 @@ struct RowState {
 // The last steps of a block: every warp has left its unnormalised O of row r at o + warp * stride + r * kRow, and the row's max and sum
 // behind it.  They are merged in the block, then by the blocks of the cluster, each of which takes its share of the rows'
 // 16-byte pieces from its peers' shared memory.  A row's weights are made once, by one thread.  (With each thread's own weights for
-// each pair of elements the fixed cost of a call of 16 rows was 14 us; MERGE_FIGURES.)
+// each pair of elements a call of 16 keys and 16 rows on 256 KV heads took 13.9 us instead of 5.8.)
 template <int kD>
 constexpr int kRow = kD + 4;   // floats: a row, its max and sum, 16-byte aligned
 

@@ -26,7 +26,7 @@ cudaError_t launch_bwd_simt(const BwdParams& p, int dtype, cudaStream_t stream, 
   return e;
 }
 
-// B200, us, one block per tile with sinks / shared: B3 Hq8 Hkv4 S777 D64, window 200, dK/dV SINK_FIGURES
+// B200, us, one block per tile with sinks / shared: B3 Hq8 Hkv4 S777 D64, window 200, 3 sinks: dK/dV kernel 170 / 92 and 2.7 for the sums
 int simt_sink_chunks(const BwdParams& p, int* tile_rows) {
   const int rows = *tile_rows = key_rows(p);
   if (!p.window) return 1;
