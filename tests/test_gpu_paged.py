@@ -5,6 +5,8 @@ Bounds of the attention, element by element (u half a step of the type, s the re
   4 bits:  P vs is rounded to the type before it multiplies c - 8, and P is before it multiplies vs and vm, whose sums make that
            of P (vm + 8 vs).  With F = sum(P vs |c - 8|), G = sum(P |vm + 8 vs|):    u (F + G) + u |out| + 3 s (F + G)
            scores: sums of q ks c and of q km
+           The sums of P vm and of 8 P vs are taken in 32 bits and then added, so a step of theirs counts by what each of them is
+           and not by their sum: 2^-23 (keys + 4) sum(P (|vm| + 8 vs))
 All but u |out| times 1 + u, since it is the sum with these errors that is rounded to the type.
 A float16 has no step below 2^-24: t = 2^-25 more for each rounding to it.  Appending and reading back round once, in a given
 order: their results are equal to the formula in fp32, bit for bit.
@@ -97,7 +99,7 @@ class Pool:
 
     def held(self, b, n=None):
         """k, v of sequence b as the cache holds them, (Hkv, n, D) in 32 bits, and with 4 bits the sizes of the two parts that the
-        kernel takes them in: scale * code and minimum (of a value: code - 8 and the minimum + 8 scales)."""
+        kernel takes them in: scale * code and minimum (of a value: code - 8 and the minimum + 8 scales, then |minimum| + 8 scales)."""
         n = self.k[b].shape[1] if n is None else n
         page, slot = self.place(b, 0, n)
         got = []
@@ -105,19 +107,20 @@ class Pool:
                                        (self.cache.v, self.cache.v_scales, v_element(self.D))):
             rows = pages[page, :, slot].transpose(0, 1)
             if self.bits == 16:
-                got.append((rows.float(), rows.float().abs(), None))
+                got.append((rows.float(), rows.float().abs(), None, None))
                 continue
             s = scales[page, :, slot].transpose(0, 1).float()
             codes = unpacked(rows, element).unflatten(-1, (-1, 32))
             middle = 0 if pages is self.cache.k else 8
-            parts = (codes * s[..., :1] + s[..., 1:], (codes - middle).abs() * s[..., :1], (s[..., 1:] + middle * s[..., :1]).abs().expand_as(codes))
+            parts = (codes * s[..., :1] + s[..., 1:], (codes - middle).abs() * s[..., :1], (s[..., 1:] + middle * s[..., :1]).abs().expand_as(codes),
+                     (s[..., 1:].abs() + middle * s[..., :1]).expand_as(codes))
             got.append(tuple(x.flatten(-2) for x in parts))
         return got
 
 
 def expected(pool, q, b, n, window, sinks):
     """(out, its bound), (lse, its bound) of the n new tokens of sequence b; q (Hq, S, D)."""
-    (k, _, _), (v, scaled, low) = pool.held(b)
+    (k, _, _, _), (v, scaled, low, apart) = pool.held(b)
     Hq, length, D = q.shape[0], k.shape[1], q.shape[2]
     u = torch.finfo(q.dtype).eps / 2
     t = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
@@ -137,7 +140,7 @@ def expected(pool, q, b, n, window, sinks):
     # an fp32 sum of D products, each at most 2^-23 off
     size = float((q.abs() @ k.abs().mT).max()) * D ** -0.5
     if pool.bits == 4:
-        (_, ks, km), _ = pool.held(b)
+        (_, ks, km, _), _ = pool.held(b)
         size = float((q.abs() @ (ks + km).double().repeat_interleave(group, 0).mT).max()) * D ** -0.5
     e = size * D * 2 ** -23 + 2.0 ** -20 + int(seen.sum(1).max()) * 2.0 ** -24
     if pool.bits == 16:
@@ -145,6 +148,7 @@ def expected(pool, q, b, n, window, sinks):
     else:
         low = low.double().repeat_interleave(group, 0)
         bound = (u + 3 * e) * (p @ scaled + p @ low) + t * 8 * seen.sum(1, keepdim=True) + t * (seen.double() @ low)
+        bound += 2.0 ** -23 * (seen.sum(1, keepdim=True) + 4) * (p @ apart.double().repeat_interleave(group, 0))
         bound = (1 + u) * bound + u * out.abs() + t
     return (out, bound), (lse, e + 2.0 ** -22 * lse.abs())
 
@@ -296,7 +300,7 @@ def test_append_and_gather_against_the_formula(lengths, new, S, Hq, Hkv, D, page
     assert int(status) == 0
     for b, length in enumerate(lengths):
         assert (gk[b, :, length:] == 0).all() and (gv[b, :, length:] == 0).all()
-        (wk, _, _), (wv, _, _) = pool.held(b, length)
+        (wk, *_), (wv, *_) = pool.held(b, length)
         assert torch.equal(gk[b, :, :length], wk.to(dtype)) and torch.equal(gv[b, :, :length], wv.to(dtype))
 
 

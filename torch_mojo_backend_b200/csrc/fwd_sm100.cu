@@ -259,7 +259,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
   }
   const int n_max = max(n_t[0], n_t[1]);
   // The second half of the last block of sinks, where it has none (nor a window's keys: a gap follows), is not computed: block
-  // `half_block` of this CTA has one half.  `whole` half-blocks come before half-block (j, half) of a tile.
+  // `half_block` of this CTA has one half.
   int half_block = -1;
   if constexpr (kWindow) {
     if (list.n_sink > 0 && (min(p.sinks, p.Sk) - 1) % kBN < kBN / 2) half_block = list.n_sink - 1 - j_first;
