@@ -105,6 +105,57 @@ def test_a_training_step_on_a_side_stream_and_in_a_graph():
     assert alive.requires_grad
 
 
+@pytest.mark.parametrize("how", ["one tensor twice", "views of one", "twice into a grad", "with another operator"])
+def test_what_the_engine_adds_on_a_side_stream_and_in_a_graph(how):
+    """Sums of gradients and gradients of views are the engine's, on its own thread."""
+    q, k, v, grad = inputs(7, 1, 4, 4, 2048, 2048, 128, torch.bfloat16)
+    g = tmb.from_cuda(grad)
+    if how == "views of one":
+        fused = leaves(torch.stack([q, k, v]))
+        call = lambda: tmb.window_attention(*(fused[0][i] for i in range(3)), 200)   # noqa: E731
+    else:
+        fused = leaves(q, k, v)
+        mk, mv = fused[1], fused[1 if how == "one tensor twice" else 2]
+        call = lambda: tmb.window_attention(fused[0], mk, mv, 200)   # noqa: E731
+    if how == "with another operator":
+        first = call
+        call = lambda: torch.nn.functional.scaled_dot_product_attention(first(), mk, mv, is_causal=True)   # noqa: E731
+
+    def step():
+        for t in fused:
+            t.grad = None
+        with torch.autograd.set_multithreading_enabled(how != "with another operator"):
+            for _ in range(2 if how == "twice into a grad" else 1):
+                call().backward(g)
+        return [tmb.to_cuda(t.grad).clone() for t in fused if t.grad is not None]
+
+    want = step()
+    torch.cuda.synchronize()
+    busy = torch.ones(8192, 8192, device="cuda")
+    side = torch.cuda.Stream()
+    for on in (side, torch.cuda.default_stream()):   # the stream that is behind
+        torch.cuda.synchronize()
+        with torch.cuda.stream(on):
+            for _ in range(4):
+                busy @ busy
+        with torch.cuda.stream(side):
+            got = step()
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for t in got:
+        t.zero_()
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    streams = []   # the engine's thread is back on its own
+    fused[0].register_hook(lambda _: streams.append(torch.cuda.current_stream()))
+    got = step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and set(streams) == {torch.cuda.default_stream()}
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 def test_paged_cache_on_the_device(bits):
     B, Hq, Hkv, D, page = 2, 8, 2, 128, 16

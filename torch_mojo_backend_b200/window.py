@@ -9,7 +9,9 @@ window argument no entry point reaches (torch_mojo_backend/eager_flash_attention
 
 from __future__ import annotations
 
+import contextlib
 import math
+import threading
 
 import torch
 
@@ -61,6 +63,31 @@ def _backward(dout, q, k, v, out, lse, window, sinks, causal, scale):
     return dq, dk, dv
 
 
+@contextlib.contextmanager
+def _on_stream(stream):
+    """A backward on the forward's stream.  What else the engine has to do for it (sums of a tensor's gradients, gradients of
+    views) goes to the current stream of the engine's thread: the two wait for one another, and in the end the forward's, where the
+    caller goes on, for the other.  A stream that is being captured cannot wait for one that is not: it becomes the thread's current one
+    until the engine is done."""
+    current = torch.cuda.current_stream(stream.device)
+    if current == stream:
+        yield
+        return
+    at_the_end = torch.autograd.Variable._execution_engine.queue_callback
+    with torch.cuda.stream(stream):
+        captured = torch.cuda.is_current_stream_capturing()
+        if not captured:
+            stream.wait_stream(current)
+        yield
+    if captured:
+        torch.cuda.set_stream(stream)
+        thread = threading.get_ident()
+        at_the_end(lambda: torch.cuda.set_stream(current) if threading.get_ident() == thread else None)
+    else:
+        current.wait_stream(stream)
+        at_the_end(lambda: stream.wait_stream(current))
+
+
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, value, window, sinks, causal, scale):
@@ -68,7 +95,7 @@ class _WindowAttention(torch.autograd.Function):
         out, lse = _forward(q, k, v, window, sinks, causal, scale)
         ctx.save_for_backward(query, key, value, out, lse)
         ctx.how = window, sinks, causal, scale
-        # The engine calls the backward from a thread of its own, whose current stream is not the caller's: it runs on this one
+        # The engine calls the backward from a thread of its own, whose current stream is not the caller's (`_on_stream`)
         ctx.stream = torch.cuda.current_stream(q._device_index) if q._holder.is_cuda else None
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -80,7 +107,7 @@ class _WindowAttention(torch.autograd.Function):
         if dout is None:
             return (None,) * 7
         query, key, value, out, lse = (payload(t) for t in ctx.saved_tensors)
-        with torch.cuda.stream(ctx.stream):
+        with _on_stream(ctx.stream):
             return (*_backward(payload(dout), query, key, value, out, lse, *ctx.how), None, None, None, None)
 
 
@@ -90,7 +117,8 @@ def window_attention(query, key, value, window: int, *, sinks: int = 0, bottom_r
 
     Tensors, types, ``scale`` and ``enable_gqa`` as for ``F.scaled_dot_product_attention`` on the device.  The last key a query
     i may see is i, or, ``bottom_right``, i + Sk - Sq (new queries against a longer key sequence).  Differentiable once, on the
-    stream that the call was made on; ``return_lse``: the logsumexp of the scaled, visible scores too, (B, H, Sq) float32,
+    stream that the call was made on (which a graph that also holds other operators of the device needs for all of them: on a stream that
+    is not the default one, call its backward under ``torch.autograd.set_multithreading_enabled(False)``); ``return_lse``: the logsumexp of the scaled, visible scores too, (B, H, Sq) float32,
     which has no gradient.  Under ``torch.autocast("mojo")`` the tensors are cast to its type, as for the attention operators.
     """
     if torch.is_autocast_enabled("mojo"):
