@@ -70,7 +70,8 @@ __device__ __forceinline__ float2 exp2_mufu2(float2 x) { return make_float2(ex2_
 // dV and dK MMAs); then the dV and dK accumulators; dP^T at D = 64 in a third buffer, at D = 128 in the other step's.
 // ------------------------------------------------------------------------------------------
 // Under a window a K/V tile with sinks in it is seen by every later query row, all others by those of a window.  Its steps are
-// dealt to sink_chunks blocks, which leave fp32 sums for sink_sum_kernel to add up (bwd_sink_chunks says when).
+// dealt to sink_chunks blocks, which leave fp32 sums for sink_sum_kernel to add up (bwd_sink_chunks says when).  Tensor-bound:
+// B2 Hq32 Hkv8 S8192 D128 bf16, window 1024, 4 sinks: 545 us, 1010 TFLOP/s of visible pairs, as of the causal mask on that box.
 template <int kD, bool kBf16, int kMask, bool kDropout>
 __global__ void __launch_bounds__(kDkdvThreads, 1)
 bwd_dkdv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
@@ -1066,6 +1067,9 @@ cudaError_t launch_mask(const CUtensorMap& mq, const CUtensorMap& mk, const CUte
 }  // namespace
 
 // (the fp32 sums of a share are 128 KB at head dimension 128)
+// B200, us of this kernel, one block per tile with sinks / shared + the sums: B2 Hq32 Hkv8 S8192 D128, window 1024, 4 sinks 895 /
+// 551 + 5; B1 Hq8 Hkv2 S16384, window 512 928 / 113 + 11; B1 Hq4 Hkv1 S8192, window 256, 130 sinks 454 / 30 + 5; a window of as many
+// keys as there are, B1 Hq16 Hkv4 S4096 217 / 211 + 3; B2 Hq12 S1024 D64, window 256, is not shared: 17.7.
 int bwd_sink_chunks(const BwdParams& p, int* tile_rows) {
   *tile_rows = kTile;
   if (!p.window) return 1;

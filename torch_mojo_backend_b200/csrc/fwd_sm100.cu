@@ -258,14 +258,6 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
     for (int t = 0; t < kTiles; ++t) n_t[t] = max(0, min(n_t[t], j_end) - j_first);
   }
   const int n_max = max(n_t[0], n_t[1]);
-  // The second half of the last block of sinks, where it has none (nor a window's keys: a gap follows), is not computed: block
-  // `half_block` of this CTA has one half.
-  int half_block = -1;
-  if constexpr (kWindow) {
-    if (list.n_sink > 0 && (min(p.sinks, p.Sk) - 1) % kBN < kBN / 2) half_block = list.n_sink - 1 - j_first;
-  }
-  auto is_left_out = [&](int j, int half) { return kWindow && half == 1 && j == half_block; };
-  auto left_out = [&](int j) { return kWindow && half_block >= 0 && j > half_block ? 1 : 0; };   // half-blocks ahead of block j
   // first key row of this CTA's K/V block j
   auto key_row = [&](int j) { return (kWindow ? list.at(j_first + j) : j_first + j) * kBN; };
 
@@ -363,9 +355,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
       // P V of the other half and then the next block's Q K^T into the columns that P V just freed.
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        if (is_left_out(j, half)) continue;
         const uint32_t tSh = tS + half * 64;
-        B200FA_WAIT(&s_full[t * 2 + half], (half == 1 ? j - left_out(j) : j) & 1, 0x100 + t * 2 + half);
+        B200FA_WAIT(&s_full[t * 2 + half], j & 1, 0x100 + t * 2 + half);
         tc_fence_after();
         uint32_t s[64];
         float* sf = reinterpret_cast<float*>(s);
@@ -428,7 +419,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
           sc = ex2_approx((m - m_new) * c);
           m = m_new;
         }
-        const int hb = 2 * j + half - left_out(j);   // half-block index
+        const int hb = 2 * j + half;   // half-block index
         if (hb > 0 && any_moved) {
           B200FA_WAIT(&pv_done[t], (hb - 1) & 1, 0x108 + t);
           tc_fence_after();
@@ -451,9 +442,9 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
         // leaving it idle together.  (Only the overlap depends on the turns, no result does.)
         if constexpr (kTiles == 2) {
           if (t == 0) {
-            if (hb > 0 && hb - 1 < 2 * n_t[1] - left_out(n_t[1])) { B200FA_WAIT(&xturn[warp & 3], (hb - 1) & 1, 0x110); }
+            if (hb > 0 && hb - 1 < 2 * n_t[1]) { B200FA_WAIT(&xturn[warp & 3], (hb - 1) & 1, 0x110); }
           } else {
-            if (hb < 2 * n_t[0] - left_out(n_t[0])) { B200FA_WAIT(&xturn[4 + (warp & 3)], hb & 1, 0x111); }
+            if (hb < 2 * n_t[0]) { B200FA_WAIT(&xturn[4 + (warp & 3)], hb & 1, 0x111); }
           }
         }
         const float mc = kWindow && m == -INFINITY ? 0.f : m * c;
@@ -641,10 +632,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
         tc_fence_after();
         issue_qk(0, 0);
         umma_commit(&s_full[t * 2]);
-        if (!is_left_out(0, 1)) {
-          issue_qk(0, 1);
-          umma_commit(&s_full[t * 2 + 1]);
-        }
+        issue_qk(0, 1);
+        umma_commit(&s_full[t * 2 + 1]);
         umma_commit(&kv_empty[0]);
         int slot = 1;         // ring slot of V_j; K_{j+1} follows in the next slot
         uint32_t phase = 0;   // parity of the ring pass V_j's slot is in
@@ -658,13 +647,11 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             // one half-block: P V of this half, then the next block's Q K^T into the S columns it frees
-            if (!is_left_out(j, half)) {
-              B200FA_WAIT(&p_full[t * 2 + half], (half == 1 ? j - left_out(j) : j) & 1, 0x320 + t * 2 + half);
-              tc_fence_after();
-              issue_pv(vslot * umma_off(Cfg::kTileBytes), j == 0 && half == 0, half);
-              umma_commit(&pv_done[t]);
-            }
-            if (has_next && !is_left_out(j + 1, half)) {
+            B200FA_WAIT(&p_full[t * 2 + half], j & 1, 0x320 + t * 2 + half);
+            tc_fence_after();
+            issue_pv(vslot * umma_off(Cfg::kTileBytes), j == 0 && half == 0, half);
+            umma_commit(&pv_done[t]);
+            if (has_next) {
               issue_qk(slot * umma_off(Cfg::kTileBytes), half);
               umma_commit(&s_full[t * 2 + half]);
             }
@@ -870,6 +857,11 @@ cudaError_t launch_mask(const CUtensorMap& mq, const CUtensorMap& mk, const CUte
               : launch_one<kD, kBf16, kAll, false>(mq, mk, mv, mo, p, sched, stream);
 }
 
+// Under a window two tiles of different heads share all of their blocks, two tiles of one head that lie below each other all but
+// one at each end.  B200, us, below each other / two heads: B2 Hq32 Hkv8 S8192 D128 bf16, window 1024, 4 sinks 379 / 342 (804 TFLOP/s
+// of visible pairs); Hq32 Hkv8 Sq16384 Sk20001 fp16, window 2048 625 / 591; B1 Hq8 Hkv2 S16384, window 512 91.6 / 83.6; a window of
+// as many keys as there are, B1 Hq16 Hkv4 S4096: 77.0 / 75.5.  (Leaving out the half of a block of sinks that holds none costs
+// more than it saves: the first two 344 and 597.)
 FwdSched schedule(const FwdParams& p) {
   FwdSched sched;
   sched.one_tile = choose_one_tile(p, p.tiles_per_cta);
