@@ -243,15 +243,20 @@ int b200fa_paged_append(const b200fa_paged_kv* cache, const b200fa_tensor4* k, c
  * Rows behind a sequence's new tokens are left as they are; a row that sees no key gets out = 0, lse = -inf.  Keys that no
  * new token of the sequence sees are not read: pages that hold none of the others may be given away.  `longest` (0: not
  * known, table_width * page_size then) is no bound but a hint, how many keys to spread over the GPU.  Sums of a row depend
- * on how many blocks share its keys, which goes by the sizes, that hint and the GPU, not by the contents of the device tensors.
- * What a query does not see but another of the same call does has to have finite values (0 * inf is NaN).  No
- * workspace: the blocks that share the keys of a KV head are a cluster.  16-bit pages and 4-bit pages; rows beyond 16 of a
+ * on how many blocks share its keys, which goes by the sizes, that hint, the workspace's size and the GPU, not by the contents of the device tensors.
+ * What a query does not see but another of the same call does has to have finite values (0 * inf is NaN).  The blocks
+ * that share the keys of a KV head are a cluster, of at most 16; with a `workspace` (caller-owned device scratch, 16-byte
+ * aligned, contents irrelevant, one per call in flight; or NULL) several clusters share them where there are few KV heads with
+ * many keys: up to as many as it has room for, b200fa_paged_attention_workspace_bytes(...) at most, which is 0 where one
+ * cluster is all that is used.  `longest` there: the most keys that a token sees, as far as the caller knows.  16-bit pages and 4-bit pages; rows beyond 16 of a
  * KV head's group (Hq / heads * S) read the pages again, 16 at a time (long prompts: b200fa_paged_gather, then b200fa_window_fwd
  * or b200fa_fwd).
  */
 int b200fa_paged_attention(const b200fa_paged_kv* cache, const b200fa_tensor4* q, const b200fa_tensor4* out, float* lse,
-                           int64_t window, int64_t sinks, float scale, int64_t longest, void* stream, int device,
-                           uint32_t* status_word);
+                           int64_t window, int64_t sinks, float scale, int64_t longest, void* workspace,
+                           size_t workspace_bytes, void* stream, int device, uint32_t* status_word);
+size_t b200fa_paged_attention_workspace_bytes(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t seqlen_q,
+                                              int64_t head_dim, int64_t longest);
 
 /*
  * The first S tokens of every sequence as dense k and v (batch, heads, S, head_dim) of `dtype`, rows behind a sequence's

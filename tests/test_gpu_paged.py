@@ -364,6 +364,62 @@ def test_indexes_out_of_range_are_reported_and_never_used(what, bits):
     assert not torch.equal(pool.cache.k, before[0])
 
 
+TEAMS = [
+    # lengths, S, Hq, Hkv, D, page, window, sinks
+    ([9000], 1, 8, 1, 128, 16, 0, 0),
+    ([1], 1, 8, 1, 128, 64, 0, 0),                        # far fewer keys than the table has room for: teams without any
+    ([20000, 0, 33], 1, 8, 1, 64, 64, 0, 0),
+    ([12345, 17], 3, 12, 2, 64, 32, 0, 0),                # 18 rows: two tiles
+    ([9000, 12], 1, 32, 4, 128, 64, 0, 0),
+    ([70000], 2, 4, 1, 64, 128, 65536, 5),                # a window of as many keys
+    ([9000, 8500], 4, 16, 2, 128, 16, 9000, 4),           # (sixteen units of 9000 keys: one cluster each)
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("lengths,S,Hq,Hkv,D,page,window,sinks", TEAMS)
+def test_several_clusters_share_the_keys_of_a_head(lengths, S, Hq, Hkv, D, page, window, sinks, bits, dtype):
+    pool = Pool(11, lengths, Hkv, D, page, dtype, bits, extra_width=131072 // page)
+    q = pool.draw(len(lengths), Hq, S, D)
+    new = torch.tensor([min(S, n) for n in lengths], dtype=torch.int32, device="cuda")
+    before = _lib.launch_count()
+    call = lambda **how: raw.paged_attention(q, pool.cache, pool.table, pool.lengths, new_lengths=new, window=window,   # noqa: E731
+                                             sinks=sinks, **how)
+    out, lse = call()
+    launches = 1 if window == 9000 else 2
+    assert _lib.launch_count() == before + launches
+    one, _ = call(workspace=torch.empty(0, dtype=torch.uint8, device="cuda"))
+    assert _lib.launch_count() == before + launches + 1
+    need = _lib.paged_attention_workspace_bytes(len(lengths), Hq, Hkv, S, D, 131072)
+    dirty = torch.full((need + 64,), 255, dtype=torch.uint8, device="cuda")   # NaN
+    again, again_lse = call(workspace=dirty[:need])
+    assert torch.equal(again, out) and torch.equal(again_lse, lse) and (dirty[need:] == 255).all()
+    call(workspace=dirty[:need // 3])                                         # room for fewer
+    assert (dirty[need:] == 255).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        later, _ = call()
+    graph.replay()
+    assert torch.equal(later, out)
+    for b, length in enumerate(lengths):
+        t = int(new[b])
+        assert (out[b, :, t:] == 0).all() and torch.isneginf(lse[b, :, t:]).all()
+        if t:
+            (o, ob), (l, lb) = expected(pool, q[b], b, t, window, sinks)
+            check("out", out[b, :, :t], o, ob)
+            check("one cluster", one[b, :, :t], o, ob)
+            check("lse", lse[b, :, :t], l, lb)
+    table, status = pool.table.clone(), torch.zeros(1, dtype=torch.int32, device="cuda")
+    if lengths[0]:
+        table[0, 0 if not window or sinks else (lengths[0] - 1) // page] = -1   # a page that some team reads
+        bad, bad_lse = raw.paged_attention(q, pool.cache, table, pool.lengths, new_lengths=new, window=window, sinks=sinks, status=status)
+        t = int(new[0])
+        assert _lib.status_to_error(int(status)) == _lib.ERR_BAD_INDEX
+        assert torch.isnan(bad[0, :, :t]).all() and torch.isnan(bad_lse[0, :, :t]).all()
+        assert torch.equal(bad[1:], out[1:])
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 def test_a_serving_run(bits):
     """Prompts appended, decoded with sinks and a window token by token in one captured graph whose device tensors change, and

@@ -109,6 +109,7 @@ def test_calls_on_a_paged_cache_validate_the_rest_before_launch():
     q, k = t4(FAKE, (3, 4, 2, 64)), t4(FAKE, (3, 2, 2, 64))
     attend = lambda q=q, out=None, lse=FAKE, window=0, sinks=0, scale=0.1, longest=0: _lib.paged_attention(
         c, q, out or q, lse, window, sinks, scale, longest, 0, 0)
+    assert _lib.paged_attention(c, q, q, FAKE, 0, 0, 0.1, 0, 0, 0, 0, FAKE + 4, 1 << 20) == _lib.ERR_MISALIGNED   # the workspace
     assert attend(lse=0) == _lib.ERR_NULL and attend(lse=FAKE + 1) == _lib.ERR_MISALIGNED
     assert attend(window=-1) == attend(sinks=-1) == attend(longest=-1) == attend(scale=-1.0) == _lib.ERR_UNSUPPORTED
     assert attend(t4(FAKE, (3, 3, 2, 64))) == _lib.ERR_BAD_SHAPE          # heads of q
@@ -129,6 +130,15 @@ def test_calls_on_a_paged_cache_validate_the_rest_before_launch():
     assert gather(k, t4(FAKE, (3, 2, 3, 64))) == _lib.ERR_BAD_SHAPE and gather(None, k) == _lib.ERR_NULL
     assert gather(t4(FAKE, (3, 2, 1 << 25, 64)), k) == _lib.ERR_BAD_SHAPE
     assert _lib.launch_count() == before
+
+
+def test_the_workspace_of_attention_over_a_paged_cache():
+    need = _lib.paged_attention_workspace_bytes
+    assert need(1, 8, 1, 1, 128, 100000) == 16 * 8 * 132 * 4            # 16 clusters, 8 rows, their maxima and sums
+    assert need(1, 8, 1, 4, 64, 100000) == 16 * 2 * 16 * 68 * 4         # two tiles of 16 rows
+    assert need(1, 8, 1, 1, 128, 4096) == need(64, 32, 8, 1, 128, 100000) == 0
+    assert need(1, 3, 2, 1, 128, 100000) == need(0, 8, 1, 1, 128, 100000) == need(1, 8, 0, 1, 128, 100000) == 0
+    assert need(1, 8, 1, 1, 96, 100000) == need(1, 8, 1, 1 << 40, 64, 100000) == need(1 << 62, 8, 1, 1, 64, 1 << 62) == 0
 
 
 def test_valid_calls_without_a_gpu_report_an_error():

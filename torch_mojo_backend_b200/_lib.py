@@ -10,6 +10,7 @@ fallback path, a missing library is an ``ImportError``-style hard failure.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import struct
 from typing import Sequence
@@ -58,6 +59,7 @@ EXPORTED_SYMBOLS = (
     "b200fa_window_bwd",
     "b200fa_paged_append",
     "b200fa_paged_attention",
+    "b200fa_paged_attention_workspace_bytes",
     "b200fa_paged_gather",
     "b200fa_set_wait_budget",
     "b200fa_wait_budget",
@@ -172,8 +174,10 @@ def load() -> ctypes.CDLL:
                                                        ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
     lib.b200fa_paged_append.restype = ctypes.c_int
     lib.b200fa_paged_attention.argtypes = [packed, packed, packed, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_float,
-                                           ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
+                                           ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
     lib.b200fa_paged_attention.restype = ctypes.c_int
+    lib.b200fa_paged_attention_workspace_bytes.argtypes = [ctypes.c_int64] * 6
+    lib.b200fa_paged_attention_workspace_bytes.restype = ctypes.c_size_t
     lib.b200fa_paged_gather.argtypes = [packed, packed, packed, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
     lib.b200fa_paged_gather.restype = ctypes.c_int
     lib.b200fa_dropout_threshold.argtypes = [ctypes.c_float]
@@ -311,9 +315,15 @@ def paged_append(cache: bytes, k: bytes, v: bytes, q: bytes | None, q_out: bytes
 
 
 def paged_attention(cache: bytes, q: bytes, out: bytes, lse_ptr: int, window: int, sinks: int, scale: float, longest: int,
-                    stream: int, device: int, status_ptr: int = 0) -> int:
+                    stream: int, device: int, status_ptr: int = 0, workspace_ptr: int = 0, workspace_bytes: int = 0) -> int:
     """Raw attention over a paged cache (see b200fa_paged_attention); returns the library's status code."""
-    return load().b200fa_paged_attention(cache, q, out, lse_ptr, window, sinks, scale, longest, stream, device, status_ptr)
+    return load().b200fa_paged_attention(cache, q, out, lse_ptr, window, sinks, scale, longest, workspace_ptr, workspace_bytes, stream,
+                                         device, status_ptr)
+
+
+@functools.lru_cache(maxsize=1024)   # (of sizes alone)
+def paged_attention_workspace_bytes(B: int, Hq: int, Hkv: int, S: int, D: int, longest: int) -> int:
+    return int(load().b200fa_paged_attention_workspace_bytes(B, Hq, Hkv, S, D, longest))
 
 
 def paged_gather(cache: bytes, k: bytes, v: bytes, stream: int, device: int, status_ptr: int = 0) -> int:

@@ -772,9 +772,17 @@ int b200fa_paged_gather(const b200fa_paged_kv* cache, const b200fa_tensor4* k, c
                 [&](int* n) { return launch_paged_gather(p, dtype, static_cast<cudaStream_t>(stream), n); });
 }
 
+size_t b200fa_paged_attention_workspace_bytes(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t seqlen_q, int64_t head_dim,
+                                              int64_t longest) {
+  if (batch <= 0 || heads_kv <= 0 || heads_q <= 0 || heads_q % heads_kv != 0 || seqlen_q <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  if (batch > INT_MAX || heads_q > 65535 || seqlen_q > (1 << 24)) return 0;
+  const int teams = paged_teams(batch, heads_q, heads_kv, seqlen_q, longest);
+  return teams > 1 ? teams * paged_part_bytes(batch, heads_q, heads_kv, seqlen_q, head_dim) : 0;
+}
+
 int b200fa_paged_attention(const b200fa_paged_kv* cache, const b200fa_tensor4* q, const b200fa_tensor4* out, float* lse,
-                           int64_t window, int64_t sinks, float scale, int64_t longest, void* stream, int device,
-                           uint32_t* status_word) {
+                           int64_t window, int64_t sinks, float scale, int64_t longest, void* workspace,
+                           size_t workspace_bytes, void* stream, int device, uint32_t* status_word) {
   AttendParams p;
   std::memset(&p, 0, sizeof(p));
   int rc = check_cache(cache, status_word, &p.c);
@@ -788,6 +796,9 @@ int b200fa_paged_attention(const b200fa_paged_kv* cache, const b200fa_tensor4* q
   if (reinterpret_cast<uintptr_t>(lse) % 4 != 0) return B200FA_ERR_MISALIGNED;
   if ((rc = check_view(q, B, Hq, S, p.c.D, cache->dtype, &p.q)) != B200FA_OK) return rc;
   if ((rc = check_view(out, B, Hq, S, p.c.D, cache->dtype, &p.out, true)) != B200FA_OK) return rc;
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return B200FA_ERR_MISALIGNED;
+  if (!workspace) workspace_bytes = 0;
+  p.parts = static_cast<float*>(workspace);
   p.lse = lse;
   p.Hq = static_cast<int>(Hq); p.S = static_cast<int>(S);
   p.window = static_cast<int>(std::min(window, kMaxWindow));
@@ -798,7 +809,7 @@ int b200fa_paged_attention(const b200fa_paged_kv* cache, const b200fa_tensor4* q
   if (window) keys = std::min<int64_t>(keys, int64_t(p.window) + p.sinks + S - 1);
   const int dtype = cache->dtype;
   return run_on(device, "b200fa_paged_attention",
-                [&](int* n) { return launch_paged_attention(p, dtype, keys, static_cast<cudaStream_t>(stream), n); });
+                [&](int* n) { return launch_paged_attention(p, dtype, keys, workspace_bytes, static_cast<cudaStream_t>(stream), n); });
 }
 
 int b200fa_selftest_wait_timeout(uint32_t* status_word, long long budget_cycles, void* stream, int device) {

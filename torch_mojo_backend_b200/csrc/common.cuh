@@ -128,7 +128,8 @@ struct AttendParams {
   View4 q, out;                 // (B, Hq, S, D)
   float* lse;                   // (B, Hq, S)
   int Hq, S, window, sinks;     // window 0: none
-  int peers, group;             // set by the launcher: blocks that share a unit, query heads of a KV head
+  int peers, teams, group;      // set by the launcher: blocks of a cluster, clusters that share a unit, query heads of a KV head
+  float* parts;                 // workspace, if teams > 1: rows and (max, sum) of every team (merge in paged.cu)
   long long wait_budget;        // SM cycles that a wait for a copy may take
   float scale_log2;
   uint32_t one_f16, one_bf16;   // kOneF16, kOneBf16 (paged.cu)
@@ -165,8 +166,11 @@ inline int sink_chunks_for(int64_t pairs, int64_t tiles, int64_t sink_tiles, int
 }
 cudaError_t launch_paged_append(const AppendParams& p, int dtype, cudaStream_t stream, int* launches);
 cudaError_t launch_paged_gather(const GatherParams& p, int dtype, cudaStream_t stream, int* launches);
-// `keys`: the most that a query row can see, as far as the host knows
-cudaError_t launch_paged_attention(const AttendParams& p, int dtype, int64_t keys, cudaStream_t stream, int* launches);
+// `keys`: the most that a query row can see, as far as the host knows; `part_bytes` at p.parts
+cudaError_t launch_paged_attention(const AttendParams& p, int dtype, int64_t keys, size_t part_bytes, cudaStream_t stream, int* launches);
+// Bytes of a team's part, and how many teams (clusters that share a unit) are worth a workspace for a call that sees `keys` keys
+size_t paged_part_bytes(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t S, int64_t D);
+int paged_teams(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t S, int64_t keys);
 // A one-warp kernel whose only job is to wait, with `budget` SM cycles, on a barrier nobody
 // arrives at: exercises the bounded-wait give-up path without touching the attention kernels.
 cudaError_t launch_wait_timeout_selftest(uint32_t* status, long long budget, cudaStream_t stream, int* launches);

@@ -378,6 +378,7 @@ __device__ __forceinline__ void codes_of(uint32_t w, float minus, uint32_t one, 
 // The rows and keys of one unit, as a block sees them.
 struct Unit {
   int b, hk, rank;                   // sequence, KV head, place in the cluster
+  unsigned part;                     // the cluster's number among those of all units, team by team
   int row0, rows, group;             // rows row0 .. row0 + rows - 1 of the group's (new tokens x query heads)
   int first_pos, p_first, p_last;    // positions of the first new token, of the unit's first row and of its last
   KeyBlocks list;                    // steps of keys
@@ -391,8 +392,10 @@ __device__ __forceinline__ Unit unit_of(const AttendParams& p, int max_rows) {
   Unit u;
   u.b = blockIdx.z;
   u.hk = blockIdx.y;
-  const unsigned tile = blockIdx.x / static_cast<unsigned>(p.peers);
-  u.rank = blockIdx.x - tile * p.peers;
+  const unsigned shares = p.peers * p.teams, tile = blockIdx.x / shares, share = blockIdx.x - tile * shares;
+  const unsigned team = share / static_cast<unsigned>(p.peers), tiles = gridDim.x / shares;
+  u.rank = share - team * p.peers;
+  u.part = ((blockIdx.z * gridDim.y + blockIdx.y) * tiles + tile) * p.teams + team;
   u.row0 = tile * max_rows;
   u.group = p.group;
   Sequence seq;
@@ -415,9 +418,9 @@ __device__ __forceinline__ Unit unit_of(const AttendParams& p, int max_rows) {
     u.hidden_to = u.p_first - p.window + 1;
     u.low = u.p_last - p.window;
   }
-  // (at most 2^20 steps and 16 peers)
-  u.begin = static_cast<int>(static_cast<unsigned>(u.list.n * u.rank) / static_cast<unsigned>(p.peers));
-  u.end = static_cast<int>(static_cast<unsigned>(u.list.n * (u.rank + 1)) / static_cast<unsigned>(p.peers));
+  // (at most 2^20 steps and 256 shares)
+  u.begin = static_cast<int>(static_cast<unsigned>(u.list.n * share) / shares);
+  u.end = static_cast<int>(static_cast<unsigned>(u.list.n * (share + 1)) / shares);
   return u;
 }
 // place in a step of the key that is read for key `k` of it
@@ -547,9 +550,25 @@ struct RowState {
 // The last steps of a block: every warp has left its unnormalised O of row r at o + warp * stride + r * kRow, and the row's max and sum
 // behind it.  They are merged in the block, then by the blocks of the cluster, each of which takes its share of the rows'
 // 16-byte pieces from its peers' shared memory.  A row's weights are made once, by one thread.  (With each thread's own weights for
-// each pair of elements a call of 16 keys and 16 rows on 256 KV heads took 13.9 us instead of 5.8.)
+// each pair of elements a call of 16 keys and 16 rows on 256 KV heads took 13.9 us instead of 5.8.)  Where several clusters, `teams`,
+// share a unit, each leaves its rows like a warp does, in the workspace, for paged_join_kernel.
 template <int kD>
 constexpr int kRow = kD + 4;   // floats: a row, its max and sum, 16-byte aligned
+
+template <typename T>
+__device__ __forceinline__ void write_row(const AttendParams& p, const Unit& u, int r, int c, float4 x) {
+  const int row = u.row0 + r, s = static_cast<int>(static_cast<unsigned>(row) / static_cast<unsigned>(u.group)), h = u.hk * u.group + row - s * u.group;
+  T* dst = reinterpret_cast<T*>(p.out.ptr) + static_cast<int64_t>(u.b) * p.out.sb + static_cast<int64_t>(h) * p.out.sh + static_cast<int64_t>(s) * p.out.ss + c * 4;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_t<T>(x.x, x.y), pack_t<T>(x.z, x.w));
+}
+// 1 / sum, and the row's lse; a row without a key is 0 with lse -inf; a NaN stays one
+__device__ __forceinline__ float finish_row(const AttendParams& p, const Unit& u, int r, float m, float l, bool lse) {
+  if (lse) {
+    const int row = u.row0 + r, s = static_cast<int>(static_cast<unsigned>(row) / static_cast<unsigned>(u.group)), h = u.hk * u.group + row - s * u.group;
+    p.lse[(static_cast<int64_t>(u.b) * p.Hq + h) * p.S + s] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+  }
+  return l == 0.f ? 0.f : 1.f / l;
+}
 
 template <typename T, int kD, int kNT, int kWarps>
 __device__ __forceinline__ void merge(const AttendParams& p, const Unit& u, float* o, int stride) {
@@ -557,19 +576,7 @@ __device__ __forceinline__ void merge(const AttendParams& p, const Unit& u, floa
   __shared__ float sWeight[kRows][kWarps > kMaxPeers ? kWarps : kMaxPeers];
   __shared__ float2 sML[kRows];
   const int tid = threadIdx.x, peers = p.peers, rank = u.rank;
-  auto write = [&](int r, int c, float4 x) {
-    const int row = u.row0 + r, s = static_cast<int>(static_cast<unsigned>(row) / static_cast<unsigned>(u.group)), h = u.hk * u.group + row - s * u.group;
-    T* dst = reinterpret_cast<T*>(p.out.ptr) + static_cast<int64_t>(u.b) * p.out.sb + static_cast<int64_t>(h) * p.out.sh + static_cast<int64_t>(s) * p.out.ss + c * 4;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_t<T>(x.x, x.y), pack_t<T>(x.z, x.w));
-  };
-  // 1 / sum, and the row's lse; a row without a key is 0 with lse -inf; a NaN stays one
-  auto finish = [&](int r, float m, float l, bool lse) {
-    if (lse) {
-      const int row = u.row0 + r, s = static_cast<int>(static_cast<unsigned>(row) / static_cast<unsigned>(u.group)), h = u.hk * u.group + row - s * u.group;
-      p.lse[(static_cast<int64_t>(u.b) * p.Hq + h) * p.S + s] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
-    }
-    return l == 0.f ? 0.f : 1.f / l;
-  };
+  float* const part = p.teams > 1 ? p.parts + static_cast<int64_t>(u.part) * (kRows * kRow<kD>) : nullptr;   // (never with one peer)
   __syncthreads();
   if (tid < u.rows) {
     const float* row = o + tid * kRow<kD> + kD;
@@ -583,7 +590,7 @@ __device__ __forceinline__ void merge(const AttendParams& p, const Unit& u, floa
       weight[w] = ex2_approx(row[w * stride] - m_use);   // 0 for a warp that saw no key of the row
       l = fmaf(row[w * stride + 1], weight[w], l);
     }
-    const float inv = peers == 1 ? finish(tid, m, l, true) : 1.f;
+    const float inv = peers == 1 ? finish_row(p, u, tid, m, l, true) : 1.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) sWeight[tid][w] = weight[w] * inv;
     sML[tid] = make_float2(m, l);
@@ -598,7 +605,7 @@ __device__ __forceinline__ void merge(const AttendParams& p, const Unit& u, floa
       const float a = sWeight[r][w];
       acc.x = fmaf(x.x, a, acc.x); acc.y = fmaf(x.y, a, acc.y); acc.z = fmaf(x.z, a, acc.z); acc.w = fmaf(x.w, a, acc.w);
     }
-    if (peers == 1) write(r, c, acc);
+    if (peers == 1) write_row<T>(p, u, r, c, acc);
     else *reinterpret_cast<float4*>(o + r * kRow<kD> + c * 4) = acc;   // (this thread alone reads and writes the piece)
   }
   if (peers == 1) return;
@@ -617,7 +624,8 @@ __device__ __forceinline__ void merge(const AttendParams& p, const Unit& u, floa
       v[i].x = ex2_approx(v[i].x - m_use);
       l = fmaf(v[i].y, v[i].x, l);
     }
-    const float inv = finish(tid, m, l, rank == 0);
+    if (part && rank == 0) *reinterpret_cast<float2*>(part + tid * kRow<kD> + kD) = make_float2(m, l);
+    const float inv = part ? 1.f : finish_row(p, u, tid, m, l, rank == 0);
 #pragma unroll
     for (int i = 0; i < kMaxPeers; ++i) sWeight[tid][i] = v[i].x * inv;
   }
@@ -642,9 +650,57 @@ __device__ __forceinline__ void merge(const AttendParams& p, const Unit& u, floa
         }
       }
     }
-    write(r, c, acc);
+    if (part) *reinterpret_cast<float4*>(part + r * kRow<kD> + c * 4) = acc;
+    else write_row<T>(p, u, r, c, acc);
   }
   cluster_sync();   // no block leaves while a peer may still read its shared memory
+}
+
+// The rows of a unit from its teams' parts, in the order of the teams.  `p` has one peer and one team: a block is a unit.
+constexpr int kMaxTeams = 16, kJoinThreads = 256;
+template <typename T, int kD, int kRows>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttendParams p, const int teams) {
+  constexpr int kPieces = kD / 4;
+  __shared__ float2 sML[kRows][kMaxTeams];
+  __shared__ float sWeight[kRows][kMaxTeams];
+  const int tid = threadIdx.x;
+  const Unit u = unit_of<16>(p, kRows);
+  const float* const parts = p.parts + static_cast<int64_t>(u.part) * teams * (kRows * kRow<kD>);
+  for (int i = tid; i < u.rows * teams; i += kJoinThreads) {
+    const int r = i / teams, k = i - r * teams;
+    sML[r][k] = *reinterpret_cast<const float2*>(parts + (k * kRows + r) * kRow<kD> + kD);
+  }
+  __syncthreads();
+  if (tid < u.rows) {
+    float m = -INFINITY, l = 0.f;
+    for (int k = 0; k < teams; ++k) m = fmaxf(m, sML[tid][k].x);
+    const float m_use = m == -INFINITY ? 0.f : m;
+    for (int k = 0; k < teams; ++k) {
+      const float weight = ex2_approx(sML[tid][k].x - m_use);
+      l = fmaf(sML[tid][k].y, weight, l);
+      sWeight[tid][k] = weight;
+    }
+    const float inv = finish_row(p, u, tid, m, l, true);
+    for (int k = 0; k < teams; ++k) sWeight[tid][k] *= inv;
+  }
+  __syncthreads();
+  for (int i = tid; i < u.rows * kPieces; i += kJoinThreads) {
+    const int r = i / kPieces, c = i % kPieces;
+    float4 x[kMaxTeams];
+#pragma unroll
+    for (int k = 0; k < kMaxTeams; ++k) {
+      if (k < teams) x[k] = *reinterpret_cast<const float4*>(parts + (k * kRows + r) * kRow<kD> + c * 4);
+    }
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kMaxTeams; ++k) {
+      if (k < teams) {
+        const float a = sWeight[r][k];
+        acc.x = fmaf(x[k].x, a, acc.x); acc.y = fmaf(x[k].y, a, acc.y); acc.z = fmaf(x[k].z, a, acc.z); acc.w = fmaf(x[k].w, a, acc.w);
+      }
+    }
+    write_row<T>(p, u, r, c, acc);
+  }
 }
 
 // Blocks of four warps that an SM takes, by their registers; a block of `kWide` warps has an SM to itself.
@@ -1072,9 +1128,24 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? AttendCfg<kD, kNT, 
   merge<T, kD, kNT, kWarps>(p, u, smem_f, Cfg::kWarpBytes / 4);
 }
 
-// How a unit's keys are shared: `peers` blocks of a cluster, of four warps each or, `wide`, of as many as an SM takes.
+// rows of a unit, and units, of a call
+int64_t tile_of(int64_t heads_q, int64_t heads_kv, int64_t S) { return heads_q / heads_kv * S <= 8 ? 8 : 16; }
+int64_t units_of(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t S) {
+  const int64_t tile = tile_of(heads_q, heads_kv, S);
+  return batch * heads_kv * ((heads_q / heads_kv * S + tile - 1) / tile);
+}
+
+// Several clusters share a unit where there are few units and many keys: one cluster has 16 SMs.  B200, us, one token, D = 128, one
+// cluster at most / teams: B1 Hq8 Hkv1, 16384 keys 20.5 / 18.4, 65536 47.1 / 26.6, 131072 82 / 31; B1 Hq32 Hkv4, 131072 82 / 70; B2 Hq32 Hkv8,
+// 131072 221 / 188, with 4 bits 160 / 108; 8192 keys and fewer never gain.  The join (a kernel of its own) is entered dearer than it is,
+// 6 us for about 3: where that decides, the model is no better than its 5 % (B3 Hq32 Hkv8, 32768 keys, 4 bits 53 / 59; B7 Hkv1,
+// 131072, 16 bits 100 / 110 are the worst of 30).
+constexpr int64_t kTeamKeys = 8192, kTeamUnits = 128;
+constexpr double kJoinCost = 6.0;   // us
+
+// How a unit's keys are shared: `teams` clusters of `peers` blocks, of four warps each or, `wide`, of as many as an SM takes.
 struct Shares {
-  int peers;
+  int peers, teams;
   bool wide;
 };
 // The cheapest by this model, in us and keys of a unit: a block alone works through `alone` (`alone_wide`) keys a us, all of them
@@ -1084,23 +1155,26 @@ struct Shares {
 // 16 forced: the choice takes 4.7 % more time than each call's best (99 in 100: at most 26 %); as many blocks as fit at once, 21 %.
 // B200, us, four-warp blocks 1 / 4 / 8 / 16 and 12-warp blocks 1 / 4 / 8 / 16: B8 Hq32 Hkv8 Sk32768 spread 60 % D128 16 bits 468 / 153 / 139 /
 // 149, 267 / 134 / 154 / 202; B1 Hq8 Hkv1 Sk65536 888 / 228 / 120 / 66, 527 / 140 / 76 / 44.
-Shares choose_shares(int64_t units, int64_t keys, int D, int bits, int row_tile, const int* fits, const int* fits_wide) {
+Shares choose_shares(int64_t units, int64_t keys, int D, int bits, int row_tile, int max_teams, const int* fits, const int* fits_wide) {
   static constexpr float kRates[2][2][2][3] = {   // [D = 128][16 bits][two tiles of rows]: alone, alone_wide, total
       {{{92, 240, 33000}, {99, 56, 18000}}, {{130, 280, 63000}, {100, 200, 17000}}},
       {{{56, 120, 11000}, {57, 91, 5700}}, {{75, 130, 15000}, {90, 33, 12000}}}};
   const float* rate = kRates[D == 128][bits == 16][row_tile == 2];
-  Shares best = {1, false};
+  Shares best = {1, 1, false};
   double least = -1.0;
   for (int wide = 0; wide < 2; ++wide) {
     for (int peers = 1; peers <= kMaxPeers; ++peers) {
       const int fit = (wide ? fits_wide : fits)[peers];
       if (fit < 1) continue;
-      const double x = static_cast<double>(units) / fit, waves = 0.89 * std::ceil(x) + 0.11 * x;
-      const double all = static_cast<double>(units) * keys / rate[2], chain = waves * keys / peers / rate[wide];
-      const double cost = (wide ? 1.9 : 0.0) + (peers > 1 ? 0.39 * peers : 0.0) + std::cbrt(all * all * all + chain * chain * chain);
-      if (least < 0.0 || cost < least) {
-        least = cost;
-        best = Shares{peers, wide != 0};
+      const double all = static_cast<double>(units) * keys / rate[2];
+      for (int teams = 1; teams <= (peers % 8 == 0 ? max_teams : 1); ++teams) {
+        const double x = static_cast<double>(units) * teams / fit, waves = 0.89 * std::ceil(x) + 0.11 * x;
+        const double chain = waves * keys / (peers * teams) / rate[wide];
+        const double cost = (wide ? 1.9 : 0.0) + (peers > 1 ? 0.39 * peers : 0.0) + (teams > 1 ? kJoinCost : 0.0) + std::cbrt(all * all * all + chain * chain * chain);
+        if (least < 0.0 || cost < least) {
+          least = cost;
+          best = Shares{peers, teams, wide != 0};
+        }
       }
     }
   }
@@ -1159,7 +1233,7 @@ cudaError_t clusters_that_fit(const int** fits) {
 }
 
 template <typename T, int kD, int kNT, int kBits>
-cudaError_t launch_attend(AttendParams p, int64_t keys, cudaStream_t stream) {
+cudaError_t launch_attend(AttendParams p, int64_t keys, size_t part_bytes, cudaStream_t stream, int* launches) {
   constexpr int kWide = AttendCfg<kD, kNT, kBits>::kWide;
   const int *fits = nullptr, *fits_wide = nullptr;
   cudaError_t e = clusters_that_fit<T, kD, kNT, kBits, 4>(&fits);
@@ -1169,22 +1243,34 @@ cudaError_t launch_attend(AttendParams p, int64_t keys, cudaStream_t stream) {
   const int row_tiles = (p.group * p.S + 8 * kNT - 1) / (8 * kNT);
   p.one_f16 = kOneF16;
   p.one_bf16 = kOneBf16;
-  const Shares s = choose_shares(static_cast<int64_t>(p.c.B) * p.c.Hkv * row_tiles, keys, kD, kBits, kNT, fits, fits_wide);
+  const int64_t units = static_cast<int64_t>(p.c.B) * p.c.Hkv * row_tiles;
+  const int max_teams = std::min<int64_t>(part_bytes / paged_part_bytes(p.c.B, p.Hq, p.c.Hkv, p.S, kD), paged_teams(p.c.B, p.Hq, p.c.Hkv, p.S, keys));
+  const Shares s = choose_shares(units, keys, kD, kBits, kNT, max_teams, fits, fits_wide);
   p.peers = s.peers;
-  const dim3 grid(s.peers * row_tiles, p.c.Hkv, p.c.B);
+  p.teams = s.teams;
+  const dim3 grid(s.peers * s.teams * row_tiles, p.c.Hkv, p.c.B);
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr;
   if (s.wide) {
     config_of<kD, kNT, kBits, kWide>(&cfg, &attr, grid, s.peers, stream);
-    return cudaLaunchKernelEx(&cfg, attention_kernel<T, kD, kNT, kBits, kWide>(), p);
+    e = cudaLaunchKernelEx(&cfg, attention_kernel<T, kD, kNT, kBits, kWide>(), p);
+  } else {
+    config_of<kD, kNT, kBits, 4>(&cfg, &attr, grid, s.peers, stream);
+    e = cudaLaunchKernelEx(&cfg, attention_kernel<T, kD, kNT, kBits, 4>(), p);
   }
-  config_of<kD, kNT, kBits, 4>(&cfg, &attr, grid, s.peers, stream);
-  return cudaLaunchKernelEx(&cfg, attention_kernel<T, kD, kNT, kBits, 4>(), p);
+  if (e != cudaSuccess) return e;
+  *launches += 1;
+  if (s.teams == 1) return e;
+  p.peers = p.teams = 1;
+  paged_join_kernel<T, kD, 8 * kNT><<<dim3(row_tiles, p.c.Hkv, p.c.B), kJoinThreads, 0, stream>>>(p, s.teams);
+  *launches += 1;
+  return cudaGetLastError();
 }
 
 template <typename T, int kD, int kBits>
-cudaError_t launch_attend_rows(const AttendParams& p, int64_t keys, cudaStream_t stream) {
-  return p.Hq / p.c.Hkv * p.S <= 8 ? launch_attend<T, kD, 1, kBits>(p, keys, stream) : launch_attend<T, kD, 2, kBits>(p, keys, stream);
+cudaError_t launch_attend_rows(const AttendParams& p, int64_t keys, size_t part_bytes, cudaStream_t stream, int* launches) {
+  return tile_of(p.Hq, p.c.Hkv, p.S) == 8 ? launch_attend<T, kD, 1, kBits>(p, keys, part_bytes, stream, launches)
+                                          : launch_attend<T, kD, 2, kBits>(p, keys, part_bytes, stream, launches);
 }
 
 // calls f with a value of the cache's type, its head dimension and its bits as constants
@@ -1226,12 +1312,18 @@ cudaError_t launch_paged_gather(const GatherParams& p, int dtype, cudaStream_t s
   return e;
 }
 
-cudaError_t launch_paged_attention(const AttendParams& p, int dtype, int64_t keys, cudaStream_t stream, int* launches) {
-  const cudaError_t e = with_cache(p.c, dtype, [&](auto type, auto d, auto bits) {
-    return launch_attend_rows<decltype(type), d, bits>(p, keys, stream);
+cudaError_t launch_paged_attention(const AttendParams& p, int dtype, int64_t keys, size_t part_bytes, cudaStream_t stream, int* launches) {
+  return with_cache(p.c, dtype, [&](auto type, auto d, auto bits) {
+    return launch_attend_rows<decltype(type), d, bits>(p, keys, part_bytes, stream, launches);
   });
-  if (e == cudaSuccess && launches) *launches += 1;
-  return e;
+}
+
+size_t paged_part_bytes(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t S, int64_t D) {
+  return sizeof(float) * units_of(batch, heads_q, heads_kv, S) * tile_of(heads_q, heads_kv, S) * (D + 4);
+}
+
+int paged_teams(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t S, int64_t keys) {
+  return keys < kTeamKeys ? 1 : static_cast<int>(std::min<int64_t>(kMaxTeams, std::max<int64_t>(1, kTeamUnits / units_of(batch, heads_q, heads_kv, S))));
 }
 
 }  // namespace b200fa

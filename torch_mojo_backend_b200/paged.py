@@ -44,7 +44,7 @@ class PagedKVCache:
     elements.  Which pages a sequence has is the caller's: every call takes the ``block_table`` (B, pages of a sequence) and the
     ``lengths`` (B,), int32 mojo tensors that are read on the device (``raw.paged_append`` says how, and what ``new_lengths``
     are).  A call is safe beside others on other streams as long as no two write, or one writes and another reads, the same
-    places; it keeps no workspace.
+    places; it keeps no workspace (a call's own scratch is allocated on the stream it runs on).
     """
 
     def __init__(self, pages: int, kv_heads: int, page_size: int, head_dim: int, *, dtype=torch.bfloat16, bits: int = 16,

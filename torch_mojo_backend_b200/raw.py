@@ -317,16 +317,17 @@ def paged_append(k, v, cache: PagedKV, block_table, lengths, *, new_lengths=None
 
 
 def paged_attention(q, cache: PagedKV, block_table, lengths, *, new_lengths=None, window: int = 0, sinks: int = 0,
-                    scale: float | None = None, out=None, lse=None, longest: int = 0, status=None):
+                    scale: float | None = None, out=None, lse=None, longest: int = 0, workspace=None, status=None):
     """out, lse = causal attention of the newest tokens' ``q`` (B, Hq, S, D) over the pages of their sequences.
 
     ``block_table``, ``lengths`` and ``new_lengths`` as for ``paged_append``, which comes first: the new tokens see each other and
     themselves.  ``window`` > 0: the last ``window`` keys and the first ``sinks`` ones alone.  Rows behind a sequence's new tokens
     are left as they are (out zero and lse -inf in new tensors).  ``longest``: a hint, the longest of the lengths, where the block
-    table is much wider.
+    table is much wider.  ``workspace``: scratch on q's device, for calls of few KV heads (a new tensor by default; one without
+    elements keeps a KV head to one cluster).
     """
     B, Hq, S, D = q.shape
-    c, dtype, _, head_dim, device = _paged(cache, block_table, lengths, new_lengths, B)
+    c, dtype, heads, head_dim, device = _paged(cache, block_table, lengths, new_lengths, B)
     if D != head_dim or q.dtype is not dtype or q.device != device:
         raise ValueError(f"q has to be {dtype} of head dimension {head_dim} on {device}")
     if scale is None:
@@ -340,9 +341,19 @@ def paged_attention(q, cache: PagedKV, block_table, lengths, *, new_lengths=None
     else:
         _fp32_statistic(lse, (B, Hq, S), q.device)
     _same_kind(q, (out,))
+    scratch = scratch_bytes = 0
+    if workspace is None and B * heads <= 64:   # (with more KV heads there is none)
+        keys = longest or block_table.shape[1] * cache.k.shape[2]
+        need = _lib.paged_attention_workspace_bytes(B, Hq, heads, S, D, min(keys, window + sinks + S) if window else keys)
+        if need:
+            workspace = torch.empty((need,), dtype=torch.uint8, device=device)
+    if workspace is not None:
+        if workspace.device != device or not workspace.is_contiguous():
+            raise ValueError(f"workspace has to be contiguous, on {device}")
+        scratch, scratch_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     stream, dev = _stream_and_device(q)
     rc = _lib.paged_attention(c, _t4b(q), _t4b(out), lse.data_ptr(), window, sinks, float(scale), longest, stream, dev,
-                              status.data_ptr() if status is not None else 0)
+                              status.data_ptr() if status is not None else 0, scratch, scratch_bytes)
     if rc != _lib.OK:
         raise _lib.B200FAError(rc, "b200fa_paged_attention")
     return out, lse
