@@ -413,10 +413,14 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
         // warp that rescales its rows of O in tensor memory, once the P V of the previous half-block
         // has completed (P V of this half cannot start before this warp announces P).  The common
         // step has no hand-over to another warp at all.
-        const bool any_moved = __any_sync(0xffffffffu, (m_new - m) * c > kRescaleLog2);   // always on the first half-block (m = -inf)
+        // Under a window the first half-blocks may hide every key of a row, whose O is zero then: it takes its first maximum
+        // without a rescale (else each tile has one where there are no sinks: B2 Hq32 Hkv8 S8192 D128, us with / without,
+        // window 128 177 / 157, 512 240 / 227, 1024 327 / 315).
+        const bool first = kWindow && m == -INFINITY;
+        const bool any_moved = __any_sync(0xffffffffu, !first && (m_new - m) * c > kRescaleLog2);   // without a window: always on the first half-block (m = -inf)
         float sc = 1.f;
-        if (any_moved && m_new > m) {
-          sc = ex2_approx((m - m_new) * c);
+        if ((any_moved || first) && m_new > m) {
+          if (!first) sc = ex2_approx((m - m_new) * c);
           m = m_new;
         }
         const int hb = 2 * j + half;   // half-block index
