@@ -362,20 +362,27 @@ fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUt
         float* sf = reinterpret_cast<float*>(s);
         const int col0 = key_row(j) + half * 64;
         // mask: causal diagonal and/or columns beyond Sk, columns between the sinks and the window
-        const bool need_mask = (kCausal && (col0 + 63 > r0 + p.causal_off)) || (col0 + 64 > p.Sk);
-        const bool need_low = kWindow && col0 <= r0 + kBM - 1 + p.causal_off - p.window && col0 + 63 >= p.sinks;
+        const int first_row = kWindow ? r0 + (row & ~31) : r0;   // of the warp; of the tile
+        const bool need_mask = (kCausal && (col0 + 63 > first_row + p.causal_off)) || (col0 + 64 > p.Sk);
+        // Under a window a warp goes by its own rows, and where all columns lie ahead of all their windows one comparison with the sinks
+        // does (B2 Hq32 Hkv8 S8192 D128, 4 sinks, us by the tile / so: window 128 189 / 183, 1024 347 / 343).  Leaving out the
+        // exponentials of columns that no row of the warp sees costs every other block more: 368.
+        const int low = first_row + p.causal_off - p.window;   // the last column ahead of the window of the warp's first row
+        const bool need_low = kWindow && col0 <= low + 31 && col0 + 63 >= p.sinks;
+        const bool ahead = need_low && col0 + 63 <= low;
         auto load_scores = [&]() {
           tmem_ld32(tSh + 0, s + 0);
           tmem_ld32(tSh + 32, s + 32);
           tmem_wait_ld();
-          if (need_mask) {
-            const int limit = kCausal ? min(q_row + p.causal_off, p.Sk - 1) : (p.Sk - 1);  // last visible column
+          if (need_mask || ahead) {
+            int limit = kCausal ? min(q_row + p.causal_off, p.Sk - 1) : (p.Sk - 1);  // last visible column
+            if (ahead) limit = min(limit, p.sinks - 1);
 #pragma unroll
             for (int i = 0; i < 64; ++i) {
               if (col0 + i > limit) sf[i] = -INFINITY;
             }
           }
-          if (kWindow && need_low) {
+          if (need_low && !ahead) {
             const int before = q_row + p.causal_off - p.window;   // the last column ahead of the row's window
             if (col0 >= p.sinks) {
 #pragma unroll
