@@ -71,7 +71,8 @@ __device__ __forceinline__ float2 exp2_mufu2(float2 x) { return make_float2(ex2_
 // ------------------------------------------------------------------------------------------
 // Under a window a K/V tile with sinks in it is seen by every later query row, all others by those of a window.  Its steps are
 // dealt to sink_chunks blocks, which leave fp32 sums for sink_sum_kernel to add up (bwd_sink_chunks says when).  Tensor-bound:
-// B2 Hq32 Hkv8 S8192 D128 bf16, window 1024, 4 sinks: 545 us, 1010 TFLOP/s of visible pairs, as of the causal mask on that box.
+// B2 Hq32 Hkv8 S8192 D128 bf16, window 1024, 4 sinks: 545 us, 945 TFLOP/s of visible pairs (the causal
+// mask at S4096: 1140).
 template <int kD, bool kBf16, int kMask, bool kDropout>
 __global__ void __launch_bounds__(kDkdvThreads, 1)
 bwd_dkdv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,

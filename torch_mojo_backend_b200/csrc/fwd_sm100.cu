@@ -869,7 +869,7 @@ cudaError_t launch_mask(const CUtensorMap& mq, const CUtensorMap& mk, const CUte
 }
 
 // Under a window two tiles of different heads share all of their blocks, two tiles of one head that lie below each other all but
-// one at each end.  B200, us, below each other / two heads: B2 Hq32 Hkv8 S8192 D128 bf16, window 1024, 4 sinks 379 / 342 (804 TFLOP/s
+// one at each end.  B200, us, below each other / two heads: B2 Hq32 Hkv8 S8192 D128 bf16, window 1024, 4 sinks 379 / 342 (753 TFLOP/s
 // of visible pairs); Hq32 Hkv8 Sq16384 Sk20001 fp16, window 2048 625 / 591; B1 Hq8 Hkv2 S16384, window 512 91.6 / 83.6; a window of
 // as many keys as there are, B1 Hq16 Hkv4 S4096: 77.0 / 75.5.  (Leaving out the half of a block of sinks that holds none costs
 // more than it saves: the first two 344 and 597.)
