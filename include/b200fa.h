@@ -22,7 +22,8 @@
  *     success or a negative B200FA_ERR_* code; no C++ exception crosses this boundary.
  *   - `status_word` (optional, may be NULL) points to a zero-initialised uint32 in device
  *     memory.  A kernel whose internal wait exceeded its budget writes a non-zero code there
- *     and finishes early instead of hanging; the caller reads it after synchronising.
+ *     and finishes early instead of hanging; the caller reads it after synchronising.  A paged cache's index out of range is
+ *     reported there too; it stops no other kernel, and a wait that runs out later takes its place.
  */
 #ifndef B200FA_H_
 #define B200FA_H_
@@ -356,9 +357,9 @@ int b200fa_bwd_parts(const b200fa_tensor4* q, const b200fa_tensor4* k, const b20
  * Bounded waits.  Every wait inside the tensor-core kernels gives up after a budget of SM
  * cycles (default about 2 s; environment variable B200FA_WAIT_BUDGET, or this setter; 0 restores
  * the default), writes 0x5741xxxx (xxxx = where it gave up) to the status word and lets the
- * kernel finish; later thread blocks that see a non-zero status word do no work and write nothing.
- * b200fa_status_to_error maps a status word read back from the device to B200FA_OK or
- * B200FA_ERR_TIMEOUT.  b200fa_selftest_wait_timeout launches a one-warp kernel whose only job
+ * kernel finish; later thread blocks that see that in the status word do no work and write nothing.
+ * b200fa_status_to_error maps a status word read back from the device to B200FA_OK,
+ * B200FA_ERR_TIMEOUT or B200FA_ERR_BAD_INDEX.  b200fa_selftest_wait_timeout launches a one-warp kernel whose only job
  * is to wait `budget_cycles` on a barrier nobody arrives at, so the give-up path can be tested
  * without disturbing an attention kernel.  No counterpart in the reference.
  */

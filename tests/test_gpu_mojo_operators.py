@@ -189,3 +189,50 @@ def test_paged_cache_on_the_device(bits):
     again = cache.attention(turned, *m, new_lengths=m[1], window=20, sinks=1)
     torch.mojo.synchronize()
     assert torch.equal(tmb.to_cuda(again), want)
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float16, 128), (torch.float32, 64)])
+def test_a_bad_index_stops_no_other_call(dtype, D):
+    """The device's status word also stops kernels whose waits have run out: an index out of range of a paged call is not that."""
+    q, k, v, grad = inputs(8, 1, 4, 2, 700, 700, D, dtype)
+    cache = tmb.PagedKVCache(4, 2, 16, 64)
+    cache.kv.k.zero_(), cache.kv.v.zero_()
+    table = torch.arange(4, dtype=torch.int32).view(1, 4).to("mojo")
+    lengths = [torch.tensor([n], dtype=torch.int32).to("mojo") for n in (65, 64)]   # one more than there is room for; all of them
+    query = torch.zeros(1, 2, 1, 64, dtype=torch.bfloat16).to("mojo")
+
+    def calls():
+        got = []
+        for call in (lambda *t: tmb.window_attention(*t, 100, sinks=3, enable_gqa=True),
+                     lambda *t: torch.nn.functional.scaled_dot_product_attention(*t, is_causal=True, enable_gqa=True)):
+            t = leaves(q, k, v)
+            out = call(*t)
+            out.backward(tmb.from_cuda(grad))
+            got += [tmb.to_cuda(x).clone() for x in (out.detach(), *(x.grad for x in t))]
+        return got
+
+    want = calls()
+    torch.mojo.synchronize()
+    assert torch.isnan(tmb.to_cuda(cache.attention(query, table, lengths[0]))).all()
+    got = calls()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert not tmb.to_cuda(cache.attention(query, table, lengths[1])).any()
+    with pytest.raises(_lib.B200FAError) as err:
+        torch.mojo.synchronize()
+    assert err.value.code == _lib.ERR_BAD_INDEX
+    torch.mojo.synchronize()
+
+
+def test_a_wait_that_runs_out_takes_a_bad_indexs_place():
+    status = torch.tensor([0x42490006], dtype=torch.int32, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    assert _lib.selftest_wait_timeout(status.data_ptr(), 1_000_000, stream, 0) == _lib.OK
+    torch.cuda.synchronize()
+    assert _lib.status_to_error(int(status) & 0xFFFFFFFF) == _lib.ERR_TIMEOUT
+    # and an index out of range does not take its
+    pool = raw.PagedKV.empty(1, 1, 16, 64)
+    held = int(status)
+    raw.paged_gather(pool, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.full((1,), 17, dtype=torch.int32, device="cuda"), 3,
+                     status=status)
+    torch.cuda.synchronize()
+    assert int(status) == held

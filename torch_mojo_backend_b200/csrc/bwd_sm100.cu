@@ -163,7 +163,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant_
     return;
   }
   if ((smem_u32(smem) & 1023u) != 0u) {
-    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, kStatusOk, 0x414c0000u);
+    if (threadIdx.x == 0) report_status(p.status, 0x414c0000u);
     cudaGridDependencySynchronize();
     return;
   }
@@ -584,7 +584,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ 
     return;
   }
   if ((smem_u32(smem) & 1023u) != 0u) {
-    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, kStatusOk, 0x414c0001u);
+    if (threadIdx.x == 0) report_status(p.status, 0x414c0001u);
     if (last_block) cudaGridDependencySynchronize();
     return;
   }

@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) fwd_fp32_kernel(const __grid_cons
 
   if (status_is_set(p.status)) return;
   if ((smem_u32(smem) & 1023u) != 0u) {
-    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, kStatusOk, 0x414c0002u);
+    if (threadIdx.x == 0) report_status(p.status, 0x414c0002u);
     return;
   }
   if (threadIdx.x == 0) {
@@ -1341,7 +1341,7 @@ __global__ void __launch_bounds__(kThreads, 1) bwd_dkdv_fp32_kernel(const __grid
     return;
   }
   if ((smem_u32(smem) & 1023u) != 0u) {
-    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, kStatusOk, 0x414c0003u);
+    if (threadIdx.x == 0) report_status(p.status, 0x414c0003u);
     cudaGridDependencySynchronize();
     return;
   }
@@ -1352,7 +1352,7 @@ __global__ void __launch_bounds__(kThreads, 1) bwd_dq_fp32_kernel(const __grid_c
   extern __shared__ __align__(1024) uint8_t smem[];
   if (!status_is_set(p.status)) {
     if ((smem_u32(smem) & 1023u) != 0u) {
-      if (threadIdx.x == 0 && p.status) atomicCAS(p.status, kStatusOk, 0x414c0004u);
+      if (threadIdx.x == 0) report_status(p.status, 0x414c0004u);
     } else {
       dq_block<kD, kDropout>(p, static_cast<int>(blockIdx.x), smem);
     }

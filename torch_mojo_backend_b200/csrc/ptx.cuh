@@ -13,11 +13,19 @@
 namespace b200fa {
 
 // ---------------------------------------------------------------------------------------
-// error codes written to the device status word (first writer wins)
+// What kernels write to the device status word.  The first writer wins, but for this: an index out of range concerns the call that was
+// given it, so kernels run on beside it (status_is_set), and what stops them is written over it (report_status).
 // ---------------------------------------------------------------------------------------
 constexpr uint32_t kStatusOk = 0;
 constexpr uint32_t kStatusWaitTimeout = 0x57410000u;  // | site id in the low 16 bits
 constexpr uint32_t kStatusBadIndex = 0x42490000u;     // | site id: a page, length or position out of range
+
+// Reports what stops kernels: a broken protocol, or shared memory that they cannot use.  (A bad index stays until it is replaced.)
+__device__ __forceinline__ void report_status(uint32_t* status, uint32_t value) {
+  if (status == nullptr) return;
+  const uint32_t old = atomicCAS(status, kStatusOk, value);
+  if ((old & 0xffff0000u) == kStatusBadIndex) atomicCAS(status, old, value);
+}
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -92,7 +100,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
       if (*abort_flag) return false;
       if (clock64() - t0 > budget) {
         *abort_flag = 1u;
-        if (status) atomicCAS(status, kStatusOk, kStatusWaitTimeout | (site & 0xffffu));
+        report_status(status, kStatusWaitTimeout | (site & 0xffffu));
         return false;
       }
     }
@@ -121,9 +129,12 @@ __device__ __forceinline__ void settle_if_aborted(const volatile uint32_t* abort
 
 // True when an earlier CTA of this launch (or an earlier launch sharing the status word) has
 // already reported a failed wait: later CTAs then leave at once instead of each spending its
-// own budget on a protocol that is known to be broken.
+// own budget on a protocol that is known to be broken.  A bad index of a paged call (kStatusBadIndex) stops nobody: its results
+// alone are wrong.
 __device__ __forceinline__ bool status_is_set(const uint32_t* status) {
-  return status != nullptr && *reinterpret_cast<const volatile uint32_t*>(status) != kStatusOk;
+  if (status == nullptr) return false;
+  const uint32_t held = *reinterpret_cast<const volatile uint32_t*>(status);
+  return held != kStatusOk && (held & 0xffff0000u) != kStatusBadIndex;
 }
 
 // ---------------------------------------------------------------------------------------
