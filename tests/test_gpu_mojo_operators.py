@@ -236,3 +236,53 @@ def test_a_wait_that_runs_out_takes_a_bad_indexs_place():
                      status=status)
     torch.cuda.synchronize()
     assert int(status) == held
+
+
+class Held(torch.autograd.Function):
+    """A CPU tensor that stands for `held` on the device: its own gradient is the caller's thread's business."""
+
+    @staticmethod
+    def forward(ctx, x, held):
+        return held.detach()
+
+    @staticmethod
+    def backward(ctx, grad):
+        return torch.zeros(1), None
+
+
+@pytest.mark.parametrize("fails", [True, False])
+def test_a_captured_backward_that_fails_or_ends_on_another_thread(fails):
+    """It leaves the engine's thread on the stream that it found there: backwards behind it are ordered with the default stream."""
+    q, k, v, grad = inputs(9, 1, 4, 4, 1024, 1024, 64, torch.bfloat16)
+    g = tmb.from_cuda(grad)
+
+    def step(call):
+        t = leaves(q, k, v)
+        streams = []
+        t[0].register_hook(lambda _: streams.append(torch.cuda.current_stream()))
+        call(*t).backward(g)
+        return [tmb.to_cuda(x.grad).clone() for x in t], streams
+
+    calls = (lambda *t: tmb.window_attention(*t, 100), lambda *t: torch.nn.functional.scaled_dot_product_attention(*t, is_causal=True))
+    want = [step(call)[0] for call in calls]
+    held = [tmb.from_cuda(t) for t in (q, k, v)]
+    x, called = torch.zeros(1, requires_grad=True), []
+
+    def hook(_):
+        called.append(1)
+        if fails:
+            raise ValueError("on purpose")
+
+    x.register_hook(hook)
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph):
+            tmb.window_attention(Held.apply(x, held[0]), *held[1:], 100).backward(g)
+    except ValueError:
+        assert fails
+    assert called
+    torch.cuda.synchronize()
+    for call, ref in zip(calls[::-1], want[::-1]):
+        got, streams = step(call)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, ref)) and streams == [torch.cuda.default_stream()]

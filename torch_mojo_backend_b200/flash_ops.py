@@ -52,6 +52,8 @@ def _log(msg: str, *values) -> None:
 
 def _stream_for(index: int) -> int:
     """The CUDA stream (as an integer handle) every mojo op on device `index` is ordered on."""
+    if tensor._lent:
+        tensor.take_back_stream()
     return torch._C._cuda_getCurrentRawStream(index)
 
 

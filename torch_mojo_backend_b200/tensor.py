@@ -12,6 +12,7 @@ CUDA stream, and ``_ptr`` is a plain CUDA device address the C ABI consumes dire
 from __future__ import annotations
 
 import math
+import threading
 import weakref
 
 import torch
@@ -89,8 +90,48 @@ def pinned_empty(shape, dtype: torch.dtype) -> torch.Tensor:
     return t
 
 
+#: Threads whose current stream a captured backward pass has changed for its own duration (`lend_stream`): thread -> (the stream that
+#: was its own, the captured one, a weak reference to what lives as long as the pass).
+_lent: dict[int, tuple] = {}
+
+
+class _Pass:
+    """Called at the end of a backward pass that gets there; gone with every pass."""
+
+    def __init__(self) -> None:
+        self.thread = threading.get_ident()
+
+    def __call__(self) -> None:
+        if threading.get_ident() == self.thread:
+            take_back_stream(over=True)
+
+
+def lend_stream(stream) -> None:
+    """Makes `stream` the current one of this thread, which runs a node of a backward pass, until the pass is over."""
+    own, running = torch.cuda.current_stream(stream.device), _Pass()
+    # (the engine drops its callbacks with the pass, and calls them only if it succeeds, from the thread that it ends on)
+    torch.autograd.Variable._execution_engine.queue_callback(running)
+    _lent[running.thread] = own, stream, weakref.ref(running)
+    torch.cuda.set_stream(stream)
+
+
+def take_back_stream(over: bool = False) -> None:
+    """Gives this thread its own stream back if the pass that changed it is over, however it ended.  Everything of this package that
+    allocates on, copies on or launches on a thread's current stream asks first."""
+    held = _lent.get(threading.get_ident())
+    if held is None:
+        return
+    own, stream, running = held
+    if over or running() is None:
+        del _lent[threading.get_ident()]
+        if torch.cuda.current_stream(own.device) == stream:
+            torch.cuda.set_stream(own)
+
+
 def _alloc_holder(nbytes: int, index: int) -> torch.Tensor:
     """One device allocation: a flat byte buffer on CUDA device `index` (never zero bytes)."""
+    if _lent:
+        take_back_stream()
     return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=_cuda_device(index))
 
 
@@ -195,6 +236,8 @@ class TorchMojoTensor(torch.Tensor):
     # ------------------------------------------------------------------ payload access
     def _cuda_view(self) -> torch.Tensor:
         """The same memory as a plain CUDA tensor (for copies and DLPack export)."""
+        if _lent:
+            take_back_stream()
         holder = self._holder
         if holder.dtype == torch.uint8 and holder.dim() == 1:
             nbytes = holder.numel()

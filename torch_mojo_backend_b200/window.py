@@ -11,7 +11,6 @@ from __future__ import annotations
 
 import contextlib
 import math
-import threading
 
 import torch
 
@@ -65,27 +64,29 @@ def _backward(dout, q, k, v, out, lse, window, sinks, causal, scale):
 
 @contextlib.contextmanager
 def _on_stream(stream):
-    """A backward on the forward's stream.  What else the engine has to do for it (sums of a tensor's gradients, gradients of
-    views) goes to the current stream of the engine's thread: the two wait for one another, and in the end the forward's, where the
-    caller goes on, for the other.  A stream that is being captured cannot wait for one that is not: it becomes the thread's current one
-    until the engine is done."""
+    """A backward on the forward's stream (None: no CUDA memory, no stream).  What else the engine has to do for it (sums of a tensor's
+    gradients, gradients of views) goes to the current stream of the engine's thread: the two wait for one another, and in the end the
+    forward's, where the caller goes on, for the other.  A stream that is being captured cannot wait for one that is not: it becomes the
+    thread's current one until the pass is over."""
+    if stream is None:
+        yield
+        return
+    tensor.take_back_stream()
     current = torch.cuda.current_stream(stream.device)
     if current == stream:
         yield
         return
-    at_the_end = torch.autograd.Variable._execution_engine.queue_callback
+    lend = not torch.cuda.is_current_stream_capturing()
     with torch.cuda.stream(stream):
-        captured = torch.cuda.is_current_stream_capturing()
-        if not captured:
+        lend = lend and torch.cuda.is_current_stream_capturing()
+        if not lend:
             stream.wait_stream(current)
         yield
-    if captured:
-        torch.cuda.set_stream(stream)
-        thread = threading.get_ident()
-        at_the_end(lambda: torch.cuda.set_stream(current) if threading.get_ident() == thread else None)
+    if lend:
+        tensor.lend_stream(stream)
     else:
         current.wait_stream(stream)
-        at_the_end(lambda: stream.wait_stream(current))
+        torch.autograd.Variable._execution_engine.queue_callback(lambda: stream.wait_stream(current))
 
 
 class _WindowAttention(torch.autograd.Function):
