@@ -258,6 +258,10 @@ int b200fa_paged_attention(const b200fa_paged_kv* cache, const b200fa_tensor4* q
                            size_t workspace_bytes, void* stream, int device, uint32_t* status_word);
 size_t b200fa_paged_attention_workspace_bytes(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t seqlen_q,
                                               int64_t head_dim, int64_t longest);
+/* How a call's keys are shared on `device`: a KV head's (for 16 rows of its group) by `teams` clusters of `peers` blocks of `warps`. */
+int b200fa_paged_attention_shares(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t seqlen_q, int64_t head_dim, int dtype,
+                                  int bits, int64_t longest, size_t workspace_bytes, int device, int* peers, int* teams,
+                                  int* warps);
 
 /*
  * The first S tokens of every sequence as dense k and v (batch, heads, S, head_dim) of `dtype`, rows behind a sequence's

@@ -495,3 +495,24 @@ def test_pages_beyond_32_bits():
     s = torch.softmax(q.double() @ x.double().mT * D ** -0.5, -1)
     a = s @ x.double().abs()
     assert ((out.double() - s @ x.double()).abs() <= 2 ** -8 * (a + 2 * out.double().abs()) + 2 ** -12 * a).all()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_clusters_of_every_size_without_a_workspace(bits):
+    """A KV head has up to 16 blocks, by the calls' model, with a workspace or without; each size that it takes is right."""
+    calls = {}
+    for keys in [*range(64, 8192, 64), 16384, 32768, 65536]:
+        peers, teams, warps = _lib.paged_attention_shares(1, 4, 1, 1, 128, _lib.BF16, bits, keys)
+        assert teams == 1
+        calls.setdefault((peers, warps), keys)
+    assert {8, 16} <= {peers for peers, _ in calls} and max(calls)[0] == 16
+    need = _lib.paged_attention_workspace_bytes(1, 4, 1, 1, 128, 131072)
+    assert _lib.paged_attention_shares(1, 4, 1, 1, 128, _lib.BF16, bits, 131072, need)[1] > 1
+    none = torch.empty(0, dtype=torch.uint8, device="cuda")
+    for keys in calls.values():
+        pool = Pool(12, [keys], 1, 128, 64, torch.bfloat16, bits)
+        q = pool.draw(1, 4, 1, 128)
+        out, lse = raw.paged_attention(q, pool.cache, pool.table, pool.lengths, longest=keys, workspace=none)
+        (o, ob), (l, lb) = expected(pool, q[0], 0, 1, 0, 0)
+        check("out", out[0], o, ob)
+        check("lse", lse[0], l, lb)

@@ -204,3 +204,13 @@ def test_a_paged_cache_refuses_what_the_kernels_do_not_serve(mojo_registered):
         with pytest.raises((NotImplementedError, RuntimeError)) as err:
             mojo_registered.PagedKVCache(**{**args, **how})
         assert err.type is NotImplementedError
+
+
+def test_the_shares_of_a_paged_call_are_refused_before_a_device_is_asked():
+    good = dict(B=2, Hq=8, Hkv=2, S=1, D=128, dtype=_lib.BF16, bits=16, longest=1000)
+    for how, code in ((dict(B=0), _lib.ERR_BAD_SHAPE), (dict(Hq=7), _lib.ERR_BAD_SHAPE), (dict(Hkv=0), _lib.ERR_BAD_SHAPE), (dict(S=0), _lib.ERR_BAD_SHAPE),
+                      (dict(longest=0), _lib.ERR_BAD_SHAPE), (dict(longest=1 << 25), _lib.ERR_BAD_SHAPE), (dict(S=1 << 40), _lib.ERR_BAD_SHAPE),
+                      (dict(D=96), _lib.ERR_UNSUPPORTED), (dict(bits=8), _lib.ERR_UNSUPPORTED), (dict(dtype=_lib.F32), _lib.ERR_BAD_DTYPE)):
+        with pytest.raises(_lib.B200FAError) as err:
+            _lib.paged_attention_shares(**{**good, **how})
+        assert err.value.code == code

@@ -60,6 +60,7 @@ EXPORTED_SYMBOLS = (
     "b200fa_paged_append",
     "b200fa_paged_attention",
     "b200fa_paged_attention_workspace_bytes",
+    "b200fa_paged_attention_shares",
     "b200fa_paged_gather",
     "b200fa_set_wait_budget",
     "b200fa_wait_budget",
@@ -178,6 +179,9 @@ def load() -> ctypes.CDLL:
     lib.b200fa_paged_attention.restype = ctypes.c_int
     lib.b200fa_paged_attention_workspace_bytes.argtypes = [ctypes.c_int64] * 6
     lib.b200fa_paged_attention_workspace_bytes.restype = ctypes.c_size_t
+    lib.b200fa_paged_attention_shares.argtypes = ([ctypes.c_int64] * 5 + [ctypes.c_int] * 2 + [ctypes.c_int64, ctypes.c_size_t, ctypes.c_int]
+                                                  + [ctypes.POINTER(ctypes.c_int)] * 3)
+    lib.b200fa_paged_attention_shares.restype = ctypes.c_int
     lib.b200fa_paged_gather.argtypes = [packed, packed, packed, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
     lib.b200fa_paged_gather.restype = ctypes.c_int
     lib.b200fa_dropout_threshold.argtypes = [ctypes.c_float]
@@ -324,6 +328,16 @@ def paged_attention(cache: bytes, q: bytes, out: bytes, lse_ptr: int, window: in
 @functools.lru_cache(maxsize=1024)   # (of sizes alone)
 def paged_attention_workspace_bytes(B: int, Hq: int, Hkv: int, S: int, D: int, longest: int) -> int:
     return int(load().b200fa_paged_attention_workspace_bytes(B, Hq, Hkv, S, D, longest))
+
+
+def paged_attention_shares(B: int, Hq: int, Hkv: int, S: int, D: int, dtype: int, bits: int, longest: int, workspace_bytes: int = 0,
+                           device: int = 0) -> tuple[int, int, int]:
+    """(blocks of a cluster, clusters, warps of a block) that share the keys of a KV head (see b200fa_paged_attention_shares)."""
+    got = [ctypes.c_int() for _ in range(3)]
+    rc = load().b200fa_paged_attention_shares(B, Hq, Hkv, S, D, dtype, bits, longest, workspace_bytes, device, *map(ctypes.byref, got))
+    if rc != OK:
+        raise B200FAError(rc, "b200fa_paged_attention_shares")
+    return tuple(n.value for n in got)
 
 
 def paged_gather(cache: bytes, k: bytes, v: bytes, stream: int, device: int, status_ptr: int = 0) -> int:

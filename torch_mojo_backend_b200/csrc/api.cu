@@ -812,6 +812,22 @@ int b200fa_paged_attention(const b200fa_paged_kv* cache, const b200fa_tensor4* q
                 [&](int* n) { return launch_paged_attention(p, dtype, keys, workspace_bytes, static_cast<cudaStream_t>(stream), n); });
 }
 
+int b200fa_paged_attention_shares(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t seqlen_q, int64_t head_dim, int dtype,
+                                  int bits, int64_t longest, size_t workspace_bytes, int device, int* peers, int* teams,
+                                  int* warps) {
+  if (!peers || !teams || !warps) return B200FA_ERR_NULL;
+  if (dtype != kBF16 && dtype != kF16) return B200FA_ERR_BAD_DTYPE;
+  if ((bits != 16 && bits != 4) || (head_dim != 64 && head_dim != 128)) return B200FA_ERR_UNSUPPORTED;
+  if (batch <= 0 || batch > 65535 || heads_kv <= 0 || heads_q <= 0 || heads_q > 65535 || heads_q % heads_kv != 0 || seqlen_q <= 0 ||
+      seqlen_q > (1 << 24) || heads_q * seqlen_q > INT_MAX / 16 || longest <= 0 || longest > (1 << 24)) return B200FA_ERR_BAD_SHAPE;
+  AttendParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.c.B = static_cast<int>(batch); p.c.Hkv = static_cast<int>(heads_kv); p.c.D = static_cast<int>(head_dim); p.c.bits = bits;
+  p.Hq = static_cast<int>(heads_q); p.S = static_cast<int>(seqlen_q);
+  return run_on(device, "b200fa_paged_attention_shares",
+                [&](int*) { return paged_shares(p, dtype, longest, workspace_bytes, peers, teams, warps); });
+}
+
 int b200fa_selftest_wait_timeout(uint32_t* status_word, long long budget_cycles, void* stream, int device) {
   if (!status_word) return B200FA_ERR_NULL;
   if (budget_cycles <= 0 || budget_cycles > kWaitBudgetCycles) return B200FA_ERR_UNSUPPORTED;

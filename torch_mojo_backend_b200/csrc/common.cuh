@@ -168,6 +168,8 @@ cudaError_t launch_paged_append(const AppendParams& p, int dtype, cudaStream_t s
 cudaError_t launch_paged_gather(const GatherParams& p, int dtype, cudaStream_t stream, int* launches);
 // `keys`: the most that a query row can see, as far as the host knows; `part_bytes` at p.parts
 cudaError_t launch_paged_attention(const AttendParams& p, int dtype, int64_t keys, size_t part_bytes, cudaStream_t stream, int* launches);
+// How such a call's keys are shared on the current device: blocks of a cluster, clusters of a unit, warps of a block (p: c, Hq, S)
+cudaError_t paged_shares(const AttendParams& p, int dtype, int64_t keys, size_t part_bytes, int* peers, int* teams, int* warps);
 // Bytes of a team's part, and how many teams (clusters that share a unit) are worth a workspace for a call that sees `keys` keys
 size_t paged_part_bytes(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t S, int64_t D);
 int paged_teams(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t S, int64_t keys);

@@ -1135,11 +1135,11 @@ int64_t units_of(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t S) {
   return batch * heads_kv * ((heads_q / heads_kv * S + tile - 1) / tile);
 }
 
-// Several clusters share a unit where there are few units and many keys: one cluster has 16 SMs.  B200, us, one token, D = 128, one
-// cluster at most / teams: B1 Hq8 Hkv1, 16384 keys 20.5 / 18.4, 65536 47.1 / 26.6, 131072 82 / 31; B1 Hq32 Hkv4, 131072 82 / 70; B2 Hq32 Hkv8,
-// 131072 221 / 188, with 4 bits 160 / 108; 8192 keys and fewer never gain.  The join (a kernel of its own) is entered dearer than it is,
-// 6 us for about 3: where that decides, the model is no better than its 5 % (B3 Hq32 Hkv8, 32768 keys, 4 bits 53 / 59; B7 Hkv1,
-// 131072, 16 bits 100 / 110 are the worst of 30).
+// Several clusters share a unit where there are few units and many keys: one cluster has 16 SMs.  B200, us of the kernels, caches cold, one
+// token, D = 128, one cluster (no workspace) / teams: B1 Hq8 Hkv1, 16384 keys 15.4 / 11.8, 65536 40.5 / 20.2, 131072 73 / 23; B1 Hq32 Hkv4,
+// 131072 73 / 51; B2 Hq32 Hkv8, 131072 196 / 160, with 4 bits 143 / 100; 8192 keys and fewer never gain.  The join (a kernel of its own) is
+// entered dearer than it is, 6 us for about 3: where that decides, the model is no better than its 5 % (B7 Hkv1, 131072 keys, 16 bits 77 /
+// 86; B1 Hq8 Hkv8 D64, 23508 keys, 16 bits 16.7 / 17.4: the two that lose among 48).
 constexpr int64_t kTeamKeys = 8192, kTeamUnits = 128;
 constexpr double kJoinCost = 6.0;   // us
 
@@ -1232,20 +1232,29 @@ cudaError_t clusters_that_fit(const int** fits) {
   return result[dev];
 }
 
+// How a call's keys are shared, with `part_bytes` of workspace; 0 bytes are one cluster's share too.
+template <typename T, int kD, int kNT, int kBits>
+cudaError_t shares_of(const AttendParams& p, int64_t keys, size_t part_bytes, Shares* s) {
+  const int *fits = nullptr, *fits_wide = nullptr;
+  cudaError_t e = clusters_that_fit<T, kD, kNT, kBits, 4>(&fits);
+  if (e == cudaSuccess) e = clusters_that_fit<T, kD, kNT, kBits, AttendCfg<kD, kNT, kBits>::kWide>(&fits_wide);
+  if (e != cudaSuccess) return e;
+  const int64_t room = part_bytes / paged_part_bytes(p.c.B, p.Hq, p.c.Hkv, p.S, kD);
+  const int max_teams = std::max<int64_t>(1, std::min<int64_t>(room, paged_teams(p.c.B, p.Hq, p.c.Hkv, p.S, keys)));
+  *s = choose_shares(units_of(p.c.B, p.Hq, p.c.Hkv, p.S), keys, kD, kBits, kNT, max_teams, fits, fits_wide);
+  return e;
+}
+
 template <typename T, int kD, int kNT, int kBits>
 cudaError_t launch_attend(AttendParams p, int64_t keys, size_t part_bytes, cudaStream_t stream, int* launches) {
   constexpr int kWide = AttendCfg<kD, kNT, kBits>::kWide;
-  const int *fits = nullptr, *fits_wide = nullptr;
-  cudaError_t e = clusters_that_fit<T, kD, kNT, kBits, 4>(&fits);
-  if (e == cudaSuccess) e = clusters_that_fit<T, kD, kNT, kBits, kWide>(&fits_wide);
+  Shares s;
+  cudaError_t e = shares_of<T, kD, kNT, kBits>(p, keys, part_bytes, &s);
   if (e != cudaSuccess) return e;
   p.group = p.Hq / p.c.Hkv;
   const int row_tiles = (p.group * p.S + 8 * kNT - 1) / (8 * kNT);
   p.one_f16 = kOneF16;
   p.one_bf16 = kOneBf16;
-  const int64_t units = static_cast<int64_t>(p.c.B) * p.c.Hkv * row_tiles;
-  const int max_teams = std::min<int64_t>(part_bytes / paged_part_bytes(p.c.B, p.Hq, p.c.Hkv, p.S, kD), paged_teams(p.c.B, p.Hq, p.c.Hkv, p.S, keys));
-  const Shares s = choose_shares(units, keys, kD, kBits, kNT, max_teams, fits, fits_wide);
   p.peers = s.peers;
   p.teams = s.teams;
   const dim3 grid(s.peers * s.teams * row_tiles, p.c.Hkv, p.c.B);
@@ -1315,6 +1324,20 @@ cudaError_t launch_paged_gather(const GatherParams& p, int dtype, cudaStream_t s
 cudaError_t launch_paged_attention(const AttendParams& p, int dtype, int64_t keys, size_t part_bytes, cudaStream_t stream, int* launches) {
   return with_cache(p.c, dtype, [&](auto type, auto d, auto bits) {
     return launch_attend_rows<decltype(type), d, bits>(p, keys, part_bytes, stream, launches);
+  });
+}
+
+cudaError_t paged_shares(const AttendParams& p, int dtype, int64_t keys, size_t part_bytes, int* peers, int* teams, int* warps) {
+  return with_cache(p.c, dtype, [&](auto type, auto d, auto bits) {
+    using T = decltype(type);
+    Shares s;
+    const bool one_tile = tile_of(p.Hq, p.c.Hkv, p.S) == 8;
+    const cudaError_t e = one_tile ? shares_of<T, d, 1, bits>(p, keys, part_bytes, &s) : shares_of<T, d, 2, bits>(p, keys, part_bytes, &s);
+    if (e != cudaSuccess) return e;
+    *peers = s.peers;
+    *teams = s.teams;
+    *warps = !s.wide ? 4 : one_tile ? AttendCfg<d, 1, bits>::kWide : AttendCfg<d, 2, bits>::kWide;
+    return e;
   });
 }
 
