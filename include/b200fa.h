@@ -231,8 +231,11 @@ typedef struct b200fa_paged_kv {
  * multiple of 16 (0: none, q NULL), in pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if `interleaved`; cos, sin:
  * (positions, rotary_dim / 2) fp32, 16-byte aligned.  (a, b) becomes (a c - b s, b c + a s), every operation rounded to fp32,
  * then to `dtype`.  4 bits: scale = (max - min) / 15 rounded to `dtype`, code = round((x - min) / scale); a group with an
- * element that is not finite reads NaN.  Rows of q_out behind a sequence's new tokens are left as they are.
+ * element that is not finite reads NaN.  Rows of q_out behind a sequence's new tokens, and those of tokens that are not there, are left
+ * as they are, also where an index is out of range; with B200FA_APPEND_CLEAR or'ed to `interleaved` they become zero, and NaN where a
+ * length or a position is out of range (for a q_out that holds nothing yet).
  */
+#define B200FA_APPEND_CLEAR 0x100
 int b200fa_paged_append(const b200fa_paged_kv* cache, const b200fa_tensor4* k, const b200fa_tensor4* v,
                         const b200fa_tensor4* q, const b200fa_tensor4* q_out, const float* cos, const float* sin,
                         int64_t rotary_dim, int64_t positions, int interleaved, void* stream, int device,

@@ -516,3 +516,35 @@ def test_clusters_of_every_size_without_a_workspace(bits):
         (o, ob), (l, lb) = expected(pool, q[0], 0, 1, 0, 0)
         check("out", out[0], o, ob)
         check("lse", lse[0], l, lb)
+
+
+@pytest.mark.parametrize("D,Hq", [(64, 3), (128, 8)])
+@pytest.mark.parametrize("padded", [True, False])
+def test_a_new_tensor_of_queries_is_whole(padded, D, Hq):
+    """Rows that no new token has are zero in the tensor that the call makes, and NaN where an index is out of range."""
+    lengths = [2, 0, 30, 40, 999, 20]        # fewer tokens than S; an idle place; all there; behind the angles; no such length
+    S, new = 5, [4, 0, 5, 5, 5, 2]
+    pool = Pool(13, [2, 0, 30, 40, 45, 20], 2, D, 16, torch.bfloat16, 16)
+    pool.lengths.copy_(torch.tensor(lengths))
+    q, k, v = pool.draw(6, Hq, S, D), pool.draw(6, 2, S, D), pool.draw(6, 2, S, D)
+    angle = torch.rand(38, D // 2, device="cuda")
+    rotary = angle.cos(), angle.sin()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    n = torch.tensor(new, dtype=torch.int32, device="cuda") if padded else None
+    held = torch.full_like(q, 3.0)
+    raw.paged_append(k, v, pool.cache, pool.table, pool.lengths, new_lengths=n, rotary=rotary, q=q, q_out=held)
+    torch.full_like(q, 7.0)                  # (what its memory held)
+    out = raw.paged_append(k, v, pool.cache, pool.table, pool.lengths, new_lengths=n, rotary=rotary, q=q, status=status)
+    assert _lib.status_to_error(int(status)) == _lib.ERR_BAD_INDEX
+    for b in range(6):
+        t = new[b] if padded else S
+        for s in range(S):
+            pos = lengths[b] - t + s
+            row, given = out[b, :, s], held[b, :, s]
+            if b == 4 or (s < t and pos >= 38):
+                assert torch.isnan(row).all() and (given == 3.0).all()
+            elif s >= t or pos < 0:
+                assert (row == 0).all() and (given == 3.0).all()
+            else:
+                want = rotated(q[b, :, s], rotary[0][pos], rotary[1][pos], False)
+                assert torch.equal(row, want) and torch.equal(given, want)

@@ -33,6 +33,7 @@ ERR_CUDA = -7
 ERR_NULL = -8
 ERR_TIMEOUT = -9
 ERR_BAD_INDEX = -10
+APPEND_CLEAR = 0x100
 
 #: every symbol include/b200fa.h declares; the CPU test-suite checks the library exports them
 EXPORTED_SYMBOLS = (
@@ -311,11 +312,12 @@ def window_bwd(q: bytes, k: bytes, v: bytes, out: bytes, dout: bytes, lse_ptr: i
 
 
 def paged_append(cache: bytes, k: bytes, v: bytes, q: bytes | None, q_out: bytes | None, cos_ptr: int, sin_ptr: int,
-                 rotary_dim: int, positions: int, interleaved: bool, stream: int, device: int, status_ptr: int = 0) -> int:
-    """Raw append to a paged cache (see b200fa_paged_append), descriptors as `pack_paged_kv` and `pack_tensor4` make them; returns
-    the library's status code."""
-    return load().b200fa_paged_append(cache, k, v, q, q_out, cos_ptr, sin_ptr, rotary_dim, positions, 1 if interleaved else 0, stream,
-                                      device, status_ptr)
+                 rotary_dim: int, positions: int, interleaved: bool, stream: int, device: int, status_ptr: int = 0,
+                 clear: bool = False) -> int:
+    """Raw append to a paged cache (see b200fa_paged_append), descriptors as `pack_paged_kv` and `pack_tensor4` make them; `clear`:
+    with B200FA_APPEND_CLEAR; returns the library's status code."""
+    flags = (1 if interleaved else 0) | (APPEND_CLEAR if clear else 0)
+    return load().b200fa_paged_append(cache, k, v, q, q_out, cos_ptr, sin_ptr, rotary_dim, positions, flags, stream, device, status_ptr)
 
 
 def paged_attention(cache: bytes, q: bytes, out: bytes, lse_ptr: int, window: int, sinks: int, scale: float, longest: int,

@@ -750,7 +750,8 @@ int b200fa_paged_append(const b200fa_paged_kv* cache, const b200fa_tensor4* k, c
   }
   p.cos = cos; p.sin = sin;
   p.Hq = static_cast<int>(Hq); p.S = static_cast<int>(S);
-  p.rotary = static_cast<int>(rotary_dim); p.positions = static_cast<int>(positions); p.interleaved = interleaved != 0;
+  p.rotary = static_cast<int>(rotary_dim); p.positions = static_cast<int>(positions); p.interleaved = (interleaved & ~B200FA_APPEND_CLEAR) != 0;
+  p.clear = (interleaved & B200FA_APPEND_CLEAR) != 0;
   return run_on(device, "b200fa_paged_append",
                 [&](int* n) { return launch_paged_append(p, dtype, static_cast<cudaStream_t>(stream), n); });
 }

@@ -117,6 +117,7 @@ struct AppendParams {
   View4 q, k, v, q_out;         // (B, H, S, D); q and q_out only if Hq > 0
   const float *cos, *sin;       // (positions, rotary / 2)
   int Hq, S, rotary, positions, interleaved;
+  int clear;                    // rows of q_out that no new token has become zero, or NaN by a bad index
 };
 struct GatherParams {
   PagedCache c;

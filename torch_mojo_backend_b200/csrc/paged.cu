@@ -107,14 +107,23 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const AppendParams p)
   Sequence seq;
   const bool good = sequence_of(p.c, b, p.S, &seq);
   const int pos = seq.len - seq.n + s;
+  T* const q_row = reinterpret_cast<T*>(p.q_out.ptr) + static_cast<int64_t>(b) * p.q_out.sb + static_cast<int64_t>(h0) * p.q_out.sh +
+                   static_cast<int64_t>(s) * p.q_out.ss + li * 8;   // (if what == 0)
+  auto clear = [&](uint32_t word) {   // the rows of queries that are not turned
+    if (!p.clear || what != 0) return;
+#pragma unroll
+    for (int u = 0; u < Cfg::kRows; ++u)
+      if (h0 + u * Cfg::kSide < heads) *reinterpret_cast<uint4*>(q_row + u * Cfg::kSide * p.q_out.sh) = make_uint4(word, word, word, word);
+  };
+  constexpr uint32_t kNaN2 = 0x7fff7fffu;   // in either type
   if (!good) {
     if (lane == 0) report_bad_index(p.c.status, 1);
-    return;
+    return clear(kNaN2);
   }
-  if (s >= seq.n || pos < 0) return;
+  if (s >= seq.n || pos < 0) return clear(0);
   if (p.rotary != 0 && pos >= p.positions) {
     if (lane == 0) report_bad_index(p.c.status, 2);
-    return;
+    return clear(kNaN2);
   }
   uint32_t row0 = 0;   // of head h0 in the pages
   if (what != 0) {
@@ -175,9 +184,7 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const AppendParams p)
       }
     }
     if (what == 0) {
-      if (write)
-        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.q_out.ptr) + static_cast<int64_t>(b) * p.q_out.sb + static_cast<int64_t>(h0 + u * Cfg::kSide) * p.q_out.sh +
-                                  static_cast<int64_t>(s) * p.q_out.ss + li * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (write) *reinterpret_cast<uint4*>(q_row + u * Cfg::kSide * p.q_out.sh) = make_uint4(w[0], w[1], w[2], w[3]);
       continue;
     }
     const uint64_t at = row0 + (static_cast<uint32_t>(u * Cfg::kSide) << p.c.shift);   // the row in the pages

@@ -288,8 +288,9 @@ def paged_append(k, v, cache: PagedKV, block_table, lengths, *, new_lengths=None
     ``new_lengths``: (B,) int32, how many of the S tokens are new ones (the first of each row; None: all).  Token s is written at
     position ``length - new + s``.  ``rotary``: (cos, sin), float32 (positions, R / 2): the first R elements turn, in pairs
     (i, i + R / 2) or, ``interleaved``, (2 i, 2 i + 1).  ``q``: (B, Hq, S, D), rotated the same way to ``q_out`` (a new tensor by
-    default; q itself will do), whose rows behind a sequence's new tokens are left as they are (zero in a new tensor).  ``status``: an
-    int32 tensor of one element, zero, that reports a page, length or position out of range (include/b200fa.h).
+    default; q itself will do), whose rows behind a sequence's new tokens, or of tokens before position 0, are left as they are (in a new
+    tensor zero, and NaN where a length or position is out of range).  ``status``: an int32 tensor of one element, zero, that reports a
+    page, length or position out of range (include/b200fa.h).
     """
     B, Hkv, S, D = k.shape
     c, dtype, heads, head_dim, device = _paged(cache, block_table, lengths, new_lengths, B)
@@ -305,12 +306,12 @@ def paged_append(k, v, cache: PagedKV, block_table, lengths, *, new_lengths=None
         cos_ptr, sin_ptr, positions, rotary_dim = cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1]
     if q is None and q_out is not None:
         raise ValueError("q_out without q")
-    if q is not None and q_out is None:
-        make = torch.empty if new_lengths is None else torch.zeros
-        q_out = make(tuple(q.shape), dtype=q.dtype, device=q.device)
+    clear = q is not None and q_out is None
+    if clear:
+        q_out = torch.empty(tuple(q.shape), dtype=q.dtype, device=q.device)
     stream, dev = _stream_and_device(k)
     rc = _lib.paged_append(c, _t4b(k), _t4b(v), _t4b(q) if q is not None else None, _t4b(q_out) if q is not None else None, cos_ptr, sin_ptr,
-                           rotary_dim, positions, interleaved, stream, dev, status.data_ptr() if status is not None else 0)
+                           rotary_dim, positions, interleaved, stream, dev, status.data_ptr() if status is not None else 0, clear)
     if rc != _lib.OK:
         raise _lib.B200FAError(rc, "b200fa_paged_append")
     return q_out
