@@ -259,6 +259,7 @@ int b200fa_paged_append(const b200fa_paged_kv* cache, const b200fa_tensor4* k, c
 int b200fa_paged_attention(const b200fa_paged_kv* cache, const b200fa_tensor4* q, const b200fa_tensor4* out, float* lse,
                            int64_t window, int64_t sinks, float scale, int64_t longest, void* workspace,
                            size_t workspace_bytes, void* stream, int device, uint32_t* status_word);
+#define B200FA_PAGED_TEAM_KEYS 8192   /* calls that see fewer keys want no workspace */
 size_t b200fa_paged_attention_workspace_bytes(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t seqlen_q,
                                               int64_t head_dim, int64_t longest);
 /* How a call's keys are shared on `device`: a KV head's (for 16 rows of its group) by `teams` clusters of `peers` blocks of `warps`. */

@@ -214,3 +214,28 @@ def test_the_shares_of_a_paged_call_are_refused_before_a_device_is_asked():
         with pytest.raises(_lib.B200FAError) as err:
             _lib.paged_attention_shares(**{**good, **how})
         assert err.value.code == code
+
+
+def test_calls_of_few_keys_do_not_ask_for_a_workspace(monkeypatch):
+    """The query costs a short call a tenth of its time on the host: tables of fewer keys than any workspace is for go without it."""
+    header = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "b200fa.h")).read()
+    for name, value in (("PAGED_TEAM_KEYS", _lib.PAGED_TEAM_KEYS), ("APPEND_CLEAR", _lib.APPEND_CLEAR)):
+        assert int(re.search(rf"#define B200FA_{name} (\w+)", header).group(1), 0) == value
+    need = _lib.paged_attention_workspace_bytes
+    assert need(1, 8, 1, 1, 128, _lib.PAGED_TEAM_KEYS - 1) == 0 < need(1, 8, 1, 1, 128, _lib.PAGED_TEAM_KEYS)
+    asked = []
+    monkeypatch.setattr(_lib, "paged_attention_workspace_bytes", lambda *a: asked.append(a) or 0)
+    monkeypatch.setattr(_lib, "paged_attention", lambda *a: _lib.OK)
+    monkeypatch.setattr(raw, "_stream_and_device", lambda t: (0, 0))
+    q = torch.zeros(2, 4, 3, 64, dtype=torch.bfloat16)
+
+    def call(width, **how):
+        monkeypatch.setattr(raw, "_paged", lambda *a: (b"", q.dtype, 2, 64, q.device, 16 * width))
+        raw.paged_attention(q, None, None, None, **how)
+        got = asked[:]
+        asked.clear()
+        return got
+
+    assert call(511) == [] == call(511, longest=100) == call(511, window=20)
+    assert call(512) == [(2, 4, 2, 3, 64, 8192)] and call(600, longest=9000) == [(2, 4, 2, 3, 64, 9000)]
+    assert call(600, longest=10000) == [(2, 4, 2, 3, 64, 9600)] and call(600, window=8200, sinks=4) == [(2, 4, 2, 3, 64, 8207)]

@@ -34,6 +34,7 @@ ERR_NULL = -8
 ERR_TIMEOUT = -9
 ERR_BAD_INDEX = -10
 APPEND_CLEAR = 0x100
+PAGED_TEAM_KEYS = 8192
 
 #: every symbol include/b200fa.h declares; the CPU test-suite checks the library exports them
 EXPORTED_SYMBOLS = (

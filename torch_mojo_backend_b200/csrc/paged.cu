@@ -18,6 +18,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "../../include/b200fa.h"
 #include "common.cuh"
 #include "ptx.cuh"
 
@@ -1147,7 +1148,7 @@ int64_t units_of(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t S) {
 // 131072 73 / 51; B2 Hq32 Hkv8, 131072 196 / 160, with 4 bits 143 / 100; 8192 keys and fewer never gain.  The join (a kernel of its own) is
 // entered dearer than it is, 6 us for about 3: where that decides, the model is no better than its 5 % (B7 Hkv1, 131072 keys, 16 bits 77 /
 // 86; B1 Hq8 Hkv8 D64, 23508 keys, 16 bits 16.7 / 17.4: the two that lose among 48).
-constexpr int64_t kTeamKeys = 8192, kTeamUnits = 128;
+constexpr int64_t kTeamKeys = B200FA_PAGED_TEAM_KEYS, kTeamUnits = 128;
 constexpr double kJoinCost = 6.0;   // us
 
 // How a unit's keys are shared: `teams` clusters of `peers` blocks, of four warps each or, `wide`, of as many as an SM takes.
@@ -1177,7 +1178,9 @@ Shares choose_shares(int64_t units, int64_t keys, int D, int bits, int row_tile,
       for (int teams = 1; teams <= (peers % 8 == 0 ? max_teams : 1); ++teams) {
         const double x = static_cast<double>(units) * teams / fit, waves = 0.89 * std::ceil(x) + 0.11 * x;
         const double chain = waves * keys / (peers * teams) / rate[wide];
-        const double cost = (wide ? 1.9 : 0.0) + (peers > 1 ? 0.39 * peers : 0.0) + (teams > 1 ? kJoinCost : 0.0) + std::cbrt(all * all * all + chain * chain * chain);
+        const double fixed = (wide ? 1.9 : 0.0) + (peers > 1 ? 0.39 * peers : 0.0) + (teams > 1 ? kJoinCost : 0.0);
+        if (least >= 0.0 && fixed + std::max(all, chain) >= least) continue;   // (most; the root takes a short call's host longer than the rest)
+        const double cost = fixed + std::cbrt(all * all * all + chain * chain * chain);
         if (least < 0.0 || cost < least) {
           least = cost;
           best = Shares{peers, teams, wide != 0};

@@ -247,8 +247,8 @@ def _int32(name, t, batch: int, device) -> int:
 
 
 def _paged(cache: PagedKV, block_table, lengths, new_lengths, batch: int):
-    """(the cache as the library takes it, its 16-bit type, KV heads, head dimension, device); pointers are all that the library
-    sees, so types, shapes and devices are checked here."""
+    """(the cache as the library takes it, its 16-bit type, KV heads, head dimension, device, tokens that a row of the table has room
+    for); pointers are all that the library sees, so types, shapes and devices are checked here."""
     k, v, ks, vs = cache
     device, shape = k.device, k.shape
     if device.type != "cuda":
@@ -277,7 +277,7 @@ def _paged(cache: PagedKV, block_table, lengths, new_lengths, batch: int):
         k.data_ptr(), v.data_ptr(), ks_ptr, vs_ptr, block_table.data_ptr(), _int32("lengths", lengths, batch, device),
         _int32("new_lengths", new_lengths, batch, device) if new_lengths is not None else 0,
         pages, heads, page_size, width, batch, table_shape[1], block_table.stride(0), dtype_code(dtype), bits)
-    return packed, dtype, heads, width, device
+    return packed, dtype, heads, width, device, table_shape[1] * page_size
 
 
 def paged_append(k, v, cache: PagedKV, block_table, lengths, *, new_lengths=None, rotary=None, interleaved: bool = False, q=None,
@@ -293,7 +293,7 @@ def paged_append(k, v, cache: PagedKV, block_table, lengths, *, new_lengths=None
     page, length or position out of range (include/b200fa.h).
     """
     B, Hkv, S, D = k.shape
-    c, dtype, heads, head_dim, device = _paged(cache, block_table, lengths, new_lengths, B)
+    c, dtype, heads, head_dim, device, _ = _paged(cache, block_table, lengths, new_lengths, B)
     if D != head_dim or Hkv != heads or k.dtype is not dtype or k.device != device:
         raise ValueError(f"k and v have to be {dtype} of {heads} heads of {head_dim} on {device}")
     _same_kind(k, (v, q, q_out))
@@ -328,7 +328,7 @@ def paged_attention(q, cache: PagedKV, block_table, lengths, *, new_lengths=None
     elements keeps a KV head to one cluster).
     """
     B, Hq, S, D = q.shape
-    c, dtype, heads, head_dim, device = _paged(cache, block_table, lengths, new_lengths, B)
+    c, dtype, heads, head_dim, device, keys = _paged(cache, block_table, lengths, new_lengths, B)
     if D != head_dim or q.dtype is not dtype or q.device != device:
         raise ValueError(f"q has to be {dtype} of head dimension {head_dim} on {device}")
     if scale is None:
@@ -343,9 +343,9 @@ def paged_attention(q, cache: PagedKV, block_table, lengths, *, new_lengths=None
         _fp32_statistic(lse, (B, Hq, S), q.device)
     _same_kind(q, (out,))
     scratch = scratch_bytes = 0
-    if workspace is None and B * heads <= 64:   # (with more KV heads there is none)
-        keys = longest or block_table.shape[1] * cache.k.shape[2]
-        need = _lib.paged_attention_workspace_bytes(B, Hq, heads, S, D, min(keys, window + sinks + S) if window else keys)
+    if workspace is None and keys >= _lib.PAGED_TEAM_KEYS:
+        keys = min(keys, longest or keys, window + sinks + S if window else keys)
+        need = _lib.paged_attention_workspace_bytes(B, Hq, heads, S, D, keys)
         if need:
             workspace = torch.empty((need,), dtype=torch.uint8, device=device)
     if workspace is not None:
@@ -364,7 +364,7 @@ def paged_gather(cache: PagedKV, block_table, lengths, length: int, *, k=None, v
     """k, v = the first ``length`` tokens of every sequence, (B, Hkv, length, D) of the cache's 16-bit type; rows behind a
     sequence's own length are zero.  ``k`` and ``v``: tensors to write to."""
     B = lengths.shape[0]
-    c, dtype, heads, head_dim, device = _paged(cache, block_table, lengths, None, B)
+    c, dtype, heads, head_dim, device, _ = _paged(cache, block_table, lengths, None, B)
     shape = (B, heads, length, head_dim)
     if k is None:
         k = torch.empty(shape, dtype=dtype, device=device)
