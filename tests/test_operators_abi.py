@@ -239,3 +239,37 @@ def test_calls_of_few_keys_do_not_ask_for_a_workspace(monkeypatch):
     assert call(511) == [] == call(511, longest=100) == call(511, window=20)
     assert call(512) == [(2, 4, 2, 3, 64, 8192)] and call(600, longest=9000) == [(2, 4, 2, 3, 64, 9000)]
     assert call(600, longest=10000) == [(2, 4, 2, 3, 64, 9600)] and call(600, window=8200, sinks=4) == [(2, 4, 2, 3, 64, 8207)]
+
+
+@pytest.mark.parametrize("which", ["query", "key", "value", "rotary"])
+def test_a_paged_cache_refuses_tensors_that_want_gradients(host_backed_mojo, which, monkeypatch):
+    """Their gradients would be lost without a word: nothing goes back through the pages."""
+    import torch_mojo_backend_b200 as tmb
+
+    cache = tmb.PagedKVCache.__new__(tmb.PagedKVCache)   # (its pages are CUDA memory)
+    cache.kv = cache._status = None
+    reached = []
+    monkeypatch.setattr(raw, "paged_append", lambda *a, **how: reached.append("append"))
+    monkeypatch.setattr(raw, "paged_attention", lambda *a, **how: reached.append("attention") or (torch.zeros(1), torch.zeros(1)))
+    monkeypatch.setattr(tmb.PagedKVCache.attention.__globals__["TorchMojoTensor"], "_from_cuda", staticmethod(lambda t: t))
+    make = lambda *shape, want=False: torch.zeros(*shape).to("mojo").requires_grad_(want)   # noqa: E731
+    i = torch.zeros(1, 1, dtype=torch.int32).to("mojo")
+    q, k, v = (make(1, 2, 1, 64, want=which == n) for n in ("query", "key", "value"))
+    angles = make(16, 32, want=which == "rotary"), make(16, 32)
+
+    def calls():
+        cache.append(k, v, i, i, rotary=angles, query=q)
+        if which == "query":
+            cache.attention(q, i, i)
+
+    with pytest.raises(NotImplementedError, match=f"{which} requires a gradient"):
+        cache.append(k, v, i, i, rotary=angles, query=q)
+    if which == "query":
+        with pytest.raises(NotImplementedError, match="query requires a gradient"):
+            cache.attention(q, i, i)
+    assert reached == []
+    with torch.no_grad():
+        calls()
+    with torch.inference_mode():
+        calls()
+    assert reached == (["append", "attention"] if which == "query" else ["append"]) * 2

@@ -22,6 +22,8 @@ def _cuda(name: str, t):
     held = payload(t)
     if held is None:
         raise RuntimeError(f"PagedKVCache: {name} has to be a mojo tensor, got {type(t).__name__}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(f"PagedKVCache: {name} requires a gradient, and nothing goes back through a cache; call it under torch.no_grad()")
     return held._cuda_view()
 
 
@@ -44,7 +46,8 @@ class PagedKVCache:
     elements.  Which pages a sequence has is the caller's: every call takes the ``block_table`` (B, pages of a sequence) and the
     ``lengths`` (B,), int32 mojo tensors that are read on the device (``raw.paged_append`` says how, and what ``new_lengths``
     are).  A call is safe beside others on other streams as long as no two write, or one writes and another reads, the same
-    places; it keeps no workspace (a call's own scratch is allocated on the stream it runs on).
+    places; it keeps no workspace (a call's own scratch is allocated on the stream it runs on).  Nothing is differentiated: where gradients
+    are recorded, a tensor that requires one is refused (``NotImplementedError``).
     """
 
     def __init__(self, pages: int, kv_heads: int, page_size: int, head_dim: int, *, dtype=torch.bfloat16, bits: int = 16,
@@ -75,7 +78,7 @@ class PagedKVCache:
 
     def attention(self, query, block_table, lengths, *, new_lengths=None, window: int = 0, sinks: int = 0, scale: float | None = None,
                   longest: int = 0, return_lse: bool = False):
-        """Causal attention of the newest tokens' ``query`` (B, Hq, S, D) over the pages; not differentiable."""
+        """Causal attention of the newest tokens' ``query`` (B, Hq, S, D) over the pages."""
         out, lse = raw.paged_attention(_cuda("query", query), self.kv, _cuda("block_table", block_table), _cuda("lengths", lengths),
                                        new_lengths=_cuda("new_lengths", new_lengths), window=window, sinks=sinks, scale=scale,
                                        longest=longest, status=self._status)
