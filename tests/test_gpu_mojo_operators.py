@@ -286,3 +286,35 @@ def test_a_captured_backward_that_fails_or_ends_on_another_thread(fails):
         got, streams = step(call)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, ref)) and streams == [torch.cuda.default_stream()]
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_paged_cache_on_a_side_stream(bits):
+    """append, attention and gather are ordered on the current stream, whatever the default one is doing."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    lengths = torch.tensor([9000, 700], dtype=torch.int32)
+    table = torch.arange(2 * 141, dtype=torch.int32).view(2, 141)
+    q, k, v = (torch.randn(2, h, 9000, 64, generator=g, device="cuda").bfloat16() for h in (2, 1, 1))
+    row = torch.randn(2, 2, 1, 64, generator=g, device="cuda").bfloat16()
+    busy = torch.ones(8192, 8192, device="cuda")
+
+    def run():
+        cache = tmb.PagedKVCache(2 * 141, 1, 64, 64, bits=bits)
+        m = [t.to("mojo") for t in (table, lengths)]
+        cache.append(tmb.from_cuda(k), tmb.from_cuda(v), *m, new_lengths=m[1])
+        out, lse = cache.attention(tmb.from_cuda(row), *m, return_lse=True)   # (its workspace is the stream's too)
+        return [tmb.to_cuda(t) for t in (out, lse, *cache.gather(*m, 9000))]
+
+    want = run()
+    torch.mojo.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for on in (side, torch.cuda.default_stream()):   # the stream that is behind
+        with torch.cuda.stream(on):
+            for _ in range(4):
+                busy @ busy
+        with torch.cuda.stream(side):
+            got = run()
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    torch.mojo.synchronize()

@@ -210,3 +210,13 @@ def test_a_call_is_ordered_on_its_stream_and_can_be_captured():
     want = run_both(q2, k2, v2, grad2, TL, 200, 4)
     for n, t in (("out", out), ("lse", lse), ("dq", dq), ("dk", dk), ("dv", dv)):
         assert torch.equal(want[n], t), n
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq,Sk,window,sinks", [(1, 1, 1, 0), (1, 129, 128, 0), (1, 1000, 100, 3), (1, 5000, 5001, 0), (2, 777, 1, 1), (5, 640, 130, 200)])
+def test_few_rows_against_a_longer_key_sequence(Sq, Sk, window, sinks, D, dtype):
+    q, k, v, grad = inputs(12, 2, 4, 2, Sq, Sk, D, dtype)
+    got = run_both(q, k, v, grad, BR, window, sinks)
+    for name, (want, bound) in reference(q, k, v, grad, BR, window, sinks).items():
+        check(name, got[name], want, bound)
