@@ -159,9 +159,9 @@ void b200fa_dropout_bytes_host(uint64_t philox_seed, uint64_t philox_offset, int
  * (i, or i + Sk - Sq), the row sees key j iff j <= p and (j > p - window or j < sinks).  window >= 1, sinks >= 0; a window of
  * Sk + Sq keys is the causal mask.  Otherwise the contracts of b200fa_fwd and b200fa_bwd: out, lse, gradients, types,
  * lengths, strides, rows that see no key.  Work goes with the keys that are seen: blocks of 128 keys that no row of a
- * tile sees are not visited.  Blocks that are visited have to hold finite values of v also where the mask hides them (0 * inf
- * is NaN in every kernel that multiplies whole tiles).  bf16 and fp16 run the tcgen05 kernels; fp32 runs FMA kernels, both
- * directions, so that a forward's out and lse fit the backward.
+ * tile sees are not visited.  Blocks that are visited have to hold finite values also where the mask hides them (0 * inf
+ * is NaN in every kernel that multiplies whole tiles): v in the forward, q, k, v and dout in the backward.  bf16 and fp16 run the
+ * tcgen05 kernels; fp32 runs FMA kernels in both directions.
  * `workspace` of the backward: b200fa_window_bwd_workspace_bytes(...) bytes of caller-owned device scratch, 256-byte aligned,
  * contents irrelevant (the row statistics of b200fa_bwd and, where the query rows of a K/V tile with sinks in it are shared
  * by several blocks, their fp32 sums); calls that overlap on the GPU need workspaces of their own.  No counterpart in the

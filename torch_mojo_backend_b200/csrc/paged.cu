@@ -73,8 +73,8 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
 // then to the type, so that the results are those of the formula in fp32 whatever computes it.  Copy-bound: each element is
 // read and written once.  A row of 4 bits: scale = (max - min) / 15 rounded to the type, code = round((x - min) / scale), of the
 // elements as rounded to the type.  Where an element of a group is not finite the scale is NaN, and so is the group.
-// B200, one row a thread / this: 6 prompts of up to 1500 tokens, 16 + 4 heads, D = 64, 4 bits: 21 / 12.9 us, most of it by the
-// reciprocal; 64 single tokens, 32 + 8 heads, D = 128, 16 bits: 2.8 us.
+// B200, one row a thread / this: 6 prompts of up to 1500 tokens, 16 + 4 heads, D = 64, 4 bits: 21 / 12-13 us, most of it by the
+// reciprocal; 64 single tokens, 32 + 8 heads, D = 128, 16 bits: 2.4 us.
 // ------------------------------------------------------------------------------------------
 template <typename T, int kD>
 struct AppendCfg {
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const AppendParams p)
 
 // ------------------------------------------------------------------------------------------
 // Reading back.  D / 8 lanes take a row of k and the same row of v; rows behind a sequence's last are zero.  Copy-bound:
-// four sequences of up to 16896 tokens, 8 KV heads, D = 128, 16 bits: 84 us, 6.26 TB/s of what is read and written.
+// four sequences of up to 16896 tokens, 8 KV heads, D = 128, 16 bits: 84 us, 6.3 TB/s of what is read and written.
 // ------------------------------------------------------------------------------------------
 template <typename T, int kD, int kBits>
 __global__ void __launch_bounds__(256) paged_gather_kernel(const GatherParams p) {
@@ -321,9 +321,10 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(const GatherParams p)
 //     0..15 instead would make both sums several times their difference, and the rounding of P vs_G with them.)
 // The row maximum moves only when a score exceeds it by 2^8 (a vote per step instead of six shuffles), so P is at most 256; at
 // most 4 where P vs_G is an fp16, whose largest scale is 8734.
-// B200, decode of one token, 8 KV heads, groups of 4, D = 128, bf16: 8 sequences of up to 32768 keys (spread 60 %), 16 bits: 134 us,
-// 0.91 of the copy rate; 16 of up to 32768 (spread 30 %), 4 bits: 165 us, 0.53 of it.  The 4-bit kernel is bound by issue: about
-// 430 instructions for 16 keys of a head, the logic unit at 55 % of its peak.  (16 bits by bulk copies into rings: no better.)
+// B200, decode of one token, 8 KV heads, groups of 4, D = 128, bf16: 8 sequences of up to 32768 keys (spread 60 %), 16 bits: 136 us,
+// 0.89 of the copy rate; 16 of up to 32768 (spread 30 %), 4 bits: 170-174 us, 0.51-0.52 of it.  The 4-bit kernel is bound by issue:
+// about 420 instructions for 16 keys of a head, 61 % of the issue slots and the logic unit at 59 % of its peak while an SM is busy, which is
+// 80 % of the time.  (16 bits by bulk copies into rings: no better.)
 // Keys that no row of the unit sees are never read, not even into a product with zero: their places in a step re-read a key that is
 // seen (pages behind a window may have been given to another sequence).
 // ------------------------------------------------------------------------------------------
