@@ -28,7 +28,7 @@ def _cuda(name: str, t):
 def _refuse_gradients(names, tensors) -> None:
     """Asked only where gradients are recorded: 0.3 us a tensor on the host."""
     for i, t in enumerate(tensors):
-        if t is not None and t.requires_grad:
+        if getattr(t, "requires_grad", False):
             name = names[min(i, len(names) - 1)]
             raise NotImplementedError(f"PagedKVCache: {name} requires a gradient, and nothing goes back through a cache; call it under torch.no_grad()")
 

@@ -76,9 +76,11 @@ def _on_stream(stream):
     if current == stream:
         yield
         return
-    lend = not torch.cuda.is_current_stream_capturing()
     with torch.cuda.stream(stream):
-        lend = lend and torch.cuda.is_current_stream_capturing()
+        lend = torch.cuda.is_current_stream_capturing()
+        if lend:
+            with torch.cuda.stream(current):
+                lend = not torch.cuda.is_current_stream_capturing()
         if not lend:
             stream.wait_stream(current)
         yield
