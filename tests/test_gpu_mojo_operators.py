@@ -318,3 +318,24 @@ def test_paged_cache_on_a_side_stream(bits):
         side.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     torch.mojo.synchronize()
+
+
+def test_a_bad_index_does_not_end_a_host_pass():
+    """The pipeline answers for its own kernels; an index out of range of a paged call is told by the device's synchronize."""
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (tmb.pinned_empty((2, 2, 300, 64), torch.bfloat16) for _ in range(3))
+    for t in (q, k, v):
+        t.copy_(torch.randn(t.shape, generator=g).bfloat16())
+    pipe = tmb.HostAttentionPipeline(0, piece_bytes=1 << 20)
+    want = pipe.run(q, k, v, is_causal=True)[0]
+    pipe.synchronize()
+    want = want.clone()
+    cache = tmb.PagedKVCache(2, 1, 16, 64)
+    i = torch.full((1, 1), 9, dtype=torch.int32).to("mojo")
+    cache.attention(torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16).to("mojo"), i, torch.ones(1, dtype=torch.int32).to("mojo"))
+    got = pipe.run(q, k, v, is_causal=True)[0]
+    pipe.synchronize()
+    assert torch.equal(got, want)
+    with pytest.raises(_lib.B200FAError) as err:
+        torch.mojo.synchronize()
+    assert err.value.code == _lib.ERR_BAD_INDEX

@@ -273,3 +273,20 @@ def test_a_paged_cache_refuses_tensors_that_want_gradients(host_backed_mojo, whi
     with torch.inference_mode():
         calls()
     assert reached == (["append", "attention"] if which == "query" else ["append"]) * 2
+
+
+def test_a_bad_index_waits_for_the_check_that_asks_for_it(host_backed_mojo):
+    from torch_mojo_backend_b200 import flash_ops
+
+    word = flash_ops._status_words[0]._cuda_view()
+    word.fill_(0x42490006)
+    flash_ops.check_status(0, bad_index=False)       # (what the host pipeline asks)
+    with pytest.raises(_lib.B200FAError) as err:
+        flash_ops.check_status(0)
+    assert err.value.code == _lib.ERR_BAD_INDEX
+    flash_ops.check_status(0)
+    word.fill_(0x57410320)
+    with pytest.raises(_lib.B200FAError) as err:
+        flash_ops.check_status(0, bad_index=False)
+    assert err.value.code == _lib.ERR_TIMEOUT
+    flash_ops.check_status(0)

@@ -73,19 +73,20 @@ def _status_ptr(index: int) -> int:
     return word._ptr
 
 
-def check_status(index: int | None = None) -> None:
+def check_status(index: int | None = None, bad_index: bool = True) -> None:
     """Synchronise with the device and raise ``B200FAError(ERR_TIMEOUT)`` if a kernel launched
     through the mojo ops gave up on an internal wait since the last check (its outputs are then
-    not to be trusted).  The word is cleared, so the next call starts clean."""
+    not to be trusted), or ``ERR_BAD_INDEX`` if a paged call was given an index out of range.  The word is cleared, so the next call
+    starts clean.  ``bad_index`` False: the latter is left for the next check; it concerns no other call."""
     indices = list(_status_words) if index is None else [index]
     for i in indices:
         word = _status_words.get(i)
         if word is None:
             continue
         value = int(word._cuda_view().item()) & 0xFFFFFFFF   # synchronises
-        if value:
+        rc = _lib.status_to_error(value)
+        if rc != _lib.OK and (bad_index or rc != _lib.ERR_BAD_INDEX):
             word._cuda_view().zero_()
-            rc = _lib.status_to_error(value)
             raise _lib.B200FAError(rc, f"a mojo flash-attention kernel reported status 0x{value:08x}")
 
 
