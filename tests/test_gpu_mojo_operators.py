@@ -339,3 +339,31 @@ def test_a_bad_index_does_not_end_a_host_pass():
     with pytest.raises(_lib.B200FAError) as err:
         torch.mojo.synchronize()
     assert err.value.code == _lib.ERR_BAD_INDEX
+
+
+@pytest.mark.parametrize("how", ["window", "paged", "dense"])
+def test_a_first_call_in_a_capture(how, monkeypatch):
+    """The device's status word is there before: the graph neither makes it nor wipes what was reported."""
+    from torch_mojo_backend_b200 import flash_ops, tensor
+
+    q, k, v, _ = inputs(10, 1, 2, 2, 256, 256, 64, torch.bfloat16)
+    words = {}
+    monkeypatch.setattr(flash_ops, "_status_words", words)
+    monkeypatch.setattr(tensor, "_used", set(), raising=False)
+    t = [tmb.from_cuda(x) for x in (q, k, v)]
+    cache = tmb.PagedKVCache(4, 2, 16, 64)
+    cache.kv.k.zero_(), cache.kv.v.zero_()
+    table, lengths = (tmb.from_cuda(torch.tensor(x, dtype=torch.int32, device="cuda")) for x in ([[0, 1, 2, 3]], [50]))
+    row = tmb.from_cuda(q[:, :, :1].contiguous())
+    call = {"window": lambda: tmb.window_attention(*t, 30), "paged": lambda: cache.attention(row, table, lengths),
+            "dense": lambda: torch.nn.functional.scaled_dot_product_attention(*t, is_causal=True)}[how]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    word = words[0]._cuda_view()
+    word.fill_(0x42490001)
+    graph.replay()
+    assert int(word) == 0x42490001
+    word.zero_()
+    assert torch.equal(tmb.to_cuda(out), tmb.to_cuda(call()))
+    torch.mojo.synchronize()

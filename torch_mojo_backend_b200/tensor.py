@@ -128,10 +128,26 @@ def take_back_stream(over: bool = False) -> None:
             torch.cuda.set_stream(own)
 
 
+#: devices that have had a tensor
+_used: set[int] = set()
+
+
+def _first_use(index: int) -> None:
+    """Sets up the device's status word with its first tensor: made by a first call in a capture, it would be the graph's, zeroed by each
+    replay and not before the first."""
+    if torch.cuda.is_available() and not torch.cuda.is_current_stream_capturing():
+        from . import flash_ops
+
+        _used.add(index)
+        flash_ops._status_ptr(index)
+
+
 def _alloc_holder(nbytes: int, index: int) -> torch.Tensor:
     """One device allocation: a flat byte buffer on CUDA device `index` (never zero bytes)."""
     if _lent:
         take_back_stream()
+    if index not in _used:
+        _first_use(index)
     return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=_cuda_device(index))
 
 
@@ -220,7 +236,10 @@ class TorchMojoTensor(torch.Tensor):
         if t.device.type != "cuda":
             raise RuntimeError(f"_from_cuda needs a CUDA tensor, got {t.device}")
         t = t.detach()
-        return cls._make(t, t.data_ptr(), tuple(t.shape), tuple(t.stride()), 0, t.dtype, t.device.index or 0)
+        index = t.device.index or 0
+        if index not in _used:
+            _first_use(index)
+        return cls._make(t, t.data_ptr(), tuple(t.shape), tuple(t.stride()), 0, t.dtype, index)
 
     @classmethod
     def _from_cpu(cls, cpu_tensor: torch.Tensor, index: int | None = None, *, non_blocking: bool = False):
